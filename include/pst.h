@@ -226,6 +226,61 @@ int pst_decoder_set_timing(pst_decoder* dec, int32_t enable);
 int pst_decoder_get_timing(pst_decoder* dec, float* ms);
 
 /*
+ * Token head: operators over a learned table weight [V, d] with one row per token id (the codes of a codebook and,
+ * usually, a few marks), for a sequence model over the ids that pst_tokenize makes; pst_codebook_aux gives the same
+ * kind of scores over the implicit codebook. Matrices are row-major with unit column stride and row strides ld_* in
+ * elements (any stride >= the row's length, any alignment of the type; 16-byte aligned rows of a multiple of 8 (16:
+ * int8) elements are read in place, others are copied into the workspace first). No context: a call names its device and
+ * launches on `stream` (a hipStream_t of that device, NULL = its default stream) without synchronising, so it can be
+ * captured into a graph; the calling thread's current device stays what it was. Calls on different streams or threads
+ * are independent as long as they use different workspaces (a captured graph keeps the one it was captured with).
+ * pst_head_error: the message of the calling thread's last failed call of this section.
+ */
+enum { PST_F32 = 0, PST_BF16 = 1, PST_F16 = 2 };
+const char* pst_head_error(void);
+
+/*
+ * Softmax cross entropy of each position over the vocabulary, without the logits in memory:
+ *   lse[n] = log sum_v exp(<hidden[n], weight[v]>),  loss[n] = lse[n] - <hidden[n], weight[targets[n]]>
+ *   hidden [rows, width], weight [vocab, width]  of `type` (products of 16-bit types are exact, sums 32-bit)
+ *   targets [rows]  int32 or int64 (target_bits; uint32 token ids below 2^31 are int32 ids). Positions whose target is
+ *                   `ignore` have loss 0; a target outside [0, vocab) that is not `ignore` gives loss NaN.
+ *   loss, lse [rows] f32 (lse of ignored positions too)
+ * rows = 0 writes nothing. *_workspace: bytes of the 256-byte aligned device workspace that a call with these
+ * arguments needs (negative: PST_E_*).
+ */
+int64_t pst_token_loss_workspace(int32_t type, const void* d_hidden, int64_t ld_hidden, const void* d_weight, int64_t ld_weight,
+                                 int64_t rows, int64_t vocab, int64_t width);
+int pst_token_loss(int32_t device, int32_t type, const void* d_hidden, int64_t ld_hidden, const void* d_weight, int64_t ld_weight,
+                   int64_t rows, int64_t vocab, int64_t width, const void* d_targets, int32_t target_bits, int64_t ignore,
+                   float* d_loss, float* d_lse, void* d_workspace, int64_t workspace_bytes, void* stream);
+/*
+ * Gradients of sum_n grad_loss[n] loss[n] for hidden and weight (either may be NULL), of the operands' type, from the
+ * lse of pst_token_loss. Ignored positions have zero gradient and add nothing to the weight's, whatever their hidden
+ * row holds. A target out of range makes its position's gradient, and the weight's, NaN. rows = 0 writes a zero weight
+ * gradient. No atomics: the same inputs give the same bits.
+ */
+int64_t pst_token_loss_grad_workspace(int32_t type, const void* d_hidden, int64_t ld_hidden, const void* d_weight, int64_t ld_weight,
+                                      int64_t rows, int64_t vocab, int64_t width);
+int pst_token_loss_grad(int32_t device, int32_t type, const void* d_hidden, int64_t ld_hidden, const void* d_weight, int64_t ld_weight,
+                        int64_t rows, int64_t vocab, int64_t width, const void* d_targets, int32_t target_bits, int64_t ignore,
+                        const float* d_lse, const float* d_grad_loss, void* d_grad_hidden, int64_t ld_grad_hidden, void* d_grad_weight,
+                        int64_t ld_grad_weight, void* d_workspace, int64_t workspace_bytes, void* stream);
+/*
+ * Scores in 8-bit integers: scores[n, v] = s_n * scale[v] * sum_k q[n, k] weight[v, k], where hidden's row n is rounded
+ * to q[n, k] = rint(hidden[n, k] / s_n), s_n = max_k |hidden[n, k]| * (1.0f / 127), within the call; sums are 32-bit integers
+ * (width <= 131072) and exact. weight [vocab, width] int8 and scale [vocab] f32 are pst_quantize_rows of the table, laid
+ * out once. scores [rows, vocab] of out_type. A row of zeros scores 0; one that holds an infinity or NaN scores NaN.
+ */
+int pst_quantize_rows(int32_t device, int32_t type, const void* d_x, int64_t ld_x, int64_t rows, int64_t width, int8_t* d_q,
+                      int64_t ld_q, float* d_scale, void* stream);
+int64_t pst_token_scores_i8_workspace(int32_t type, const void* d_hidden, int64_t ld_hidden, const int8_t* d_weight, int64_t ld_weight,
+                                      int64_t rows, int64_t vocab, int64_t width);
+int pst_token_scores_i8(int32_t device, int32_t type, const void* d_hidden, int64_t ld_hidden, const int8_t* d_weight,
+                        int64_t ld_weight, const float* d_weight_scale, int64_t rows, int64_t vocab, int64_t width, int32_t out_type,
+                        void* d_scores, int64_t ld_scores, void* d_workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * Native PDB parsing (host, no GPU): replaces protein_structure_from_pdb_string
  * (structure_tokenizer/data/protein_structure_sample.py:166-248, Biopython PDBParser semantics,
  * restated in pst_amd/pdb.py) for make_graph_from_pdb (scripts/inference_runner.py:47-50).

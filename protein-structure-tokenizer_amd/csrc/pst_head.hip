@@ -1,0 +1,1096 @@
+// pst_head.hip — the token head: operators over a learned table weight [V, d], one row per token id.
+//
+//   token loss        lse[n] = log sum_v exp(<x_n, w_v>), loss[n] = lse[n] - <x_n, w_t>     (t = target of n)
+//   its gradient      D[n][v] = g_n (exp(<x_n, w_v> - lse_n) - [v = t]),  dx = D W,  dW = D^T x
+//   8-bit scores      s_n s_v sum_k q_nk q_vk, q_nk = rint(x_nk / s_n), s_n = max_k |x_nk| * (1/127)
+//
+// The logits never reach memory: the loss keeps per tile of the vocabulary a running maximum and sum for each
+// row (k_loss) and joins them (k_join); the gradient makes D for a piece of the vocabulary at a time, in 16 bits
+// in a workspace that the last-level cache holds, and multiplies it in both directions from there.
+//
+// 32-bit inputs: each value is split into two 16-bit floats (hi + lo, 22 bits of mantissa) after a scaling of
+// the whole tensor by a power of two, and a product is the three passes lo hi + hi lo + hi hi on the 16-bit
+// matrix cores: about 2^-22 of the operands' product, at three sixteenths of the 32-bit instructions' time.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <new>
+#include <string>
+
+#include "../../include/pst.h"
+#include "pst_head_gemm.h"
+
+namespace pst_head {
+namespace {
+
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr int AMAX_BLOCKS = 256;
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+__device__ __forceinline__ float load1(const void* p, int type, int64_t i) {
+  if (type == PST_F32) return ((const float*)p)[i];
+  if (type == PST_BF16) return __uint_as_float((uint32_t)((const uint16_t*)p)[i] << 16);
+  return (float)((const _Float16*)p)[i];
+}
+__device__ __forceinline__ uint32_t bits16(float v, int type) {
+  if (type == PST_BF16) return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)v);
+  return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v);
+}
+// four neighbours of an output row, `n` of them valid
+__device__ __forceinline__ void store4(void* p, int type, int64_t i, const float* v, int n, bool wide) {
+  if (type == PST_F32) {
+    float* q = (float*)p + i;
+    if (wide && n >= 4) {
+      *(f32x4*)q = (f32x4){v[0], v[1], v[2], v[3]};
+    } else {
+      for (int j = 0; j < 4; ++j)
+        if (j < n) q[j] = v[j];
+    }
+  } else {
+    uint16_t* q = (uint16_t*)p + i;
+    const uint32_t a = bits16(v[0], type) | bits16(v[1], type) << 16, b = bits16(v[2], type) | bits16(v[3], type) << 16;
+    if (wide && n >= 4) {
+      *(uint2*)q = make_uint2(a, b);
+    } else {
+      for (int j = 0; j < 4; ++j)
+        if (j < n) q[j] = (uint16_t)(j < 2 ? a >> (16 * j) : b >> (16 * (j - 2)));
+    }
+  }
+}
+
+struct Targets {
+  const void* p;
+  int64_t ignore;
+  int32_t bits;   // 32 or 64
+  int32_t vocab;
+};
+// the target row, -1 where there is none to find (ignored, or out of range), and whether the position counts
+__device__ __forceinline__ int target_of(const Targets& t, int64_t n, bool& counts) {
+  const int64_t v = t.bits == 64 ? ((const int64_t*)t.p)[n] : (int64_t)((const int32_t*)t.p)[n];
+  counts = v != t.ignore;
+  return counts && v >= 0 && v < t.vocab ? (int)v : -1;
+}
+
+// ------------------------------------------------------------------ 32-bit operands: scaling and splitting
+__device__ __forceinline__ float finite_abs(float v) {
+  v = fabsf(v);
+  return v <= 3.4028234663852886e38f ? v : 0.0f;
+}
+// 2^e with max |x| 2^e in [2^13, 2^14): both halves of a product stay inside the 16-bit range
+__device__ __forceinline__ int split_exp(float amax) { return amax > 0.0f ? 13 - ilogbf(amax) : 0; }
+
+struct AmaxArgs {
+  const float* p[2];
+  int64_t ld[2];
+  int64_t rows[2];
+  int32_t width;
+  float* part;  // [2][AMAX_BLOCKS]
+};
+__global__ __launch_bounds__(256) void k_amax(AmaxArgs a) {
+  const int t = blockIdx.x / AMAX_BLOCKS, b = blockIdx.x % AMAX_BLOCKS;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float m = 0.0f;
+  for (int64_t r = b * 4 + wave; r < a.rows[t]; r += AMAX_BLOCKS * 4) {
+    const float* row = a.p[t] + r * a.ld[t];
+    for (int k = lane; k < a.width; k += 64) m = fmaxf(m, finite_abs(row[k]));
+  }
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
+  __shared__ float sm[4];
+  if (lane == 0) sm[wave] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) a.part[t * AMAX_BLOCKS + b] = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+}
+
+struct PackArgs {
+  const void* src;
+  int64_t ld;
+  int64_t rows, rows_pad;  // rows beyond `rows` are zeros
+  int32_t width, width_pad;
+  int32_t type;
+  char* dst;               // 16-bit [planes][rows_pad][width_pad]
+  int64_t plane;           // bytes
+  const float* part;       // 32-bit: the tensor's AMAX_BLOCKS maxima
+  float* unscale;          // 32-bit: 2^-e
+  Targets targets;         // p set: rows whose position does not count are zeros
+};
+// copies a matrix into rows of whole K-steps (zeros behind), splitting 32-bit values
+__global__ __launch_bounds__(256) void k_pack(PackArgs a) {
+  const int64_t groups = (int64_t)a.rows_pad * (a.width_pad / 8);
+  int e = 0;
+  if (a.type == PST_F32) {
+    float m = a.part[threadIdx.x];
+#pragma unroll
+    for (int s = 32; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
+    __shared__ float sm[4];
+    if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
+    __syncthreads();
+    e = split_exp(fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3])));
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.unscale = ldexpf(1.0f, -e);
+  }
+  for (int64_t g = blockIdx.x * (int64_t)256 + threadIdx.x; g < groups; g += (int64_t)gridDim.x * 256) {
+    const int64_t r = g / (a.width_pad / 8);
+    const int c = (int)(g - r * (a.width_pad / 8)) * 8;
+    bool keep = r < a.rows;
+    if (keep && a.targets.p) (void)target_of(a.targets, r, keep);
+    uint32_t hi[8], lo[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      hi[j] = lo[j] = 0;
+      if (keep && c + j < a.width) {
+        if (a.type == PST_F32) {
+          const float v = ldexpf(((const float*)a.src)[r * a.ld + c + j], e);
+          const _Float16 h = (_Float16)v;
+          hi[j] = __builtin_bit_cast(uint16_t, h);
+          // an infinity or NaN stands in hi alone
+          const float rest = fabsf(v) <= 65504.0f ? v - (float)h : 0.0f;
+          lo[j] = __builtin_bit_cast(uint16_t, (_Float16)rest);
+        } else {
+          hi[j] = ((const uint16_t*)a.src)[r * a.ld + c + j];
+        }
+      }
+    }
+    char* d = a.dst + (r * a.width_pad + c) * 2;
+    *(uint4*)d = make_uint4(hi[0] | hi[1] << 16, hi[2] | hi[3] << 16, hi[4] | hi[5] << 16, hi[6] | hi[7] << 16);
+    if (a.type == PST_F32)
+      *(uint4*)(d + a.plane) = make_uint4(lo[0] | lo[1] << 16, lo[2] | lo[3] << 16, lo[4] | lo[5] << 16, lo[6] | lo[7] << 16);
+  }
+}
+
+// ------------------------------------------------------------------ products with their epilogues
+struct GemmArgs {
+  Operand A, B;
+  KLoop k;
+  int32_t M, N;        // rows of A and of B that exist
+  int32_t nm, nn, nz;  // tiles along m and n, pieces of the K loop
+  int32_t steps;       // K-steps of the whole range
+  int32_t gm;
+  // unscaling of 32-bit operands (device; null: 1)
+  const float *ua, *ub;
+  // loss and logit gradient: n = position, m = vocabulary row (from v0)
+  Targets targets;
+  float2* part;        // loss: [nm][N] (maximum, sum)
+  float* tlogit;       // loss: [N]
+  const float *lse, *gloss;
+  const float* gscale; // power of two on D (device)
+  char* D;             // [planes][rows][ldd] 16-bit
+  int64_t dplane, ldd; // bytes, elements
+  int32_t dtype, dplanes, v0;
+  // matrix outputs
+  void* out;
+  int64_t ldo;
+  int32_t otype, wide, add;
+  int64_t zstride;     // dx: elements between the pieces' partial sums
+  const float *sn, *sm; // scores: scales of the rows of B and of A
+};
+
+enum Kind { LOSS, DLOGIT, DX, DW, SCORES };
+
+template <class T>
+struct Place {
+  int m0, n0, z, lane, h, col, mw, nw;  // mw, nw: this wave's first row and column
+  __device__ __forceinline__ Place(const GemmArgs& g) {
+    int m, n;
+    place(blockIdx.x, g.nm * g.nn * g.nz, g.nm, g.nn, g.gm, m, n, z);
+    m0 = m * T::BM;
+    n0 = n * T::BN;
+    lane = threadIdx.x & 63;
+    h = lane >> 5;
+    col = lane & 31;
+    const int wave = threadIdx.x >> 6;
+    mw = m0 + (wave / T::WN) * T::MI * 32;
+    nw = n0 + (wave % T::WN) * T::NI * 32;
+  }
+};
+
+template <int E, class T>
+__global__ __launch_bounds__(T::THREADS) void k_loss(GemmArgs g) {
+  extern __shared__ char smem[];
+  const Place<T> p(g);
+  typename Mma<E>::Acc acc[T::MI][T::NI];
+  multiply<E, T, false, false>(acc, g.A, g.B, g.k, p.m0, p.n0, 0, g.steps, smem);
+  const float mul = g.ua ? *g.ua * *g.ub : 1.0f;
+  float2* sm = (float2*)smem;  // [WM][BN]
+#pragma unroll
+  for (int j = 0; j < T::NI; ++j) {
+    const int n = p.nw + 32 * j + p.col;
+    float mx = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < T::MI; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int m = p.mw + 32 * i + 8 * (r >> 2) + 4 * p.h + (r & 3);
+        float v = acc[i][j][r] * mul;
+        v = m < g.M ? v : -__builtin_inff();
+        acc[i][j][r] = v;
+        mx = fmaxf(mx, v);
+      }
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    const float base = mx == -__builtin_inff() ? 0.0f : mx * LOG2E;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < T::MI; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sum += exp2_fast(__builtin_fmaf(acc[i][j][r], LOG2E, -base));
+    sum += __shfl_xor(sum, 32);
+    // the target's logit, where it is among this wave's rows
+    bool counts = false;
+    const int t = n < g.N ? target_of(g.targets, n, counts) : -1;
+    const int at = t - p.mw;
+    if (__any(t >= 0 && at >= 0 && at < T::MI * 32)) {
+#pragma unroll
+      for (int i = 0; i < T::MI; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (t >= 0 && at == 32 * i + 8 * (r >> 2) + 4 * p.h + (r & 3)) g.tlogit[n] = acc[i][j][r];
+    }
+    if (p.h == 0) sm[((threadIdx.x >> 6) / T::WN) * T::BN + (n - p.n0)] = make_float2(mx, sum);
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < T::BN; c += T::THREADS) {
+    if (p.n0 + c >= g.N) continue;
+    float2 a = sm[c];
+    for (int w = 1; w < T::WM; ++w) {
+      const float2 b = sm[w * T::BN + c];
+      const float mx = fmaxf(a.x, b.x);
+      const float safe = mx == -__builtin_inff() ? 0.0f : mx;
+      a.y = a.y * exp2_fast((a.x - safe) * LOG2E) + b.y * exp2_fast((b.x - safe) * LOG2E);
+      a.x = mx;
+    }
+    g.part[(int64_t)(p.m0 / T::BM) * g.N + p.n0 + c] = a;
+  }
+}
+
+struct JoinArgs {
+  const float2* part;
+  const float* tlogit;
+  Targets targets;
+  float *loss, *lse;
+  int32_t n, tiles;
+};
+// 16 waves share the vocabulary tiles of 64 positions
+__global__ __launch_bounds__(1024) void k_join(JoinArgs a) {
+  __shared__ float2 sm[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int n = blockIdx.x * 64 + lane;
+  float mx = -__builtin_inff(), sum = 0.0f;
+  if (n < a.n)
+    for (int t = wave; t < a.tiles; t += 16) {
+      const float2 q = a.part[(int64_t)t * a.n + n];
+      const float m2 = fmaxf(mx, q.x);
+      const float safe = m2 == -__builtin_inff() ? 0.0f : m2;
+      sum = sum * exp2_fast((mx - safe) * LOG2E) + q.y * exp2_fast((q.x - safe) * LOG2E);
+      mx = m2;
+    }
+  sm[wave][lane] = make_float2(mx, sum);
+  __syncthreads();
+  if (wave != 0 || n >= a.n) return;
+  float top = sm[0][lane].x;
+  for (int w = 1; w < 16; ++w) top = fmaxf(top, sm[w][lane].x);
+  const float safe = top == -__builtin_inff() ? 0.0f : top;
+  float s = 0.0f;
+  for (int w = 0; w < 16; ++w) s += sm[w][lane].y * exp2_fast((sm[w][lane].x - safe) * LOG2E);
+  const float lse = safe + logf(s);
+  bool counts;
+  const int t = target_of(a.targets, n, counts);
+  a.lse[n] = lse;
+  a.loss[n] = !counts ? 0.0f : t < 0 ? __builtin_nanf("") : lse - a.tlogit[n];
+}
+
+// D of one piece of the vocabulary (columns v0 ...; zeros behind the last row and for positions that do not count)
+template <int E, class T>
+__global__ __launch_bounds__(T::THREADS) void k_dlogit(GemmArgs g) {
+  extern __shared__ char smem[];
+  const Place<T> p(g);
+  typename Mma<E>::Acc acc[T::MI][T::NI];
+  multiply<E, T, false, false>(acc, g.A, g.B, g.k, p.m0, p.n0, 0, g.steps, smem);
+  const float mul = g.ua ? *g.ua * *g.ub : 1.0f;
+  const float gs = *g.gscale;
+#pragma unroll
+  for (int j = 0; j < T::NI; ++j) {
+    const int n = p.nw + 32 * j + p.col;
+    bool counts = false;
+    int t = -1;
+    float c = 0.0f, lse = 0.0f;
+    if (n < g.N) {
+      t = target_of(g.targets, n, counts);
+      if (counts) {
+        c = t < 0 ? __builtin_nanf("") : g.gloss[n] * gs;
+        lse = g.lse[n];
+      }
+    }
+    const int at = t < 0 ? -1 : t - g.v0 - p.mw;
+    const bool here = __any(at >= 0 && at < T::MI * 32);
+#pragma unroll
+    for (int i = 0; i < T::MI; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int rel = 32 * i + 8 * q + 4 * p.h;
+        float d[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          d[r] = exp2_fast((acc[i][j][4 * q + r] * mul - lse) * LOG2E);
+          if (here && at == rel + r) d[r] -= 1.0f;
+          d[r] = counts && p.mw + rel + r < g.M ? d[r] * c : 0.0f;
+        }
+        char* to = g.D + ((int64_t)n * g.ldd + p.mw + rel) * 2;
+        const uint32_t b0 = bits16(d[0], g.dtype), b1 = bits16(d[1], g.dtype), b2 = bits16(d[2], g.dtype), b3 = bits16(d[3], g.dtype);
+        *(uint2*)to = make_uint2(b0 | b1 << 16, b2 | b3 << 16);
+        if (g.dplanes == 2) {
+          const uint32_t hb[4] = {b0, b1, b2, b3};
+          uint32_t lb[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float hv = (float)__builtin_bit_cast(_Float16, (uint16_t)hb[r]);
+            lb[r] = bits16(fabsf(d[r]) <= 65504.0f ? d[r] - hv : 0.0f, PST_F16);
+          }
+          *(uint2*)(to + g.dplane) = make_uint2(lb[0] | lb[1] << 16, lb[2] | lb[3] << 16);
+        }
+      }
+  }
+}
+
+// dx's part from one piece of the vocabulary: m = column of dx, n = position, k = vocabulary row
+template <int E, class T>
+__global__ __launch_bounds__(T::THREADS) void k_dx(GemmArgs g) {
+  extern __shared__ char smem[];
+  const Place<T> p(g);
+  typename Mma<E>::Acc acc[T::MI][T::NI];
+  const int s0 = (int)((int64_t)g.steps * p.z / g.nz), s1 = (int)((int64_t)g.steps * (p.z + 1) / g.nz);
+  multiply<E, T, true, false>(acc, g.A, g.B, g.k, p.m0, p.n0, s0, s1, smem);
+  float* out = (float*)g.out + p.z * g.zstride;
+#pragma unroll
+  for (int j = 0; j < T::NI; ++j) {
+    const int n = p.nw + 32 * j + p.col;
+#pragma unroll
+    for (int i = 0; i < T::MI; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int m = p.mw + 32 * i + 8 * q + 4 * p.h;
+        if (m >= g.ldo) continue;
+        f32x4* to = (f32x4*)(out + (int64_t)n * g.ldo + m);
+        f32x4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        if (g.add) {
+          const f32x4 o = *to;
+          v.x += o.x;
+          v.y += o.y;
+          v.z += o.z;
+          v.w += o.w;
+        }
+        *to = v;
+      }
+  }
+}
+
+struct FinishArgs {
+  const float* part;
+  int64_t ldp, zstride;
+  int32_t nz, n, width, otype;
+  void* out;
+  int64_t ldo;
+  const float *u0, *u1;
+  Targets targets;
+};
+// dx from its pieces' sums
+__global__ __launch_bounds__(256) void k_finish(FinishArgs a) {
+  const int per = (a.width + 3) / 4;
+  const int64_t total = (int64_t)a.n * per;
+  const float mul = *a.u0 * (a.u1 ? *a.u1 : 1.0f);
+  for (int64_t g = blockIdx.x * (int64_t)256 + threadIdx.x; g < total; g += (int64_t)gridDim.x * 256) {
+    const int64_t n = g / per;
+    const int c = (int)(g - n * per) * 4;
+    f32x4 s = {0, 0, 0, 0};
+    for (int z = 0; z < a.nz; ++z) {
+      const f32x4 v = *(const f32x4*)(a.part + z * a.zstride + n * a.ldp + c);
+      s.x += v.x;
+      s.y += v.y;
+      s.z += v.z;
+      s.w += v.w;
+    }
+    bool counts;
+    (void)target_of(a.targets, n, counts);
+    const float v[4] = {counts ? s.x * mul : 0.0f, counts ? s.y * mul : 0.0f, counts ? s.z * mul : 0.0f, counts ? s.w * mul : 0.0f};
+    const bool wide = a.otype == PST_F32 ? ((uintptr_t)a.out & 15) == 0 && a.ldo % 4 == 0 : ((uintptr_t)a.out & 7) == 0 && a.ldo % 4 == 0;
+    store4(a.out, a.otype, n * a.ldo + c, v, a.width - c, wide);
+  }
+}
+
+// rows v0 ... of dW: m = column, n = vocabulary row of the piece, k = position
+template <int E, class T>
+__global__ __launch_bounds__(T::THREADS) void k_dw(GemmArgs g) {
+  extern __shared__ char smem[];
+  const Place<T> p(g);
+  typename Mma<E>::Acc acc[T::MI][T::NI];
+  multiply<E, T, true, true>(acc, g.A, g.B, g.k, p.m0, p.n0, 0, g.steps, smem);
+  const float mul = *g.ua * (g.ub ? *g.ub : 1.0f);
+#pragma unroll
+  for (int j = 0; j < T::NI; ++j) {
+    const int n = p.nw + 32 * j + p.col;
+    if (n >= g.N) continue;
+#pragma unroll
+    for (int i = 0; i < T::MI; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int m = p.mw + 32 * i + 8 * q + 4 * p.h;
+        if (m >= g.M) continue;
+        const float v[4] = {acc[i][j][4 * q] * mul, acc[i][j][4 * q + 1] * mul, acc[i][j][4 * q + 2] * mul, acc[i][j][4 * q + 3] * mul};
+        store4(g.out, g.otype, (int64_t)(g.v0 + n) * g.ldo + m, v, g.M - m, g.wide);
+      }
+  }
+}
+
+// 8-bit scores: m = vocabulary row, n = position
+template <class T>
+__global__ __launch_bounds__(T::THREADS) void k_scores(GemmArgs g) {
+  extern __shared__ char smem[];
+  const Place<T> p(g);
+  typename Mma<I8>::Acc acc[T::MI][T::NI];
+  multiply<I8, T, false, false>(acc, g.A, g.B, g.k, p.m0, p.n0, 0, g.steps, smem);
+#pragma unroll
+  for (int j = 0; j < T::NI; ++j) {
+    const int n = p.nw + 32 * j + p.col;
+    if (n >= g.N) continue;
+    const float sn = g.sn[n];
+#pragma unroll
+    for (int i = 0; i < T::MI; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int m = p.mw + 32 * i + 8 * q + 4 * p.h;
+        if (m >= g.M) continue;
+        float v[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = (float)acc[i][j][4 * q + r] * sn * g.sm[min(m + r, g.M - 1)];
+        store4(g.out, g.otype, (int64_t)n * g.ldo + m, v, g.M - m, g.wide);
+      }
+  }
+}
+
+struct QuantArgs {
+  const void* src;
+  int64_t ld, ldq;
+  int64_t rows;
+  int32_t width, width_pad, type;  // columns width .. width_pad - 1 become zeros
+  int8_t* q;
+  float* scale;
+};
+// one wave a row: the largest magnitude, then rint(x / s). A row that holds an infinity or a NaN gets the scale
+// NaN and zeros, so that what is computed from it says so.
+__global__ __launch_bounds__(256) void k_quantize(QuantArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t r = blockIdx.x * (int64_t)4 + (threadIdx.x >> 6);
+  if (r >= a.rows) return;
+  float m = 0.0f;
+  bool bad = false;
+  for (int k = lane; k < a.width; k += 64) {
+    const float v = fabsf(load1(a.src, a.type, r * a.ld + k));
+    bad |= !(v <= 3.4028234663852886e38f);
+    m = fmaxf(m, v);
+  }
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
+  bad = __any(bad);
+  const float s = m * (1.0f / 127.0f);
+  if (lane == 0) a.scale[r] = bad ? __builtin_nanf("") : s;
+  const bool zero = bad || !(s > 0.0f);
+  for (int k = lane; k < a.width_pad; k += 64) {
+    int q = 0;
+    // a subnormal scale can make the quotient pass 127
+    if (k < a.width && !zero) q = (int)fminf(fmaxf(rintf(load1(a.src, a.type, r * a.ld + k) / s), -127.0f), 127.0f);
+    a.q[r * a.ldq + k] = (int8_t)q;
+  }
+}
+// 8-bit rows into whole K-steps
+__global__ __launch_bounds__(256) void k_pack8(const int8_t* src, int64_t ld, int64_t rows, int32_t width, int32_t width_pad, int8_t* dst) {
+  const int per = width_pad / 16;
+  const int64_t total = rows * per;
+  for (int64_t g = blockIdx.x * (int64_t)256 + threadIdx.x; g < total; g += (int64_t)gridDim.x * 256) {
+    const int64_t r = g / per;
+    const int c = (int)(g - r * per) * 16;
+    int8_t v[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = c + j < width ? src[r * ld + c + j] : (int8_t)0;
+    *(uint4*)(dst + r * width_pad + c) = __builtin_bit_cast(uint4, *(i32x4*)v);
+  }
+}
+
+// 16-bit floats with a short exponent (and the halves of a split one): D is scaled by the power of two that
+// brings the largest |g_n| to 2^13; scale[0] = that power, scale[1] = its inverse. bfloat16: 1.
+__global__ __launch_bounds__(1024) void k_gscale(const float* g, Targets t, int64_t n, int type, float* scale) {
+  __shared__ float sm[16];
+  float m = 0.0f;
+  if (type != PST_BF16)
+    for (int64_t i = threadIdx.x; i < n; i += 1024) {
+      bool counts;
+      (void)target_of(t, i, counts);
+      if (counts) m = fmaxf(m, finite_abs(g[i]));
+    }
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
+  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 16; ++w) m = fmaxf(m, sm[w]);
+    const int e = type == PST_BF16 ? 0 : max(-100, min(100, split_exp(m)));
+    scale[0] = ldexpf(1.0f, e);
+    scale[1] = ldexpf(1.0f, -e);
+  }
+}
+
+// ------------------------------------------------------------------ host
+thread_local std::string g_error;
+
+int fail(int code, const std::string& what) {
+  g_error = what;
+  return code;
+}
+// a runtime error is reported here, and not again by the caller's next call
+int hip_fail(const std::string& what, hipError_t e) {
+  (void)hipGetLastError();
+  return fail(PST_E_HIP, what + ": " + hipGetErrorString(e));
+}
+#define HEADCHK(x)                                       \
+  do {                                                   \
+    const hipError_t e_ = (x);                           \
+    if (e_ != hipSuccess) return hip_fail(#x, e_);       \
+  } while (0)
+
+// the calling thread's current device, put back on return
+struct OnDevice {
+  int old = -1;
+  hipError_t e;
+  explicit OnDevice(int device) {
+    e = hipGetDevice(&old);
+    if (e == hipSuccess && old != device) {
+      e = hipSetDevice(device);
+    } else if (e == hipSuccess) {
+      old = -1;
+    }
+  }
+  ~OnDevice() {
+    if (e == hipSuccess && old >= 0) (void)hipSetDevice(old);
+  }
+};
+
+int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int size_of(int type) { return type == PST_F32 ? 4 : 2; }
+bool is_type(int type) { return type == PST_F32 || type == PST_BF16 || type == PST_F16; }
+
+// offsets in the caller's workspace
+struct Bump {
+  int64_t n = 0;
+  int64_t take(int64_t bytes) {
+    const int64_t at = n;
+    n += up(bytes, 256);
+    return at;
+  }
+};
+
+// a matrix that the kernels read where it is: 16-byte rows of whole 16-byte pieces
+bool in_place(const void* p, int64_t ld_bytes, int64_t row_bytes) {
+  return ((uintptr_t)p & 15) == 0 && ld_bytes % 16 == 0 && row_bytes % 16 == 0;
+}
+
+using T256 = Tile<256, 256, 2, 4>;
+using T128 = Tile<128, 128, 2, 2>;
+using T64 = Tile<64, 64, 2, 2>;
+enum TileId { TILE64 = 0, TILE128 = 1, TILE256 = 2 };
+constexpr int TILE_M[3] = {64, 128, 256};
+
+// The largest tile that still gives most compute units one.
+int tile_for(int64_t m, int64_t n, int cus) {
+  for (int t = TILE256; t > TILE64; --t)
+    if (ceil_div(m, TILE_M[t]) * ceil_div(n, TILE_M[t]) * 4 >= 3 * (int64_t)cus) return t;
+  return TILE64;
+}
+
+template <class F>
+hipError_t launch(F* f, int64_t grid, int threads, int lds, hipStream_t st, const GemmArgs& g) {
+  if (lds > 65536) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL(f, dim3((unsigned)grid), dim3(threads), lds, st, g);
+  return hipGetLastError();
+}
+template <int E, class T>
+hipError_t launch_kind(int kind, const GemmArgs& g, hipStream_t st) {
+  const int64_t grid = (int64_t)g.nm * g.nn * g.nz;
+  switch (kind) {
+    case LOSS: return launch(k_loss<E, T>, grid, T::THREADS, T::LDS, st, g);
+    case DLOGIT: return launch(k_dlogit<E, T>, grid, T::THREADS, T::LDS, st, g);
+    case DX: return launch(k_dx<E, T>, grid, T::THREADS, T::LDS, st, g);
+    default: return launch(k_dw<E, T>, grid, T::THREADS, T::LDS, st, g);
+  }
+}
+hipError_t launch_gemm(int kind, int elem, int tile, GemmArgs g, hipStream_t st) {
+  const int t = TILE_M[tile];
+  g.nm = (int32_t)ceil_div(kind == DX ? g.ldo : (int64_t)g.M, t);
+  g.nn = (int32_t)ceil_div(g.N, t);
+  if (kind == DLOGIT) g.nm = (int32_t)(g.ldd / t);  // D's zeros behind the vocabulary too
+  if (g.nz == 0) g.nz = 1;
+  if (g.gm == 0) g.gm = 4;
+  if ((int64_t)g.nm * g.nn * g.nz > 0x7fffffff) return hipErrorInvalidConfiguration;
+  if (kind == SCORES) {
+    const int64_t grid = (int64_t)g.nm * g.nn;
+    return tile == TILE256   ? launch(k_scores<T256>, grid, T256::THREADS, T256::LDS, st, g)
+           : tile == TILE128 ? launch(k_scores<T128>, grid, T128::THREADS, T128::LDS, st, g)
+                             : launch(k_scores<T64>, grid, T64::THREADS, T64::LDS, st, g);
+  }
+  if (elem == BF16)
+    return tile == TILE256 ? launch_kind<BF16, T256>(kind, g, st) : tile == TILE128 ? launch_kind<BF16, T128>(kind, g, st) : launch_kind<BF16, T64>(kind, g, st);
+  return tile == TILE256 ? launch_kind<F16, T256>(kind, g, st) : tile == TILE128 ? launch_kind<F16, T128>(kind, g, st) : launch_kind<F16, T64>(kind, g, st);
+}
+
+int cus_of(int device, int* cus) {
+  HEADCHK(hipDeviceGetAttribute(cus, hipDeviceAttributeMultiprocessorCount, device));
+  return PST_OK;
+}
+
+// What a call on [rows, width] x [vocab, width] needs of its workspace; the same for the query and for the call.
+struct Plan {
+  int type, elem, planes;
+  int64_t rows, vocab, width, width_pad, rows_pad;
+  bool pack_x, pack_w;
+  int64_t amax = 0, unscale = 0, x = 0, w = 0;   // offsets
+  int64_t part = 0, tlogit = 0;                  // loss
+  int64_t gscale = 0, D = 0, dxp = 0;            // gradient
+  int64_t piece = 0;                             // vocabulary rows of a piece
+  int nz = 1;
+  int64_t bytes = 0;
+};
+
+Plan plan_common(int type, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab, int64_t width, bool grad, Bump& b) {
+  Plan p;
+  p.type = type;
+  p.elem = type == PST_BF16 ? BF16 : F16;
+  p.planes = type == PST_F32 ? 2 : 1;
+  p.rows = rows;
+  p.vocab = vocab;
+  p.width = width;
+  p.width_pad = up(width, 64);
+  p.rows_pad = up(rows, 256);
+  const int e = size_of(type);
+  p.pack_w = type == PST_F32 || !in_place(w, ldw * e, width * e);
+  // x is the operand with zeros behind the last column; the gradient needs zeros behind the last row too
+  p.pack_x = type == PST_F32 || grad || p.width_pad != width || !in_place(x, ldx * e, width * e);
+  if (type == PST_F32) {
+    p.amax = b.take(2 * AMAX_BLOCKS * 4);
+    p.unscale = b.take(8);
+  }
+  if (p.pack_x) p.x = b.take((grad ? p.rows_pad : rows) * p.width_pad * 2 * p.planes);
+  if (p.pack_w) p.w = b.take(vocab * p.width_pad * 2 * p.planes);
+  return p;
+}
+Plan plan_loss(int type, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab, int64_t width) {
+  Bump b;
+  Plan p = plan_common(type, x, ldx, w, ldw, rows, vocab, width, false, b);
+  p.part = b.take(ceil_div(vocab, 64) * rows * 8);
+  p.tlogit = b.take(rows * 4);
+  p.bytes = b.n;
+  return p;
+}
+// bytes of D that a piece of the vocabulary may take: about what the last-level cache (256 MB) holds
+constexpr int64_t PIECE_BYTES = 288ll << 20;
+Plan plan_grad(int type, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab, int64_t width) {
+  Bump b;
+  Plan p = plan_common(type, x, ldx, w, ldw, rows, vocab, width, true, b);
+  p.gscale = b.take(8);
+  const int64_t most = std::max<int64_t>(256, PIECE_BYTES / (p.rows_pad * 2 * p.planes) / 256 * 256);
+  p.piece = up(ceil_div(vocab, ceil_div(vocab, most)), 256);
+  p.D = b.take(p.rows_pad * p.piece * 2 * p.planes);
+  // few tiles of dx: the pieces' K loops are split so that each compute unit has one
+  const int64_t tiles = ceil_div(p.width_pad, 64) * ceil_div(rows, 64);
+  p.nz = (int)std::max<int64_t>(1, std::min<int64_t>({8, p.piece / 64 / 4, 512 / std::max<int64_t>(1, tiles)}));
+  if (p.nz == 1 && ceil_div(p.width_pad, 256) * ceil_div(rows, 256) < 192) p.nz = 2;
+  p.dxp = b.take(p.nz * p.rows_pad * p.width_pad * 4);
+  p.bytes = b.n;
+  return p;
+}
+
+int check_sizes(int type, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab, int64_t width) {
+  if (!is_type(type)) return fail(PST_E_INVALID, "unknown type");
+  if (rows < 0 || vocab < 1 || width < 1) return fail(PST_E_INVALID, "rows >= 0, vocab >= 1 and width >= 1 are needed");
+  if (rows > (1ll << 30) || vocab > (1ll << 30) || width > (1 << 20)) return fail(PST_E_TOO_LARGE, "rows or vocab over 2^30, or width over 2^20");
+  if (ldx < width || ldw < width) return fail(PST_E_INVALID, "a row stride is smaller than the width");
+  if (ldx > (1 << 21) || ldw > (1 << 21)) return fail(PST_E_TOO_LARGE, "a row stride over 2^21");
+  const int e = size_of(type);
+  if (rows && (!x || ((uintptr_t)x % e))) return fail(PST_E_INVALID, "hidden is null or not aligned to its type");
+  if (!w || ((uintptr_t)w % e)) return fail(PST_E_INVALID, "weight is null or not aligned to its type");
+  return PST_OK;
+}
+int check_targets(const void* targets, int bits, int64_t rows) {
+  if (bits != 32 && bits != 64) return fail(PST_E_INVALID, "targets are 32 or 64 bits wide");
+  if (rows && (!targets || ((uintptr_t)targets % (bits / 8)))) return fail(PST_E_INVALID, "targets are null or not aligned");
+  return PST_OK;
+}
+int check_ws(const void* ws, int64_t have, int64_t need) {
+  if (have < need) return fail(PST_E_INVALID, "workspace of " + std::to_string(have) + " bytes, " + std::to_string(need) + " are needed");
+  if (!ws || ((uintptr_t)ws & 255)) return fail(PST_E_INVALID, "the workspace is null or not aligned to 256 bytes");
+  return PST_OK;
+}
+
+// grids of the copying kernels: a few workgroups a compute unit
+unsigned copy_grid(int64_t groups, int cus) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(groups, 256), cus * 16ll)); }
+
+// the operands in a form that the products read: in place, or packed (and split) into the workspace
+int operands(const Plan& p, const void* x, int64_t ldx, const void* w, int64_t ldw, const Targets* zero_rows, char* ws, int cus, hipStream_t st,
+             Operand* X, Operand* W) {
+  const int64_t xrows = zero_rows ? p.rows_pad : p.rows;
+  float* part = (float*)(ws + p.amax);
+  float* unscale = (float*)(ws + p.unscale);
+  if (p.type == PST_F32) {
+    AmaxArgs a{{(const float*)x, (const float*)w}, {ldx, ldw}, {p.rows, p.vocab}, (int32_t)p.width, part};
+    hipLaunchKernelGGL(k_amax, dim3(2 * AMAX_BLOCKS), dim3(256), 0, st, a);
+    HEADCHK(hipGetLastError());
+  }
+  auto pack = [&](const void* src, int64_t ld, int64_t rows, int64_t rows_pad, int64_t at, int which, const Targets* t) {
+    PackArgs a{};
+    a.src = src;
+    a.ld = ld;
+    a.rows = rows;
+    a.rows_pad = rows_pad;
+    a.width = (int32_t)p.width;
+    a.width_pad = (int32_t)p.width_pad;
+    a.type = p.type;
+    a.dst = ws + at;
+    a.plane = rows_pad * p.width_pad * 2;
+    a.part = part + which * AMAX_BLOCKS;
+    a.unscale = unscale + which;
+    if (t) a.targets = *t;
+    hipLaunchKernelGGL(k_pack, dim3(copy_grid(rows_pad * (p.width_pad / 8), cus)), dim3(256), 0, st, a);
+  };
+  const int e = size_of(p.type);
+  if (p.pack_x) {
+    pack(x, ldx, p.rows, xrows, p.x, 0, zero_rows);
+    HEADCHK(hipGetLastError());
+    *X = {ws + p.x, xrows * p.width_pad * 2, p.width_pad * 2, (int32_t)xrows, (int32_t)p.width_pad * 2};
+  } else {
+    *X = {(const char*)x, 0, ldx * e, (int32_t)p.rows, (int32_t)p.width * e};
+  }
+  if (p.pack_w) {
+    pack(w, ldw, p.vocab, p.vocab, p.w, 1, nullptr);
+    HEADCHK(hipGetLastError());
+    *W = {ws + p.w, p.vocab * p.width_pad * 2, p.width_pad * 2, (int32_t)p.vocab, (int32_t)p.width_pad * 2};
+  } else {
+    *W = {(const char*)w, 0, ldw * e, (int32_t)p.vocab, (int32_t)p.width * e};
+  }
+  return PST_OK;
+}
+
+// the passes of a product of split operands, the small terms first: (lo, hi), (hi, lo), (hi, hi)
+KLoop passes(int planes) { return planes == 2 ? KLoop{3, 0x01, 0x04} : KLoop{1, 0, 0}; }
+
+int token_loss(int device, int type, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab, int64_t width,
+               const void* targets, int tbits, int64_t ignore, float* loss, float* lse, void* ws_, int64_t ws_bytes, hipStream_t st) {
+  int rc = check_sizes(type, x, ldx, w, ldw, rows, vocab, width);
+  if (rc == PST_OK) rc = check_targets(targets, tbits, rows);
+  if (rc != PST_OK) return rc;
+  if (rows == 0) return PST_OK;
+  if (!loss || !lse || ((uintptr_t)loss & 3) || ((uintptr_t)lse & 3)) return fail(PST_E_INVALID, "loss or lse is null or not aligned");
+  const Plan p = plan_loss(type, x, ldx, w, ldw, rows, vocab, width);
+  rc = check_ws(ws_, ws_bytes, p.bytes);
+  if (rc != PST_OK) return rc;
+  OnDevice on(device);
+  if (on.e != hipSuccess) return hip_fail("device " + std::to_string(device), on.e);
+  int cus = 0;
+  rc = cus_of(device, &cus);
+  if (rc != PST_OK) return rc;
+  char* ws = (char*)ws_;
+  GemmArgs g{};
+  rc = operands(p, x, ldx, w, ldw, nullptr, ws, cus, st, &g.B, &g.A);
+  if (rc != PST_OK) return rc;
+  g.k = passes(p.planes);
+  g.M = (int32_t)vocab;
+  g.N = (int32_t)rows;
+  g.steps = (int32_t)(p.width_pad / 64);
+  if (p.planes == 2) {
+    g.ua = (float*)(ws + p.unscale) + 1;
+    g.ub = (float*)(ws + p.unscale);
+  }
+  g.targets = {targets, ignore, tbits, (int32_t)vocab};
+  g.part = (float2*)(ws + p.part);
+  g.tlogit = (float*)(ws + p.tlogit);
+  const int tile = tile_for(vocab, rows, cus);
+  HEADCHK(launch_gemm(LOSS, p.elem, tile, g, st));
+  JoinArgs j{g.part, g.tlogit, g.targets, loss, lse, (int32_t)rows, (int32_t)ceil_div(vocab, TILE_M[tile])};
+  hipLaunchKernelGGL(k_join, dim3((unsigned)ceil_div(rows, 64)), dim3(1024), 0, st, j);
+  HEADCHK(hipGetLastError());
+  return PST_OK;
+}
+
+int token_loss_grad(int device, int type, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab, int64_t width,
+                    const void* targets, int tbits, int64_t ignore, const float* lse, const float* gloss, void* dx, int64_t lddx, void* dw,
+                    int64_t lddw, void* ws_, int64_t ws_bytes, hipStream_t st) {
+  int rc = check_sizes(type, x, ldx, w, ldw, rows, vocab, width);
+  if (rc == PST_OK) rc = check_targets(targets, tbits, rows);
+  if (rc != PST_OK) return rc;
+  const int e = size_of(type);
+  if ((dx && lddx < width) || (dw && lddw < width)) return fail(PST_E_INVALID, "a gradient's row stride is smaller than the width");
+  if (((uintptr_t)dx % e) || ((uintptr_t)dw % e)) return fail(PST_E_INVALID, "a gradient is not aligned to its type");
+  if (!dx && !dw) return PST_OK;
+  if (rows && (!lse || !gloss || ((uintptr_t)lse & 3) || ((uintptr_t)gloss & 3))) return fail(PST_E_INVALID, "lse or grad_loss is null or not aligned");
+  if (rows == 0 && !dw) return PST_OK;
+  const Plan p = plan_grad(type, x, ldx, w, ldw, std::max<int64_t>(rows, 1), vocab, width);
+  rc = check_ws(ws_, ws_bytes, p.bytes);
+  if (rc != PST_OK) return rc;
+  OnDevice on(device);
+  if (on.e != hipSuccess) return hip_fail("device " + std::to_string(device), on.e);
+  int cus = 0;
+  rc = cus_of(device, &cus);
+  if (rc != PST_OK) return rc;
+  char* ws = (char*)ws_;
+  const Targets t{targets, ignore, tbits, (int32_t)vocab};
+  // no positions: one of zeros stands for them, so that dW is written as the zeros that it is
+  Plan q = p;
+  q.rows = rows;
+  Operand X, W;
+  rc = operands(q, x, ldx, w, ldw, &t, ws, cus, st, &X, &W);
+  if (rc != PST_OK) return rc;
+  float* gs = (float*)(ws + p.gscale);
+  hipLaunchKernelGGL(k_gscale, dim3(1), dim3(1024), 0, st, gloss, t, rows, type, gs);
+  HEADCHK(hipGetLastError());
+  const float* ux = p.planes == 2 ? (float*)(ws + p.unscale) : nullptr;
+  const float* uw = p.planes == 2 ? ux + 1 : nullptr;
+  char* D = ws + p.D;
+  float* dxp = (float*)(ws + p.dxp);
+  for (int64_t v0 = 0; v0 < vocab; v0 += p.piece) {
+    const int64_t nv = std::min(p.piece, vocab - v0), nv_pad = up(nv, 256);
+    const int64_t dplane = p.rows_pad * nv_pad * 2;
+    GemmArgs g{};
+    g.k = passes(p.planes);
+    g.A = W;
+    g.A.p += v0 * W.ld;
+    g.A.rows = (int32_t)nv;
+    g.B = X;
+    g.M = (int32_t)nv;
+    g.N = (int32_t)rows;
+    g.steps = (int32_t)(p.width_pad / 64);
+    g.ua = uw;
+    g.ub = ux;
+    g.targets = t;
+    g.lse = lse;
+    g.gloss = gloss;
+    g.gscale = gs;
+    g.D = D;
+    g.dplane = dplane;
+    g.ldd = nv_pad;
+    g.dtype = p.elem == BF16 ? PST_BF16 : PST_F16;
+    g.dplanes = p.planes;
+    g.v0 = (int32_t)v0;
+    if (rows) HEADCHK(launch_gemm(DLOGIT, p.elem, tile_for(nv, rows, cus), g, st));
+    if (dx && rows) {
+      GemmArgs d{};
+      d.k = passes(p.planes);
+      d.A = W;
+      d.A.p += v0 * W.ld;
+      d.A.rows = (int32_t)nv;
+      d.B = {D, dplane, nv_pad * 2, (int32_t)p.rows_pad, (int32_t)nv_pad * 2};
+      d.M = (int32_t)width;
+      d.N = (int32_t)rows;
+      d.steps = (int32_t)ceil_div(nv, 64);
+      d.nz = p.nz;
+      d.out = dxp;
+      d.ldo = p.width_pad;
+      d.zstride = p.rows_pad * p.width_pad;
+      d.add = v0 > 0;
+      HEADCHK(launch_gemm(DX, p.elem, tile_for(p.width_pad, rows * p.nz, cus), d, st));
+    }
+    if (dw) {
+      GemmArgs d{};
+      d.k = passes(p.planes);
+      d.A = X;
+      d.B = {D, dplane, nv_pad * 2, (int32_t)p.rows_pad, (int32_t)nv_pad * 2};
+      d.M = (int32_t)width;
+      d.N = (int32_t)nv;
+      d.steps = (int32_t)ceil_div(rows, 64);
+      d.ua = gs + 1;
+      d.ub = ux;
+      d.v0 = (int32_t)v0;
+      d.out = dw;
+      d.ldo = lddw;
+      d.otype = type;
+      d.wide = lddw % 4 == 0 && ((uintptr_t)dw & (type == PST_F32 ? 15 : 7)) == 0;
+      HEADCHK(launch_gemm(DW, p.elem, tile_for(width, nv, cus), d, st));
+    }
+  }
+  if (dx && rows) {
+    FinishArgs f{dxp, p.width_pad, p.rows_pad * p.width_pad, p.nz, (int32_t)rows, (int32_t)width, type, dx, lddx, gs + 1, uw, t};
+    hipLaunchKernelGGL(k_finish, dim3(copy_grid(rows * ceil_div(width, 4), cus)), dim3(256), 0, st, f);
+    HEADCHK(hipGetLastError());
+  }
+  return PST_OK;
+}
+
+int quantize_rows(int device, int type, const void* x, int64_t ldx, int64_t rows, int64_t width, int8_t* q, int64_t ldq, float* scale, hipStream_t st) {
+  if (!is_type(type)) return fail(PST_E_INVALID, "unknown type");
+  if (rows < 0 || width < 1) return fail(PST_E_INVALID, "rows >= 0 and width >= 1 are needed");
+  if (rows > (1ll << 30) || width > (1 << 20)) return fail(PST_E_TOO_LARGE, "rows over 2^30, or width over 2^20");
+  if (ldx < width || ldq < width) return fail(PST_E_INVALID, "a row stride is smaller than the width");
+  if (rows == 0) return PST_OK;
+  if (!x || ((uintptr_t)x % size_of(type)) || !q || !scale || ((uintptr_t)scale & 3)) return fail(PST_E_INVALID, "a buffer is null or not aligned to its type");
+  OnDevice on(device);
+  if (on.e != hipSuccess) return hip_fail("device " + std::to_string(device), on.e);
+  QuantArgs a{x, ldx, ldq, rows, (int32_t)width, (int32_t)width, type, q, scale};
+  hipLaunchKernelGGL(k_quantize, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, st, a);
+  HEADCHK(hipGetLastError());
+  return PST_OK;
+}
+
+struct ScorePlan {
+  int64_t width_pad;
+  bool pack_w;
+  int64_t q, scale, w, bytes;
+};
+ScorePlan plan_scores(const void* w, int64_t ldw, int64_t rows, int64_t vocab, int64_t width) {
+  ScorePlan p{};
+  Bump b;
+  p.width_pad = up(width, STEP);
+  p.pack_w = !in_place(w, ldw, width);
+  p.q = b.take(rows * p.width_pad);
+  p.scale = b.take(rows * 4);
+  if (p.pack_w) p.w = b.take(vocab * p.width_pad);
+  p.bytes = b.n;
+  return p;
+}
+int check_scores(int type, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab, int64_t width) {
+  if (!is_type(type)) return fail(PST_E_INVALID, "unknown type");
+  if (rows < 0 || vocab < 1 || width < 1) return fail(PST_E_INVALID, "rows >= 0, vocab >= 1 and width >= 1 are needed");
+  // 127 * 127 * width has to stay inside 32 bits
+  if (rows > (1ll << 30) || vocab > (1ll << 30) || width > 131072) return fail(PST_E_TOO_LARGE, "rows or vocab over 2^30, or width over 131072");
+  if (ldx < width || ldw < width) return fail(PST_E_INVALID, "a row stride is smaller than the width");
+  if (ldw > (1 << 23)) return fail(PST_E_TOO_LARGE, "a row stride over 2^23");
+  if (rows && (!x || ((uintptr_t)x % size_of(type)))) return fail(PST_E_INVALID, "hidden is null or not aligned to its type");
+  if (!w) return fail(PST_E_INVALID, "weight is null");
+  return PST_OK;
+}
+int token_scores_i8(int device, int type, const void* x, int64_t ldx, const int8_t* w, int64_t ldw, const float* wscale, int64_t rows, int64_t vocab,
+                    int64_t width, int otype, void* out, int64_t ldo, void* ws_, int64_t ws_bytes, hipStream_t st) {
+  int rc = check_scores(type, x, ldx, w, ldw, rows, vocab, width);
+  if (rc != PST_OK) return rc;
+  if (!is_type(otype)) return fail(PST_E_INVALID, "unknown output type");
+  if (rows == 0) return PST_OK;
+  if (ldo < vocab) return fail(PST_E_INVALID, "the scores' row stride is smaller than the vocabulary");
+  if (!wscale || ((uintptr_t)wscale & 3) || !out || ((uintptr_t)out % size_of(otype))) return fail(PST_E_INVALID, "scale or scores is null or not aligned");
+  const ScorePlan p = plan_scores(w, ldw, rows, vocab, width);
+  rc = check_ws(ws_, ws_bytes, p.bytes);
+  if (rc != PST_OK) return rc;
+  OnDevice on(device);
+  if (on.e != hipSuccess) return hip_fail("device " + std::to_string(device), on.e);
+  int cus = 0;
+  rc = cus_of(device, &cus);
+  if (rc != PST_OK) return rc;
+  char* ws = (char*)ws_;
+  QuantArgs a{x, ldx, p.width_pad, rows, (int32_t)width, (int32_t)p.width_pad, type, (int8_t*)(ws + p.q), (float*)(ws + p.scale)};
+  hipLaunchKernelGGL(k_quantize, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, st, a);
+  HEADCHK(hipGetLastError());
+  GemmArgs g{};
+  g.k = passes(1);
+  if (p.pack_w) {
+    hipLaunchKernelGGL(k_pack8, dim3(copy_grid(vocab * (p.width_pad / 16), cus)), dim3(256), 0, st, w, ldw, vocab, (int32_t)width, (int32_t)p.width_pad,
+                       (int8_t*)(ws + p.w));
+    HEADCHK(hipGetLastError());
+    g.A = {ws + p.w, 0, p.width_pad, (int32_t)vocab, (int32_t)p.width_pad};
+  } else {
+    g.A = {(const char*)w, 0, ldw, (int32_t)vocab, (int32_t)width};
+  }
+  g.B = {ws + p.q, 0, p.width_pad, (int32_t)rows, (int32_t)p.width_pad};
+  g.M = (int32_t)vocab;
+  g.N = (int32_t)rows;
+  g.steps = (int32_t)(p.width_pad / STEP);
+  g.out = out;
+  g.ldo = ldo;
+  g.otype = otype;
+  g.wide = ldo % 4 == 0 && ((uintptr_t)out & (otype == PST_F32 ? 15 : 7)) == 0;
+  g.sn = (const float*)(ws + p.scale);
+  g.sm = wscale;
+  HEADCHK(launch_gemm(SCORES, I8, tile_for(vocab, rows, cus), g, st));
+  return PST_OK;
+}
+
+template <class F>
+int guarded(F f) {
+  try {
+    return f();
+  } catch (const std::bad_alloc&) {
+    return PST_E_NOMEM;
+  } catch (...) {
+    return PST_E_INVALID;
+  }
+}
+
+}  // namespace
+}  // namespace pst_head
+
+extern "C" {
+
+const char* pst_head_error(void) { return pst_head::g_error.c_str(); }
+
+int64_t pst_token_loss_workspace(int32_t type, const void* d_hidden, int64_t ld_hidden, const void* d_weight, int64_t ld_weight, int64_t rows,
+                                 int64_t vocab, int64_t width) {
+  using namespace pst_head;
+  return guarded([&]() -> int {
+           return check_sizes(type, d_hidden, ld_hidden, d_weight, ld_weight, rows, vocab, width);
+         }) == PST_OK
+             ? plan_loss(type, d_hidden, ld_hidden, d_weight, ld_weight, rows, vocab, width).bytes
+             : (int64_t)PST_E_INVALID;
+}
+
+int pst_token_loss(int32_t device, int32_t type, const void* d_hidden, int64_t ld_hidden, const void* d_weight, int64_t ld_weight, int64_t rows,
+                   int64_t vocab, int64_t width, const void* d_targets, int32_t target_bits, int64_t ignore, float* d_loss, float* d_lse,
+                   void* d_workspace, int64_t workspace_bytes, void* stream) {
+  return pst_head::guarded([&] {
+    return pst_head::token_loss(device, type, d_hidden, ld_hidden, d_weight, ld_weight, rows, vocab, width, d_targets, target_bits, ignore, d_loss,
+                                d_lse, d_workspace, workspace_bytes, (hipStream_t)stream);
+  });
+}
+
+int64_t pst_token_loss_grad_workspace(int32_t type, const void* d_hidden, int64_t ld_hidden, const void* d_weight, int64_t ld_weight, int64_t rows,
+                                      int64_t vocab, int64_t width) {
+  using namespace pst_head;
+  return guarded([&]() -> int {
+           return check_sizes(type, d_hidden, ld_hidden, d_weight, ld_weight, rows, vocab, width);
+         }) == PST_OK
+             ? plan_grad(type, d_hidden, ld_hidden, d_weight, ld_weight, std::max<int64_t>(rows, 1), vocab, width).bytes
+             : (int64_t)PST_E_INVALID;
+}
+
+int pst_token_loss_grad(int32_t device, int32_t type, const void* d_hidden, int64_t ld_hidden, const void* d_weight, int64_t ld_weight, int64_t rows,
+                        int64_t vocab, int64_t width, const void* d_targets, int32_t target_bits, int64_t ignore, const float* d_lse,
+                        const float* d_grad_loss, void* d_grad_hidden, int64_t ld_grad_hidden, void* d_grad_weight, int64_t ld_grad_weight,
+                        void* d_workspace, int64_t workspace_bytes, void* stream) {
+  return pst_head::guarded([&] {
+    return pst_head::token_loss_grad(device, type, d_hidden, ld_hidden, d_weight, ld_weight, rows, vocab, width, d_targets, target_bits, ignore,
+                                     d_lse, d_grad_loss, d_grad_hidden, ld_grad_hidden, d_grad_weight, ld_grad_weight, d_workspace, workspace_bytes,
+                                     (hipStream_t)stream);
+  });
+}
+
+int pst_quantize_rows(int32_t device, int32_t type, const void* d_x, int64_t ld_x, int64_t rows, int64_t width, int8_t* d_q, int64_t ld_q,
+                      float* d_scale, void* stream) {
+  return pst_head::guarded(
+      [&] { return pst_head::quantize_rows(device, type, d_x, ld_x, rows, width, d_q, ld_q, d_scale, (hipStream_t)stream); });
+}
+
+int64_t pst_token_scores_i8_workspace(int32_t type, const void* d_hidden, int64_t ld_hidden, const int8_t* d_weight, int64_t ld_weight, int64_t rows,
+                                      int64_t vocab, int64_t width) {
+  using namespace pst_head;
+  return guarded([&]() -> int {
+           return check_scores(type, d_hidden, ld_hidden, d_weight, ld_weight, rows, vocab, width);
+         }) == PST_OK
+             ? plan_scores(d_weight, ld_weight, rows, vocab, width).bytes
+             : (int64_t)PST_E_INVALID;
+}
+
+int pst_token_scores_i8(int32_t device, int32_t type, const void* d_hidden, int64_t ld_hidden, const int8_t* d_weight, int64_t ld_weight,
+                        const float* d_weight_scale, int64_t rows, int64_t vocab, int64_t width, int32_t out_type, void* d_scores, int64_t ld_scores,
+                        void* d_workspace, int64_t workspace_bytes, void* stream) {
+  return pst_head::guarded([&] {
+    return pst_head::token_scores_i8(device, type, d_hidden, ld_hidden, d_weight, ld_weight, d_weight_scale, rows, vocab, width, out_type, d_scores,
+                                     ld_scores, d_workspace, workspace_bytes, (hipStream_t)stream);
+  });
+}
+
+}  // extern "C"

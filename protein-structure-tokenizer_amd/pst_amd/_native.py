@@ -33,6 +33,7 @@ class _ModelDesc(ctypes.Structure):
 
 
 _lib = None
+shares_torch_runtime = False  # libpst loaded after torch opened the GPU: one HIP runtime serves both
 EXPORTS = ("pst_param_count", "pst_create", "pst_destroy", "pst_last_error", "pst_create_error",
            "pst_tokenize", "pst_tokenize_f32", "pst_tokenize_device", "pst_aux", "pst_codebook_aux", "pst_sync",
            "pst_stream", "pst_debug_fetch", "pst_set_timing", "pst_get_timing", "pst_device_count",
@@ -42,7 +43,9 @@ EXPORTS = ("pst_param_count", "pst_create", "pst_destroy", "pst_last_error", "ps
            "pst_decoder_create_error", "pst_decoder_decode", "pst_decoder_decode_ex", "pst_decoder_debug",
            "pst_build_graph", "pst_clock_counters", "pst_set_clock_counters", "pst_pdb_batch_copy_f32",
            "pst_decoder_set_timing", "pst_decoder_get_timing", "pst_tokenize_pdb_batch",
-           "pst_tokenize_pdb_files", "pst_pdb_files_host_parsed")
+           "pst_tokenize_pdb_files", "pst_pdb_files_host_parsed", "pst_head_error", "pst_token_loss_workspace",
+           "pst_token_loss", "pst_token_loss_grad_workspace", "pst_token_loss_grad", "pst_quantize_rows",
+           "pst_token_scores_i8_workspace", "pst_token_scores_i8")
 STAGES = ("prep", "knn", "mpnn0", "mpnn1", "mpnn2", "down")
 
 
@@ -61,14 +64,15 @@ def _init_torch_hip_first():
 
 def lib():
     """Load libpst.so (raises if it was not built)."""
-    global _lib
+    global _lib, shares_torch_runtime
     if _lib is None:
         if not os.path.exists(LIB_PATH):
             raise PstError(f"libpst.so not found at {LIB_PATH}: build it with "
                            "`make -C protein-structure-tokenizer_amd/csrc` (no CPU fallback exists)")
         _init_torch_hip_first()
+        shares_torch_runtime = "torch" in sys.modules
         L = ctypes.CDLL(LIB_PATH)
-        P = ctypes.c_void_p
+        P, I, Q = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
         L.pst_param_count.restype = ctypes.c_size_t
         L.pst_param_count.argtypes = [ctypes.c_int32]
         L.pst_create.argtypes = [ctypes.c_int32, ctypes.POINTER(_ModelDesc), P, ctypes.c_size_t, ctypes.POINTER(P)]
@@ -97,9 +101,22 @@ def lib():
                          ("pst_decoder_set_timing", [P, ctypes.c_int32]), ("pst_decoder_get_timing", [P, P]),
                          ("pst_tokenize_pdb_batch", [P, P, P, P, P]),
                          ("pst_tokenize_pdb_files", [P, P, ctypes.c_int32, ctypes.c_int32, P, ctypes.c_int64, P, P, P]),
-                         ("pst_pdb_files_host_parsed", [P])):
+                         ("pst_pdb_files_host_parsed", [P]),
+                         # the token head (pst_amd.head): absent from older libraries too
+                         ("pst_head_error", []),
+                         ("pst_token_loss_workspace", [I, P, Q, P, Q, Q, Q, Q]),
+                         ("pst_token_loss", [I, I, P, Q, P, Q, Q, Q, Q, P, I, Q, P, P, P, Q, P]),
+                         ("pst_token_loss_grad_workspace", [I, P, Q, P, Q, Q, Q, Q]),
+                         ("pst_token_loss_grad", [I, I, P, Q, P, Q, Q, Q, Q, P, I, Q, P, P, P, Q, P, Q, P, Q, P]),
+                         ("pst_quantize_rows", [I, I, P, Q, Q, Q, P, Q, P, P]),
+                         ("pst_token_scores_i8_workspace", [I, P, Q, P, Q, Q, Q, Q]),
+                         ("pst_token_scores_i8", [I, I, P, Q, P, Q, P, Q, Q, Q, I, P, Q, P, Q, P])):
             if hasattr(L, name):
                 getattr(L, name).argtypes = at
+                if name.endswith("_workspace"):
+                    getattr(L, name).restype = Q
+        if hasattr(L, "pst_head_error"):
+            L.pst_head_error.restype = ctypes.c_char_p
         L.pst_pdb_parse_files.argtypes = [P, ctypes.c_int32, ctypes.c_char, ctypes.c_int32, ctypes.POINTER(P)]
         L.pst_pdb_parse_strings.argtypes = [P, P, ctypes.c_int32, ctypes.c_char, ctypes.c_int32, ctypes.POINTER(P)]
         L.pst_pdb_batch_sizes.argtypes = [P, P, P]
