@@ -38,6 +38,9 @@ __device__ __forceinline__ uint32_t bits16(float v, int type) {
   if (type == PST_BF16) return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)v);
   return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v);
 }
+__device__ __forceinline__ uint32_t pack2(float a, float b, int type) { return bits16(a, type) | bits16(b, type) << 16; }
+// what a 16-bit float leaves of v
+__device__ __forceinline__ float rest16(float v) { return fabsf(v) <= 65504.0f ? v - (float)(_Float16)v : 0.0f; }
 // four neighbours of an output row, `n` of them valid
 __device__ __forceinline__ void store4(void* p, int type, int64_t i, const float* v, int n, bool wide) {
   if (type == PST_F32) {
@@ -144,9 +147,7 @@ __global__ __launch_bounds__(256) void k_pack(PackArgs a) {
           const float v = ldexpf(((const float*)a.src)[r * a.ld + c + j], e);
           const _Float16 h = (_Float16)v;
           hi[j] = __builtin_bit_cast(uint16_t, h);
-          // an infinity or NaN stands in hi alone
-          const float rest = fabsf(v) <= 65504.0f ? v - (float)h : 0.0f;
-          lo[j] = __builtin_bit_cast(uint16_t, (_Float16)rest);
+          lo[j] = __builtin_bit_cast(uint16_t, (_Float16)rest16(v));  // an infinity or NaN stands in hi alone
         } else {
           hi[j] = ((const uint16_t*)a.src)[r * a.ld + c + j];
         }
@@ -190,63 +191,96 @@ enum Kind { LOSS, DLOGIT, DX, DW, SCORES };
 
 template <class T>
 struct Place {
-  int m0, n0, z, lane, h, col, mw, nw;  // mw, nw: this wave's first row and column
+  int m0, n0, z, lane, col, mwave, mw, nw;  // mwave, nw: this wave's first row and column, mw: this lane's first row
   __device__ __forceinline__ Place(const GemmArgs& g) {
     int m, n;
     place(blockIdx.x, g.nm * g.nn * g.nz, g.nm, g.nn, g.gm, m, n, z);
     m0 = m * T::BM;
     n0 = n * T::BN;
     lane = threadIdx.x & 63;
-    h = lane >> 5;
-    col = lane & 31;
-    const int wave = threadIdx.x >> 6;
-    mw = m0 + (wave / T::WN) * T::MI * 32;
-    nw = n0 + (wave % T::WN) * T::NI * 32;
+    col = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    mwave = m0 + (wave / T::WN) * T::MI * 16;
+    mw = mwave + 4 * (lane >> 4);
+    nw = n0 + (wave % T::WN) * T::NI * 16;
   }
 };
+
+template <class T>
+__device__ __forceinline__ void unscale(f32x4 (&acc)[T::MI][T::NI], float mul) {
+#pragma unroll
+  for (int i = 0; i < T::MI; ++i)
+#pragma unroll
+    for (int j = 0; j < T::NI; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[i][j][r] *= mul;
+}
+
+// Two blocks' packed 16-bit values (w[u][q]: block u, the lane's values 2q and 2q + 1) to 32 consecutive columns of the
+// lane's row, whose first is at `to`: the exchange of odd and even 16-lane groups leaves 16 consecutive bytes in a lane.
+__device__ __forceinline__ void store_pair(char* to, const uint32_t (&w)[2][2], int lane, bool row = true) {
+  const auto x = __builtin_amdgcn_permlane16_swap(w[0][0], w[1][0], false, false);
+  const auto y = __builtin_amdgcn_permlane16_swap(w[0][1], w[1][1], false, false);
+  const int g = lane >> 4;
+  if (row) *(uint4*)(to + (g & 1) * 32 + (g >> 1) * 16) = make_uint4(x[0], y[0], x[1], y[1]);
+}
+
+// sums over the four lanes that hold a column
+__device__ __forceinline__ float col_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16));
+  return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float col_sum(float v) {
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
 
 template <int E, class T>
 __global__ __launch_bounds__(T::THREADS) void k_loss(GemmArgs g) {
   extern __shared__ char smem[];
   const Place<T> p(g);
-  typename Mma<E>::Acc acc[T::MI][T::NI];
+  f32x4 acc[T::MI][T::NI];
   multiply<E, T, false, false>(acc, g.A, g.B, g.k, p.m0, p.n0, 0, g.steps, smem);
-  const float mul = g.ua ? *g.ua * *g.ub : 1.0f;
-  float2* sm = (float2*)smem;  // [WM][BN]
-#pragma unroll
-  for (int j = 0; j < T::NI; ++j) {
-    const int n = p.nw + 32 * j + p.col;
-    float mx = -__builtin_inff();
+  if (g.ua) unscale<T>(acc, *g.ua * *g.ub);
+  if (p.mwave + T::MI * 16 > g.M) {  // rows behind the vocabulary's last
 #pragma unroll
     for (int i = 0; i < T::MI; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int m = p.mw + 32 * i + 8 * (r >> 2) + 4 * p.h + (r & 3);
-        float v = acc[i][j][r] * mul;
-        v = m < g.M ? v : -__builtin_inff();
-        acc[i][j][r] = v;
-        mx = fmaxf(mx, v);
-      }
-    mx = fmaxf(mx, __shfl_xor(mx, 32));
+      for (int r = 0; r < 4; ++r)
+        if (p.mw + 16 * i + r >= g.M) {
+#pragma unroll
+          for (int j = 0; j < T::NI; ++j) acc[i][j][r] = -__builtin_inff();
+        }
+  }
+  float2* sm = (float2*)smem;  // [WM][BN]
+#pragma unroll
+  for (int j = 0; j < T::NI; ++j) {
+    const int n = p.nw + 16 * j + p.col;
+    float mx = acc[0][j][0];
+#pragma unroll
+    for (int i = 0; i < T::MI; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) mx = fmaxf(mx, acc[i][j][r]);
+    mx = col_max(mx);
     const float base = mx == -__builtin_inff() ? 0.0f : mx * LOG2E;
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < T::MI; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sum += exp2_fast(__builtin_fmaf(acc[i][j][r], LOG2E, -base));
-    sum += __shfl_xor(sum, 32);
+      for (int r = 0; r < 4; ++r) sum += exp2_fast(__builtin_fmaf(acc[i][j][r], LOG2E, -base));
+    sum = col_sum(sum);
     // the target's logit, where it is among this wave's rows
     bool counts = false;
     const int t = n < g.N ? target_of(g.targets, n, counts) : -1;
-    const int at = t - p.mw;
-    if (__any(t >= 0 && at >= 0 && at < T::MI * 32)) {
+    if (__any(t >= p.mwave && t < p.mwave + T::MI * 16)) {
+      const int at = t < 0 ? -1 : t - p.mw;
 #pragma unroll
       for (int i = 0; i < T::MI; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (t >= 0 && at == 32 * i + 8 * (r >> 2) + 4 * p.h + (r & 3)) g.tlogit[n] = acc[i][j][r];
+        for (int r = 0; r < 4; ++r)
+          if (at == 16 * i + r) g.tlogit[n] = acc[i][j][r];
     }
-    if (p.h == 0) sm[((threadIdx.x >> 6) / T::WN) * T::BN + (n - p.n0)] = make_float2(mx, sum);
+    if (p.lane < 16) sm[((threadIdx.x >> 6) / T::WN) * T::BN + (n - p.n0)] = make_float2(mx, sum);
   }
   __syncthreads();
   for (int c = threadIdx.x; c < T::BN; c += T::THREADS) {
@@ -304,13 +338,14 @@ template <int E, class T>
 __global__ __launch_bounds__(T::THREADS) void k_dlogit(GemmArgs g) {
   extern __shared__ char smem[];
   const Place<T> p(g);
-  typename Mma<E>::Acc acc[T::MI][T::NI];
+  f32x4 acc[T::MI][T::NI];
   multiply<E, T, false, false>(acc, g.A, g.B, g.k, p.m0, p.n0, 0, g.steps, smem);
-  const float mul = g.ua ? *g.ua * *g.ub : 1.0f;
+  if (g.ua) unscale<T>(acc, *g.ua * *g.ub);
   const float gs = *g.gscale;
+  const bool edge = p.mwave + T::MI * 16 > g.M;
 #pragma unroll
   for (int j = 0; j < T::NI; ++j) {
-    const int n = p.nw + 32 * j + p.col;
+    const int n = p.nw + 16 * j + p.col;
     bool counts = false;
     int t = -1;
     float c = 0.0f, lse = 0.0f;
@@ -321,34 +356,46 @@ __global__ __launch_bounds__(T::THREADS) void k_dlogit(GemmArgs g) {
         lse = g.lse[n];
       }
     }
-    const int at = t < 0 ? -1 : t - g.v0 - p.mw;
-    const bool here = __any(at >= 0 && at < T::MI * 32);
 #pragma unroll
     for (int i = 0; i < T::MI; ++i)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int rel = 32 * i + 8 * q + 4 * p.h;
-        float d[4];
+      for (int r = 0; r < 4; ++r) acc[i][j][r] = exp2_fast((acc[i][j][r] - lse) * LOG2E);
+    t -= g.v0;
+    if (__any(t >= p.mwave && t < p.mwave + T::MI * 16)) {
+      const int at = t - p.mw;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          d[r] = exp2_fast((acc[i][j][4 * q + r] * mul - lse) * LOG2E);
-          if (here && at == rel + r) d[r] -= 1.0f;
-          d[r] = counts && p.mw + rel + r < g.M ? d[r] * c : 0.0f;
-        }
-        char* to = g.D + ((int64_t)n * g.ldd + p.mw + rel) * 2;
-        const uint32_t b0 = bits16(d[0], g.dtype), b1 = bits16(d[1], g.dtype), b2 = bits16(d[2], g.dtype), b3 = bits16(d[3], g.dtype);
-        *(uint2*)to = make_uint2(b0 | b1 << 16, b2 | b3 << 16);
-        if (g.dplanes == 2) {
-          const uint32_t hb[4] = {b0, b1, b2, b3};
-          uint32_t lb[4];
+      for (int i = 0; i < T::MI; ++i)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float hv = (float)__builtin_bit_cast(_Float16, (uint16_t)hb[r]);
-            lb[r] = bits16(fabsf(d[r]) <= 65504.0f ? d[r] - hv : 0.0f, PST_F16);
-          }
-          *(uint2*)(to + g.dplane) = make_uint2(lb[0] | lb[1] << 16, lb[2] | lb[3] << 16);
-        }
+        for (int r = 0; r < 4; ++r)
+          if (at == 16 * i + r) acc[i][j][r] -= 1.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < T::MI; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[i][j][r] = counts ? acc[i][j][r] * c : 0.0f;
+    if (edge) {
+#pragma unroll
+      for (int i = 0; i < T::MI; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[i][j][r] = p.mw + 16 * i + r < g.M ? acc[i][j][r] : 0.0f;
+    }
+    char* to = g.D + ((int64_t)n * g.ldd + p.mwave) * 2;
+#pragma unroll
+    for (int i = 0; i < T::MI; i += 2) {
+      uint32_t w[2][2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) w[u][q] = pack2(acc[i + u][j][2 * q], acc[i + u][j][2 * q + 1], g.dtype);
+      store_pair(to + i * 32, w, p.lane);
+      if (g.dplanes == 2) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) w[u][q] = pack2(rest16(acc[i + u][j][2 * q]), rest16(acc[i + u][j][2 * q + 1]), PST_F16);
+        store_pair(to + g.dplane + i * 32, w, p.lane);
       }
+    }
   }
 }
 
@@ -357,30 +404,28 @@ template <int E, class T>
 __global__ __launch_bounds__(T::THREADS) void k_dx(GemmArgs g) {
   extern __shared__ char smem[];
   const Place<T> p(g);
-  typename Mma<E>::Acc acc[T::MI][T::NI];
+  f32x4 acc[T::MI][T::NI];
   const int s0 = (int)((int64_t)g.steps * p.z / g.nz), s1 = (int)((int64_t)g.steps * (p.z + 1) / g.nz);
   multiply<E, T, true, false>(acc, g.A, g.B, g.k, p.m0, p.n0, s0, s1, smem);
   float* out = (float*)g.out + p.z * g.zstride;
 #pragma unroll
   for (int j = 0; j < T::NI; ++j) {
-    const int n = p.nw + 32 * j + p.col;
+    const int n = p.nw + 16 * j + p.col;
 #pragma unroll
-    for (int i = 0; i < T::MI; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int m = p.mw + 32 * i + 8 * q + 4 * p.h;
-        if (m >= g.ldo) continue;
-        f32x4* to = (f32x4*)(out + (int64_t)n * g.ldo + m);
-        f32x4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-        if (g.add) {
-          const f32x4 o = *to;
-          v.x += o.x;
-          v.y += o.y;
-          v.z += o.z;
-          v.w += o.w;
-        }
-        *to = v;
+    for (int i = 0; i < T::MI; ++i) {
+      const int m = p.mw + 16 * i;
+      if (m >= g.ldo) continue;
+      f32x4* to = (f32x4*)(out + (int64_t)n * g.ldo + m);
+      f32x4 v = acc[i][j];
+      if (g.add) {
+        const f32x4 o = *to;
+        v.x += o.x;
+        v.y += o.y;
+        v.z += o.z;
+        v.w += o.w;
       }
+      *to = v;
+    }
   }
 }
 
@@ -417,28 +462,48 @@ __global__ __launch_bounds__(256) void k_finish(FinishArgs a) {
   }
 }
 
+// A wave's blocks as rows of a matrix of 32- or 16-bit floats: column n of the product is row `row0 + n` of the output,
+// which has M columns. `wide`: rows and base allow 16-byte stores (of 16-bit values: two blocks make 16 bytes a lane).
+template <class T>
+__device__ __forceinline__ void store_rows(const f32x4 (&acc)[T::MI][T::NI], const GemmArgs& g, const Place<T>& p, int64_t row0) {
+  const bool whole = g.wide && p.mwave + T::MI * 16 <= g.M;
+#pragma unroll
+  for (int j = 0; j < T::NI; ++j) {
+    const int n = p.nw + 16 * j + p.col;
+    const bool row = n < g.N;
+    const int64_t at = (row0 + n) * g.ldo;
+    if (whole && g.otype != PST_F32) {
+      char* to = (char*)g.out + (at + p.mwave) * 2;
+#pragma unroll
+      for (int i = 0; i < T::MI; i += 2) {
+        uint32_t w[2][2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) w[u][q] = pack2(acc[i + u][j][2 * q], acc[i + u][j][2 * q + 1], g.otype);
+        store_pair(to + i * 32, w, p.lane, row);
+      }
+    } else if (row) {
+#pragma unroll
+      for (int i = 0; i < T::MI; ++i) {
+        const int m = p.mw + 16 * i;
+        if (m >= g.M) continue;
+        const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+        store4(g.out, g.otype, at + m, v, g.M - m, g.wide);
+      }
+    }
+  }
+}
+
 // rows v0 ... of dW: m = column, n = vocabulary row of the piece, k = position
 template <int E, class T>
 __global__ __launch_bounds__(T::THREADS) void k_dw(GemmArgs g) {
   extern __shared__ char smem[];
   const Place<T> p(g);
-  typename Mma<E>::Acc acc[T::MI][T::NI];
+  f32x4 acc[T::MI][T::NI];
   multiply<E, T, true, true>(acc, g.A, g.B, g.k, p.m0, p.n0, 0, g.steps, smem);
-  const float mul = *g.ua * (g.ub ? *g.ub : 1.0f);
-#pragma unroll
-  for (int j = 0; j < T::NI; ++j) {
-    const int n = p.nw + 32 * j + p.col;
-    if (n >= g.N) continue;
-#pragma unroll
-    for (int i = 0; i < T::MI; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int m = p.mw + 32 * i + 8 * q + 4 * p.h;
-        if (m >= g.M) continue;
-        const float v[4] = {acc[i][j][4 * q] * mul, acc[i][j][4 * q + 1] * mul, acc[i][j][4 * q + 2] * mul, acc[i][j][4 * q + 3] * mul};
-        store4(g.out, g.otype, (int64_t)(g.v0 + n) * g.ldo + m, v, g.M - m, g.wide);
-      }
-  }
+  unscale<T>(acc, *g.ua * (g.ub ? *g.ub : 1.0f));
+  store_rows<T>(acc, g, p, g.v0);
 }
 
 // 8-bit scores: m = vocabulary row, n = position
@@ -446,25 +511,26 @@ template <class T>
 __global__ __launch_bounds__(T::THREADS) void k_scores(GemmArgs g) {
   extern __shared__ char smem[];
   const Place<T> p(g);
-  typename Mma<I8>::Acc acc[T::MI][T::NI];
-  multiply<I8, T, false, false>(acc, g.A, g.B, g.k, p.m0, p.n0, 0, g.steps, smem);
+  i32x4 sums[T::MI][T::NI];
+  multiply<I8, T, false, false>(sums, g.A, g.B, g.k, p.m0, p.n0, 0, g.steps, smem);
+  f32x4 acc[T::MI][T::NI];
 #pragma unroll
   for (int j = 0; j < T::NI; ++j) {
-    const int n = p.nw + 32 * j + p.col;
-    if (n >= g.N) continue;
-    const float sn = g.sn[n];
+    const float sn = g.sn[min(p.nw + 16 * j + p.col, g.N - 1)];
 #pragma unroll
     for (int i = 0; i < T::MI; ++i)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int m = p.mw + 32 * i + 8 * q + 4 * p.h;
-        if (m >= g.M) continue;
-        float v[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = (float)acc[i][j][4 * q + r] * sn * g.sm[min(m + r, g.M - 1)];
-        store4(g.out, g.otype, (int64_t)n * g.ldo + m, v, g.M - m, g.wide);
-      }
+      for (int r = 0; r < 4; ++r) acc[i][j][r] = (float)sums[i][j][r] * sn;
   }
+#pragma unroll
+  for (int i = 0; i < T::MI; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float sv = g.sm[min(p.mw + 16 * i + r, g.M - 1)];
+#pragma unroll
+      for (int j = 0; j < T::NI; ++j) acc[i][j][r] *= sv;
+    }
+  store_rows<T>(acc, g, p, 0);
 }
 
 struct QuantArgs {
@@ -593,7 +659,10 @@ bool in_place(const void* p, int64_t ld_bytes, int64_t row_bytes) {
   return ((uintptr_t)p & 15) == 0 && ld_bytes % 16 == 0 && row_bytes % 16 == 0;
 }
 
-using T256 = Tile<256, 256, 2, 4>;
+#ifndef T256W
+#define T256W 2, 4
+#endif
+using T256 = Tile<256, 256, T256W>;
 using T128 = Tile<128, 128, 2, 2>;
 using T64 = Tile<64, 64, 2, 2>;
 enum TileId { TILE64 = 0, TILE128 = 1, TILE256 = 2 };
@@ -912,7 +981,7 @@ int token_loss_grad(int device, int type, const void* x, int64_t ldx, const void
       d.out = dw;
       d.ldo = lddw;
       d.otype = type;
-      d.wide = lddw % 4 == 0 && ((uintptr_t)dw & (type == PST_F32 ? 15 : 7)) == 0;
+      d.wide = lddw % (16 / e) == 0 && ((uintptr_t)dw & 15) == 0;
       HEADCHK(launch_gemm(DW, p.elem, tile_for(width, nv, cus), d, st));
     }
   }
@@ -1003,7 +1072,7 @@ int token_scores_i8(int device, int type, const void* x, int64_t ldx, const int8
   g.out = out;
   g.ldo = ldo;
   g.otype = otype;
-  g.wide = ldo % 4 == 0 && ((uintptr_t)out & (otype == PST_F32 ? 15 : 7)) == 0;
+  g.wide = ldo % (16 / size_of(otype)) == 0 && ((uintptr_t)out & 15) == 0;
   g.sn = (const float*)(ws + p.scale);
   g.sm = wscale;
   HEADCHK(launch_gemm(SCORES, I8, tile_for(vocab, rows, cus), g, st));

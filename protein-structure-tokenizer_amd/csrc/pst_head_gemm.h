@@ -1,30 +1,34 @@
 // pst_head_gemm.h — the matrix product under the token head's operators (gfx950 / CDNA4).
 //
-// D[m][n] = sum_k A[m][k] B[n][k] on a BM x BN tile, 16-bit floats (f32 sums) or 8-bit integers (i32 sums),
-// by v_mfma_*_32x32x16 / 32x32x32. Lane l of a wave holds, of each 32x32 block, column n = l & 31 and rows
-// m = 8 (r >> 2) + 4 (l >> 5) + (r & 3), r = 0..15: the operand whose index runs along the outputs' contiguous
-// axis is A (four neighbours in one lane), and a reduction over that axis stays inside a lane.
+// D[m][n] = sum_k A[m][k] B[n][k] on a BM x BN tile, 16-bit floats (f32 sums) or 8-bit integers (i32 sums), by
+// v_mfma_*_16x16x32 / 16x16x64. Lane l of a wave holds, of each 16x16 block, column n = l & 15 and rows
+// m = 4 (l >> 4) + r, r = 0..3: the operand whose index runs along the outputs' contiguous axis is A (four
+// neighbours in one lane), and a reduction over that axis is 32 values in a lane and two lane exchanges.
+//
+// What bounds the large products is power: with operands of random bits the card sustains 2.06 PFLOP/s of bf16
+// 16x16x32 and 1.77 of 32x32x16 (whose sums move twice the bits for each product; 8-bit: 4.04 and 3.40), all from
+// registers. So the small block is used, and bytes are moved as rarely as the registers allow: 128 x 64 a wave.
 //
 // A K-step is 128 bytes of k (64 16-bit values, 128 8-bit ones) of every tile row. Operands are staged by
 // global_load_lds_dwordx4 (global memory to LDS without registers: lane i of the instruction fills 16 bytes
 // at base + 16 i, so what is permuted is the global address each lane reads) in two forms:
 //   ROWS  memory holds k contiguous in each row. LDS: [row][8 chunks of 16 bytes], chunk c of row r at place
-//         c ^ (r & 7): the 32 rows that a fragment read touches at one c lie in all banks.
-//   COLS  memory holds the tile's rows as columns: [k][m]. LDS: [k][m], 64-byte pieces of row k at place
-//         p ^ (k & 3) (p ^ (k >> 1 & 1) for 128-byte rows); ds_read_b64_tr_b16 turns four k-rows of 16 columns
-//         into four consecutive k of one column per lane, so no transposed copy of a matrix is ever made.
+//         c ^ (r >> 1 & 7): 16 rows read at one c fill the 64 banks once.
+//   COLS  memory holds the tile's rows as columns: [k][m]. LDS: [k][m], 32-byte pieces of row k permuted by swizzle(k)
+//         so that the 16 k-rows of a read spread over the banks; ds_read_b64_tr_b16 turns four k-rows of 16
+//         columns into four consecutive k of one column per lane: no transposed copy of a matrix is ever made.
 // k that passes the end: the last K-step reads the last valid chunk or row again; the caller sees to it that
 // the other operand holds zeros there.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace pst_head {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef int i32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -36,23 +40,23 @@ template <int E>
 struct Mma;
 template <>
 struct Mma<BF16> {
-  typedef f32x16 Acc;
+  typedef f32x4 Acc;
   static __device__ __forceinline__ Acc mma(i32x4 a, i32x4 b, Acc c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
 };
 template <>
 struct Mma<F16> {
-  typedef f32x16 Acc;
+  typedef f32x4 Acc;
   static __device__ __forceinline__ Acc mma(i32x4 a, i32x4 b, Acc c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
 };
 template <>
 struct Mma<I8> {
-  typedef i32x16 Acc;
+  typedef i32x4 Acc;
   static __device__ __forceinline__ Acc mma(i32x4 a, i32x4 b, Acc c) {
-    return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
   }
 };
 
@@ -91,6 +95,19 @@ __device__ __forceinline__ void landed_and_met() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
+// The same with the last N loads still in flight.
+template <int N>
+__device__ __forceinline__ void landed_but() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// COLS: what the number of a 32-byte piece of LDS row k is xored with, rows of RT bytes. A read takes k-rows
+// 8 g + i (g, i = 0..3) and one piece of each: eight places of the 256-byte bank row, each twice.
+template <int RT>
+__device__ __forceinline__ int swizzle(int k) {
+  return RT == 128 ? (k >> 1 & 1) | (k >> 2 & 2) : (k & 3) | (k >> 1 & 4);
+}
+
 // R: tile rows (m or n); NW: waves that share the loading
 template <int R, bool COLS, int NW>
 struct Stager {
@@ -102,9 +119,9 @@ struct Stager {
   const char* base;  // of the current plane's tile
   int32_t k_bytes;   // ROWS: valid bytes of a row; COLS: valid k-rows
   int64_t ld;
-
-  // swizzle of LDS row k's 64-byte pieces
-  static __device__ __forceinline__ int sw(int k) { return RT == 128 ? (k >> 1) & 1 : k & 3; }
+  const char* src;   // the K-step being loaded, what is valid of it, and where it goes
+  int32_t left = 1 << 30;
+  uint32_t to;
 
   __device__ __forceinline__ void init(const Operand& o, int row0, int lane, int wave) {
     ld = o.ld;
@@ -117,128 +134,174 @@ struct Stager {
       const int r = (wave * NI + j) * PER + lane / (RT / 16);  // LDS row
       const int c = lane % (RT / 16);                          // 16-byte place in it
       if (COLS) {
-        const int col = (((c >> 2) ^ sw(r)) << 6) | ((c & 3) << 4);
+        const int col = (((c >> 1) ^ swizzle<RT>(r)) << 5) | ((c & 1) << 4);
         off[j] = (uint32_t)(r * (int64_t)o.ld) + (uint32_t)min(col, o.bytes - 16 - first);
       } else {
-        off[j] = (uint32_t)(min(r, o.rows - 1 - first) * o.ld) + (uint32_t)((c ^ (r & 7)) << 4);
+        off[j] = (uint32_t)(min(r, o.rows - 1 - first) * o.ld) + (uint32_t)((c ^ (r >> 1 & 7)) << 4);
       }
     }
   }
-  // loads K-step `step` of plane `plane_off` into the LDS tile at `lds`
-  __device__ __forceinline__ void issue(int64_t plane_off, int step, uint32_t lds, int lane, int wave) {
-    const char* b = base + plane_off + (COLS ? (int64_t)min(step * 64, k_bytes - 1) * ld : (int64_t)step * STEP);
-    const int left = COLS ? k_bytes - step * 64 : k_bytes - step * STEP;
-    const uint32_t to = __builtin_amdgcn_readfirstlane(lds + (uint32_t)wave * (NI * 1024));
-    if (left >= (COLS ? 64 : STEP)) {
+  // K-step `step` of plane `plane_off` goes to the LDS tile at `lds`, by one(0) ... one(NI - 1)
+  __device__ __forceinline__ void aim(int64_t plane_off, int step, uint32_t lds, int lane, int wave) {
+    constexpr int WHOLE = COLS ? 64 : STEP;
+    if (left < WHOLE) shift(left, 1, lane, wave);  // a pass behind the first: undo the last K-step's
+    src = base + plane_off + (COLS ? (int64_t)min(step * 64, k_bytes - 1) * ld : (int64_t)step * STEP);
+    left = COLS ? k_bytes - step * 64 : k_bytes - step * STEP;
+    if (left < WHOLE) shift(left, -1, lane, wave);
+    to = __builtin_amdgcn_readfirstlane(lds + (uint32_t)wave * (NI * 1024));
+  }
+  // a K-step of which `valid` (k-rows or bytes) exist: what lies behind reads the last of them
+  __device__ __forceinline__ void shift(int valid, int sign, int lane, int wave) {
 #pragma unroll
-      for (int j = 0; j < NI; ++j) load_lds(b, off[j], to + j * 1024);
-    } else {
-#pragma unroll
-      for (int j = 0; j < NI; ++j) {
-        const int r = (wave * NI + j) * PER + lane / (RT / 16);
-        const int c = lane % (RT / 16);
-        uint32_t o = off[j];
-        if (COLS) {
-          o -= (uint32_t)((int64_t)max(0, r - max(0, left - 1)) * ld);
-        } else {
-          o -= (uint32_t)max(0, ((c ^ (r & 7)) << 4) - (left - 16));
-        }
-        load_lds(b, o, to + j * 1024);
-      }
+    for (int j = 0; j < NI; ++j) {
+      const int r = (wave * NI + j) * PER + lane / (RT / 16);
+      const int c = lane % (RT / 16);
+      const uint32_t d = COLS ? (uint32_t)((int64_t)max(0, r - max(0, valid - 1)) * ld) : (uint32_t)max(0, ((c ^ (r >> 1 & 7)) << 4) - (valid - 16));
+      off[j] += sign > 0 ? d : 0u - d;
     }
   }
+  __device__ __forceinline__ void one(int j) const { load_lds(src, off[j], to + j * 1024); }
 };
 
-// Fragment addresses of one wave: NB 32-row blocks from block `blk0` of the tile
-template <int R, bool COLS, int NB>
+// Fragments of one wave, 16 rows x 64 bytes of k each: block b (from block blk0 of the tile), half s of the K-step
+template <int R, bool COLS>
 struct Reader {
-  uint32_t at[COLS ? NB : 4];
+  uint32_t at[2];
   __device__ __forceinline__ void init(int blk0, int lane) {
+    const int g = lane >> 4, i = lane & 15;
     if (COLS) {
       constexpr int RT = R * 2;
-      const int g = lane >> 4, i = lane & 15;
-      const int k = 8 * (g >> 1) + (i >> 2);
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-        at[b] = k * RT + (((blk0 + b) ^ Stager<R, true, R * STEP / 1024>::sw(k)) << 6) + ((g & 1) << 5) + ((i & 3) << 3);
+      const int k = 8 * g + (i >> 2);
+      at[0] = k * RT + ((blk0 ^ swizzle<RT>(k)) << 5) + ((i & 3) << 3);
     } else {
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
-        at[s] = (blk0 * 32 + (lane & 31)) * STEP + (((2 * s + (lane >> 5)) ^ (lane & 7)) << 4);
+      for (int s = 0; s < 2; ++s) at[s] = (blk0 * 16 + i) * STEP + (((4 * s + g) ^ (i >> 1)) << 4);
     }
   }
-  // block b, 16-byte k piece s of the K-step whose tile is at `tile`
   __device__ __forceinline__ i32x4 get(const char* tile, int b, int s) const {
     if (COLS) {
       constexpr int RT = R * 2;
       typedef __attribute__((address_space(3))) s16x4* P;
-      const char* q = tile + at[b] + s * 16 * RT;
+      const char* q = tile + (at[0] ^ (uint32_t)(b << 5)) + s * 32 * RT;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)q);
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(q + 4 * RT));
       return __builtin_bit_cast(i32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     }
-    return *(const i32x4*)(tile + at[s] + b * 32 * STEP);
+    return *(const i32x4*)(tile + at[s] + b * 16 * STEP);
   }
 };
 
 template <int BM_, int BN_, int WM_, int WN_>
 struct Tile {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NW = WM_ * WN_, THREADS = NW * 64;
-  static constexpr int MI = BM_ / WM_ / 32, NI = BN_ / WN_ / 32;
+  static constexpr int MI = BM_ / WM_ / 16, NI = BN_ / WN_ / 16;  // a wave's 16x16 blocks
   static constexpr int STAGE = (BM_ + BN_) * STEP, LDS = 2 * STAGE;
 };
 
-// The K loop: acc[MI][NI] of this wave. Two LDS stages; the loads of K-step t + 1 fly while t is multiplied.
+// The K loop: acc[MI][NI] of this wave. Two LDS stages: the loads of K-step t + 2 start when all waves have read the
+// last of step t, and fly while t + 1 is multiplied. A K-step is four parts, (k half, half of the wave's rows): each
+// part's fragments are read from LDS while the part before is multiplied, also across the one barrier of a K-step.
 template <int E, class T, bool ACOLS, bool BCOLS>
 __device__ __forceinline__ void multiply(typename Mma<E>::Acc (&acc)[T::MI][T::NI], const Operand& A, const Operand& B,
                                          const KLoop& kl, int m0, int n0, int step0, int step1, char* smem) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / T::WN, wn = wave % T::WN;
+  constexpr int HI = T::MI / 2;
+  // blocks of a wave start at a multiple of their number, so that a COLS read can xor the block into its address
+  static_assert((T::MI & (T::MI - 1)) == 0 && (T::NI & (T::NI - 1)) == 0 && T::MI >= 2 && T::NI >= 2, "wave tile");
   Stager<T::BM, ACOLS, T::NW> sa;
   Stager<T::BN, BCOLS, T::NW> sb;
   sa.init(A, m0, lane, wave);
   sb.init(B, n0, lane, wave);
-  Reader<T::BM, ACOLS, T::MI> ra;
-  Reader<T::BN, BCOLS, T::NI> rb;
+  Reader<T::BM, ACOLS> ra;
+  Reader<T::BN, BCOLS> rb;
   ra.init(wm * T::MI, lane);
   rb.init(wn * T::NI, lane);
 #pragma unroll
   for (int i = 0; i < T::MI; ++i)
 #pragma unroll
-    for (int j = 0; j < T::NI; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
+    for (int j = 0; j < T::NI; ++j) acc[i][j] = {0, 0, 0, 0};
   const uint32_t lds0 = lds_addr(smem);
   const int steps = step1 - step0, total = steps * kl.segs;
   int seg = 0, step = step0;  // what is loaded next
-  auto issue = [&](int stage) {
+  constexpr int LA = Stager<T::BM, ACOLS, T::NW>::NI, LB = Stager<T::BN, BCOLS, T::NW>::NI;
+  auto aim = [&](int stage) {
     const uint32_t to = lds0 + stage * T::STAGE;
-    sa.issue((int64_t)((kl.seg_a >> (2 * seg)) & 3) * A.plane, step, to, lane, wave);
-    sb.issue((int64_t)((kl.seg_b >> (2 * seg)) & 3) * B.plane, step, to + T::BM * STEP, lane, wave);
+    sa.aim((int64_t)((kl.seg_a >> (2 * seg)) & 3) * A.plane, step, to, lane, wave);
+    sb.aim((int64_t)((kl.seg_b >> (2 * seg)) & 3) * B.plane, step, to + T::BM * STEP, lane, wave);
     if (++step == step1) {
       step = step0;
       ++seg;
     }
   };
-  if (total > 0) issue(0);
-  for (int t = 0; t < total; ++t) {
-    landed_and_met();
-    if (t + 1 < total) issue((t + 1) & 1);
-    const char* ta = smem + (t & 1) * T::STAGE;
+  auto load = [&](int i) {
+    if (i < LA) sa.one(i);
+    else sb.one(i - LA);
+  };
+  auto issue = [&](int stage) {
+    aim(stage);
+#pragma unroll
+    for (int i = 0; i < LA + LB; ++i) load(i);
+  };
+  i32x4 a[2][HI], b[2][T::NI];
+  // fragments of part p of the K-step in `stage`
+  auto fetch = [&](int stage, int p) {
+    const char* ta = smem + stage * T::STAGE;
     const char* tb = ta + T::BM * STEP;
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      i32x4 a[T::MI], b[T::NI];
+    for (int i = 0; i < HI; ++i) a[p & 1][i] = ra.get(ta, (p & 1) * HI + i, p >> 1);
+    if ((p & 1) == 0) {
 #pragma unroll
-      for (int i = 0; i < T::MI; ++i) a[i] = ra.get(ta, i, s);
-#pragma unroll
-      for (int j = 0; j < T::NI; ++j) b[j] = rb.get(tb, j, s);
-#pragma unroll
-      for (int i = 0; i < T::MI; ++i)
-#pragma unroll
-        for (int j = 0; j < T::NI; ++j) acc[i][j] = Mma<E>::mma(a[i], b[j], acc[i][j]);
+      for (int j = 0; j < T::NI; ++j) b[p >> 1][j] = rb.get(tb, j, p >> 1);
     }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // multiplies part p; with `more` the loads of a K-step spread between the multiplications, since the unit that takes
+  // them accepts one in 16 clocks of the whole workgroup and a wave behind it would wait with idle matrix cores
+  auto mult = [&](int p, auto more) {
+    constexpr int TOTAL = HI * T::NI;
+#pragma unroll
+    for (int q = 0; q < TOTAL; ++q) {
+      const int i = q / T::NI, j = q % T::NI;
+      acc[(p & 1) * HI + i][j] = Mma<E>::mma(a[p & 1][i], b[p >> 1][j], acc[(p & 1) * HI + i][j]);
+      if constexpr (more.value) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int l = q * (LA + LB) / TOTAL; l < (q + 1) * (LA + LB) / TOTAL; ++l) load(l);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if (total > 0) {
+    issue(0);
+    if (total > 1) {
+      issue(1);
+      landed_but<LA + LB>();
+    } else {
+      landed_and_met();
+    }
+    fetch(0, 0);
   }
+  auto body = [&](int t, auto more, auto next) {
+    fetch(t & 1, 1);
+    mult(0, std::false_type{});
+    fetch(t & 1, 2);
+    mult(1, std::false_type{});
+    fetch(t & 1, 3);
+    mult(2, std::false_type{});
+    // the last fragments of step t are in registers: its stage is free once all waves are here
+    if constexpr (next.value) {
+      landed_and_met();
+      fetch((t + 1) & 1, 0);
+    }
+    if constexpr (more.value) aim(t & 1);
+    mult(3, more);
+  };
+  int t = 0;
+  for (; t + 2 < total; ++t) body(t, std::true_type{}, std::true_type{});
+  if (t + 1 < total) body(t++, std::false_type{}, std::true_type{});
+  if (t < total) body(t, std::false_type{}, std::false_type{});
   landed_and_met();  // the stages are free for the epilogue
 }
 
