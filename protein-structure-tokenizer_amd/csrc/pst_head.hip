@@ -91,72 +91,124 @@ struct AmaxArgs {
   int32_t width;
   float* part;  // [2][AMAX_BLOCKS]
 };
-__global__ __launch_bounds__(256) void k_amax(AmaxArgs a) {
+// the largest finite magnitude of each of two matrices, in AMAX_BLOCKS parts; a wave a row
+__global__ __launch_bounds__(1024) void k_amax(AmaxArgs a) {
   const int t = blockIdx.x / AMAX_BLOCKS, b = blockIdx.x % AMAX_BLOCKS;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   float m = 0.0f;
-  for (int64_t r = b * 4 + wave; r < a.rows[t]; r += AMAX_BLOCKS * 4) {
+  for (int64_t r = b * 16 + wave; r < a.rows[t]; r += AMAX_BLOCKS * 16) {
     const float* row = a.p[t] + r * a.ld[t];
+#pragma unroll 8
     for (int k = lane; k < a.width; k += 64) m = fmaxf(m, finite_abs(row[k]));
   }
 #pragma unroll
   for (int s = 32; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
-  __shared__ float sm[4];
+  __shared__ float sm[16];
   if (lane == 0) sm[wave] = m;
   __syncthreads();
-  if (threadIdx.x == 0) a.part[t * AMAX_BLOCKS + b] = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 16; ++w) m = fmaxf(m, sm[w]);
+    a.part[t * AMAX_BLOCKS + b] = m;
+  }
 }
 
-struct PackArgs {
-  const void* src;
+// A matrix copied into rows of whole K-steps with zeros behind, 32-bit values split into two planes
+struct PackJob {
+  const void* src;         // null: nothing to do
   int64_t ld;
   int64_t rows, rows_pad;  // rows beyond `rows` are zeros
-  int32_t width, width_pad;
-  int32_t type;
   char* dst;               // 16-bit [planes][rows_pad][width_pad]
   int64_t plane;           // bytes
   const float* part;       // 32-bit: the tensor's AMAX_BLOCKS maxima
   float* unscale;          // 32-bit: 2^-e
-  Targets targets;         // p set: rows whose position does not count are zeros
+  int32_t zero_rows;       // rows whose position does not count are zeros
+  int32_t wide;            // the source allows 16-byte loads
 };
-// copies a matrix into rows of whole K-steps (zeros behind), splitting 32-bit values
+struct PackArgs {
+  PackJob job[2];
+  int32_t blocks[2];  // workgroups of each job; one more makes the scale of the logits' gradient if gloss is set
+  int32_t width, width_pad, type;
+  Targets targets;
+  // D of 16-bit floats with a short exponent (and of the halves of a split one) is scaled by the power of two that
+  // brings the largest |g_n| to 2^13 ... 2^14; gscale[0] = that power, gscale[1] = its inverse
+  const float* gloss;
+  int64_t n;
+  float* gscale;
+};
+__device__ __forceinline__ float block_max(float m, float* sm) {
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
+  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
+  __syncthreads();
+  return fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+}
 __global__ __launch_bounds__(256) void k_pack(PackArgs a) {
-  const int64_t groups = (int64_t)a.rows_pad * (a.width_pad / 8);
-  int e = 0;
-  if (a.type == PST_F32) {
-    float m = a.part[threadIdx.x];
-#pragma unroll
-    for (int s = 32; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
-    __shared__ float sm[4];
-    if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
-    __syncthreads();
-    e = split_exp(fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3])));
-    if (blockIdx.x == 0 && threadIdx.x == 0) *a.unscale = ldexpf(1.0f, -e);
-  }
-  for (int64_t g = blockIdx.x * (int64_t)256 + threadIdx.x; g < groups; g += (int64_t)gridDim.x * 256) {
-    const int64_t r = g / (a.width_pad / 8);
-    const int c = (int)(g - r * (a.width_pad / 8)) * 8;
-    bool keep = r < a.rows;
-    if (keep && a.targets.p) (void)target_of(a.targets, r, keep);
-    uint32_t hi[8], lo[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      hi[j] = lo[j] = 0;
-      if (keep && c + j < a.width) {
-        if (a.type == PST_F32) {
-          const float v = ldexpf(((const float*)a.src)[r * a.ld + c + j], e);
-          const _Float16 h = (_Float16)v;
-          hi[j] = __builtin_bit_cast(uint16_t, h);
-          lo[j] = __builtin_bit_cast(uint16_t, (_Float16)rest16(v));  // an infinity or NaN stands in hi alone
-        } else {
-          hi[j] = ((const uint16_t*)a.src)[r * a.ld + c + j];
-        }
-      }
+  __shared__ float sm[4];
+  const int which = (int)blockIdx.x < a.blocks[0] ? 0 : 1;
+  const int block = (int)blockIdx.x - (which ? a.blocks[0] : 0);
+  if (which && block >= a.blocks[1]) {
+    float m = 0.0f;
+    for (int64_t i = threadIdx.x; i < a.n; i += 256) {
+      bool counts;
+      (void)target_of(a.targets, i, counts);
+      if (counts) m = fmaxf(m, finite_abs(a.gloss[i]));
     }
-    char* d = a.dst + (r * a.width_pad + c) * 2;
-    *(uint4*)d = make_uint4(hi[0] | hi[1] << 16, hi[2] | hi[3] << 16, hi[4] | hi[5] << 16, hi[6] | hi[7] << 16);
-    if (a.type == PST_F32)
-      *(uint4*)(d + a.plane) = make_uint4(lo[0] | lo[1] << 16, lo[2] | lo[3] << 16, lo[4] | lo[5] << 16, lo[6] | lo[7] << 16);
+    m = block_max(m, sm);
+    if (threadIdx.x == 0) {
+      const int e = max(-100, min(100, split_exp(m)));
+      a.gscale[0] = ldexpf(1.0f, e);
+      a.gscale[1] = ldexpf(1.0f, -e);
+    }
+    return;
+  }
+  const PackJob& p = a.job[which];
+  const bool f32 = a.type == PST_F32;
+  int e = 0;
+  if (f32) {
+    e = split_exp(block_max(p.part[threadIdx.x], sm));
+    if (block == 0 && threadIdx.x == 0) *p.unscale = ldexpf(1.0f, -e);
+  }
+  const int per = a.width_pad / 8;
+  const int64_t groups = p.rows_pad * per;
+  for (int64_t g = block * (int64_t)256 + threadIdx.x; g < groups; g += (int64_t)a.blocks[which] * 256) {
+    const int64_t r = g / per;
+    const int c = (int)(g - r * per) * 8;
+    bool keep = r < p.rows;
+    if (keep && p.zero_rows) (void)target_of(a.targets, r, keep);
+    char* d = p.dst + (r * a.width_pad + c) * 2;
+    if (!f32) {
+      uint4 v = make_uint4(0, 0, 0, 0);
+      const uint16_t* src = (const uint16_t*)p.src + r * p.ld + c;
+      if (keep && p.wide && c + 8 <= a.width) {
+        v = *(const uint4*)src;
+      } else if (keep) {
+        uint32_t h[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[j] = c + j < a.width ? src[j] : 0;
+        v = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+      }
+      *(uint4*)d = v;
+    } else {
+      float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      const float* src = (const float*)p.src + r * p.ld + c;
+      if (keep && p.wide && c + 8 <= a.width) {
+        const f32x4 lo = *(const f32x4*)src, hi = *(const f32x4*)(src + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = lo[j], v[4 + j] = hi[j];
+      } else if (keep) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = c + j < a.width ? src[j] : 0.0f;
+      }
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float x = ldexpf(v[2 * j], e), y = ldexpf(v[2 * j + 1], e);
+        hi[j] = pack2(x, y, PST_F16);
+        lo[j] = pack2(rest16(x), rest16(y), PST_F16);  // an infinity or NaN stands in hi alone
+      }
+      *(uint4*)d = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      *(uint4*)(d + p.plane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
   }
 }
 
@@ -175,26 +227,34 @@ struct GemmArgs {
   float2* part;        // loss: [nm][N] (maximum, sum)
   float* tlogit;       // loss: [N]
   const float *lse, *gloss;
-  const float* gscale; // power of two on D (device)
+  const float* gscale; // power of two on D (device; null: 1)
   char* D;             // [planes][rows][ldd] 16-bit
   int64_t dplane, ldd; // bytes, elements
   int32_t dtype, dplanes, v0;
   // matrix outputs
   void* out;
   int64_t ldo;
-  int32_t otype, wide, add;
-  int64_t zstride;     // dx: elements between the pieces' partial sums
+  int32_t otype, wide;
+  // outputs in parts of the K loop: 32-bit [nz][..][ldp], added to what is there with `add`
+  float* part_out;
+  int64_t ldp, zstride;
+  int32_t add;
   const float *sn, *sm; // scores: scales of the rows of B and of A
 };
 
-enum Kind { LOSS, DLOGIT, DX, DW, SCORES };
+struct GradArgs {
+  GemmArgs dx, dw;
+  int32_t dx_tiles;
+};
+
+enum Kind { LOSS, DLOGIT, SCORES };
 
 template <class T>
 struct Place {
   int m0, n0, z, lane, col, mwave, mw, nw;  // mwave, nw: this wave's first row and column, mw: this lane's first row
-  __device__ __forceinline__ Place(const GemmArgs& g) {
+  __device__ __forceinline__ Place(const GemmArgs& g, int block) {
     int m, n;
-    place(blockIdx.x, g.nm * g.nn * g.nz, g.nm, g.nn, g.gm, m, n, z);
+    place(block, g.nm * g.nn * g.nz, g.nm, g.nn, g.gm, m, n, z);
     m0 = m * T::BM;
     n0 = n * T::BN;
     lane = threadIdx.x & 63;
@@ -238,7 +298,7 @@ __device__ __forceinline__ float col_sum(float v) {
 template <int E, class T>
 __global__ __launch_bounds__(T::THREADS) void k_loss(GemmArgs g) {
   extern __shared__ char smem[];
-  const Place<T> p(g);
+  const Place<T> p(g, blockIdx.x);
   f32x4 acc[T::MI][T::NI];
   multiply<E, T, false, false>(acc, g.A, g.B, g.k, p.m0, p.n0, 0, g.steps, smem);
   if (g.ua) unscale<T>(acc, *g.ua * *g.ub);
@@ -337,11 +397,11 @@ __global__ __launch_bounds__(1024) void k_join(JoinArgs a) {
 template <int E, class T>
 __global__ __launch_bounds__(T::THREADS) void k_dlogit(GemmArgs g) {
   extern __shared__ char smem[];
-  const Place<T> p(g);
+  const Place<T> p(g, blockIdx.x);
   f32x4 acc[T::MI][T::NI];
   multiply<E, T, false, false>(acc, g.A, g.B, g.k, p.m0, p.n0, 0, g.steps, smem);
   if (g.ua) unscale<T>(acc, *g.ua * *g.ub);
-  const float gs = *g.gscale;
+  const float gs = g.gscale ? *g.gscale : 1.0f;
   const bool edge = p.mwave + T::MI * 16 > g.M;
 #pragma unroll
   for (int j = 0; j < T::NI; ++j) {
@@ -399,23 +459,19 @@ __global__ __launch_bounds__(T::THREADS) void k_dlogit(GemmArgs g) {
   }
 }
 
-// dx's part from one piece of the vocabulary: m = column of dx, n = position, k = vocabulary row
-template <int E, class T>
-__global__ __launch_bounds__(T::THREADS) void k_dx(GemmArgs g) {
-  extern __shared__ char smem[];
-  const Place<T> p(g);
-  f32x4 acc[T::MI][T::NI];
-  const int s0 = (int)((int64_t)g.steps * p.z / g.nz), s1 = (int)((int64_t)g.steps * (p.z + 1) / g.nz);
-  multiply<E, T, true, false>(acc, g.A, g.B, g.k, p.m0, p.n0, s0, s1, smem);
-  float* out = (float*)g.out + p.z * g.zstride;
+// a wave's blocks as (a part of) a 32-bit sum: column n of the product is row n of `out`
+template <class T>
+__device__ __forceinline__ void store_part(const f32x4 (&acc)[T::MI][T::NI], const GemmArgs& g, const Place<T>& p) {
+  float* out = (float*)g.part_out + p.z * g.zstride;
 #pragma unroll
   for (int j = 0; j < T::NI; ++j) {
     const int n = p.nw + 16 * j + p.col;
+    if (n >= g.N) continue;
 #pragma unroll
     for (int i = 0; i < T::MI; ++i) {
       const int m = p.mw + 16 * i;
-      if (m >= g.ldo) continue;
-      f32x4* to = (f32x4*)(out + (int64_t)n * g.ldo + m);
+      if (m >= g.ldp) continue;
+      f32x4* to = (f32x4*)(out + (int64_t)n * g.ldp + m);
       f32x4 v = acc[i][j];
       if (g.add) {
         const f32x4 o = *to;
@@ -429,36 +485,46 @@ __global__ __launch_bounds__(T::THREADS) void k_dx(GemmArgs g) {
   }
 }
 
-struct FinishArgs {
+// a gradient from its parts' sums
+struct FinishJob {
   const float* part;
   int64_t ldp, zstride;
-  int32_t nz, n, width, otype;
+  int64_t rows;
+  int32_t nz;
+  int32_t rows_count;  // rows are positions: those that do not count become zeros
   void* out;
   int64_t ldo;
   const float *u0, *u1;
+  int32_t wide;
+};
+struct FinishArgs {
+  FinishJob job[2];
+  int32_t blocks[2];
+  int32_t width, otype;
   Targets targets;
 };
-// dx from its pieces' sums
 __global__ __launch_bounds__(256) void k_finish(FinishArgs a) {
+  const int which = (int)blockIdx.x < a.blocks[0] ? 0 : 1;
+  const int block = (int)blockIdx.x - (which ? a.blocks[0] : 0);
+  const FinishJob& f = a.job[which];
   const int per = (a.width + 3) / 4;
-  const int64_t total = (int64_t)a.n * per;
-  const float mul = *a.u0 * (a.u1 ? *a.u1 : 1.0f);
-  for (int64_t g = blockIdx.x * (int64_t)256 + threadIdx.x; g < total; g += (int64_t)gridDim.x * 256) {
+  const int64_t total = f.rows * per;
+  const float mul = (f.u0 ? *f.u0 : 1.0f) * (f.u1 ? *f.u1 : 1.0f);
+  for (int64_t g = block * (int64_t)256 + threadIdx.x; g < total; g += (int64_t)a.blocks[which] * 256) {
     const int64_t n = g / per;
     const int c = (int)(g - n * per) * 4;
     f32x4 s = {0, 0, 0, 0};
-    for (int z = 0; z < a.nz; ++z) {
-      const f32x4 v = *(const f32x4*)(a.part + z * a.zstride + n * a.ldp + c);
+    for (int z = 0; z < f.nz; ++z) {
+      const f32x4 v = *(const f32x4*)(f.part + z * f.zstride + n * f.ldp + c);
       s.x += v.x;
       s.y += v.y;
       s.z += v.z;
       s.w += v.w;
     }
-    bool counts;
-    (void)target_of(a.targets, n, counts);
+    bool counts = true;
+    if (f.rows_count) (void)target_of(a.targets, n, counts);
     const float v[4] = {counts ? s.x * mul : 0.0f, counts ? s.y * mul : 0.0f, counts ? s.z * mul : 0.0f, counts ? s.w * mul : 0.0f};
-    const bool wide = a.otype == PST_F32 ? ((uintptr_t)a.out & 15) == 0 && a.ldo % 4 == 0 : ((uintptr_t)a.out & 7) == 0 && a.ldo % 4 == 0;
-    store4(a.out, a.otype, n * a.ldo + c, v, a.width - c, wide);
+    store4(f.out, a.otype, n * f.ldo + c, v, a.width - c, f.wide);
   }
 }
 
@@ -495,22 +561,37 @@ __device__ __forceinline__ void store_rows(const f32x4 (&acc)[T::MI][T::NI], con
   }
 }
 
-// rows v0 ... of dW: m = column, n = vocabulary row of the piece, k = position
+// Both gradients of a piece of the vocabulary in one launch, since D feeds both and neither fills the card evenly:
+// dx's parts (m = column, n = position, k = vocabulary row of the piece, its K loop in nz parts) and rows v0 ... of dW
+// (m = column, n = vocabulary row, k = position; in one part straight to the output, or in parts as dx).
 template <int E, class T>
-__global__ __launch_bounds__(T::THREADS) void k_dw(GemmArgs g) {
+__global__ __launch_bounds__(T::THREADS) void k_grads(GradArgs g) {
   extern __shared__ char smem[];
-  const Place<T> p(g);
+  const bool first = (int)blockIdx.x < g.dx_tiles;
   f32x4 acc[T::MI][T::NI];
-  multiply<E, T, true, true>(acc, g.A, g.B, g.k, p.m0, p.n0, 0, g.steps, smem);
-  unscale<T>(acc, *g.ua * (g.ub ? *g.ub : 1.0f));
-  store_rows<T>(acc, g, p, g.v0);
+  if (first) {
+    const Place<T> p(g.dx, blockIdx.x);
+    const int s0 = (int)((int64_t)g.dx.steps * p.z / g.dx.nz), s1 = (int)((int64_t)g.dx.steps * (p.z + 1) / g.dx.nz);
+    multiply<E, T, true, false>(acc, g.dx.A, g.dx.B, g.dx.k, p.m0, p.n0, s0, s1, smem);
+    store_part<T>(acc, g.dx, p);
+  } else {
+    const Place<T> p(g.dw, blockIdx.x - g.dx_tiles);
+    const int s0 = (int)((int64_t)g.dw.steps * p.z / g.dw.nz), s1 = (int)((int64_t)g.dw.steps * (p.z + 1) / g.dw.nz);
+    multiply<E, T, true, true>(acc, g.dw.A, g.dw.B, g.dw.k, p.m0, p.n0, s0, s1, smem);
+    if (g.dw.part_out) {
+      store_part<T>(acc, g.dw, p);
+    } else {
+      unscale<T>(acc, (g.dw.ua ? *g.dw.ua : 1.0f) * (g.dw.ub ? *g.dw.ub : 1.0f));
+      store_rows<T>(acc, g.dw, p, g.dw.v0);
+    }
+  }
 }
 
 // 8-bit scores: m = vocabulary row, n = position
 template <class T>
 __global__ __launch_bounds__(T::THREADS) void k_scores(GemmArgs g) {
   extern __shared__ char smem[];
-  const Place<T> p(g);
+  const Place<T> p(g, blockIdx.x);
   i32x4 sums[T::MI][T::NI];
   multiply<I8, T, false, false>(sums, g.A, g.B, g.k, p.m0, p.n0, 0, g.steps, smem);
   f32x4 acc[T::MI][T::NI];
@@ -581,29 +662,6 @@ __global__ __launch_bounds__(256) void k_pack8(const int8_t* src, int64_t ld, in
   }
 }
 
-// 16-bit floats with a short exponent (and the halves of a split one): D is scaled by the power of two that
-// brings the largest |g_n| to 2^13; scale[0] = that power, scale[1] = its inverse. bfloat16: 1.
-__global__ __launch_bounds__(1024) void k_gscale(const float* g, Targets t, int64_t n, int type, float* scale) {
-  __shared__ float sm[16];
-  float m = 0.0f;
-  if (type != PST_BF16)
-    for (int64_t i = threadIdx.x; i < n; i += 1024) {
-      bool counts;
-      (void)target_of(t, i, counts);
-      if (counts) m = fmaxf(m, finite_abs(g[i]));
-    }
-#pragma unroll
-  for (int s = 32; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
-  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < 16; ++w) m = fmaxf(m, sm[w]);
-    const int e = type == PST_BF16 ? 0 : max(-100, min(100, split_exp(m)));
-    scale[0] = ldexpf(1.0f, e);
-    scale[1] = ldexpf(1.0f, -e);
-  }
-}
-
 // ------------------------------------------------------------------ host
 thread_local std::string g_error;
 
@@ -668,15 +726,9 @@ using T64 = Tile<64, 64, 2, 2>;
 enum TileId { TILE64 = 0, TILE128 = 1, TILE256 = 2 };
 constexpr int TILE_M[3] = {64, 128, 256};
 
-// The largest tile that still gives most compute units one.
-int tile_for(int64_t m, int64_t n, int cus) {
-  for (int t = TILE256; t > TILE64; --t)
-    if (ceil_div(m, TILE_M[t]) * ceil_div(n, TILE_M[t]) * 4 >= 3 * (int64_t)cus) return t;
-  return TILE64;
-}
-
-template <class F>
-hipError_t launch(F* f, int64_t grid, int threads, int lds, hipStream_t st, const GemmArgs& g) {
+template <class F, class A>
+hipError_t launch(F* f, int64_t grid, int threads, int lds, hipStream_t st, const A& g) {
+  if (grid > 0x7fffffff) return hipErrorInvalidConfiguration;
   if (lds > 65536) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return e;
@@ -686,36 +738,74 @@ hipError_t launch(F* f, int64_t grid, int threads, int lds, hipStream_t st, cons
 }
 template <int E, class T>
 hipError_t launch_kind(int kind, const GemmArgs& g, hipStream_t st) {
-  const int64_t grid = (int64_t)g.nm * g.nn * g.nz;
-  switch (kind) {
-    case LOSS: return launch(k_loss<E, T>, grid, T::THREADS, T::LDS, st, g);
-    case DLOGIT: return launch(k_dlogit<E, T>, grid, T::THREADS, T::LDS, st, g);
-    case DX: return launch(k_dx<E, T>, grid, T::THREADS, T::LDS, st, g);
-    default: return launch(k_dw<E, T>, grid, T::THREADS, T::LDS, st, g);
+  const int64_t grid = (int64_t)g.nm * g.nn;
+  if constexpr (E == I8) {
+    return launch(k_scores<T>, grid, T::THREADS, T::LDS, st, g);
+  } else {
+    return kind == LOSS ? launch(k_loss<E, T>, grid, T::THREADS, T::LDS, st, g) : launch(k_dlogit<E, T>, grid, T::THREADS, T::LDS, st, g);
   }
 }
+void set_tiles(GemmArgs& g, int64_t m, int64_t n, int tile) {
+  g.nm = (int32_t)ceil_div(m, TILE_M[tile]);
+  g.nn = (int32_t)ceil_div(n, TILE_M[tile]);
+  g.nz = std::max(g.nz, 1);
+  g.gm = 4;
+}
+template <int E>
+hipError_t launch_elem(int kind, int tile, const GemmArgs& g, hipStream_t st) {
+  return tile == TILE256 ? launch_kind<E, T256>(kind, g, st) : tile == TILE128 ? launch_kind<E, T128>(kind, g, st) : launch_kind<E, T64>(kind, g, st);
+}
 hipError_t launch_gemm(int kind, int elem, int tile, GemmArgs g, hipStream_t st) {
-  const int t = TILE_M[tile];
-  g.nm = (int32_t)ceil_div(kind == DX ? g.ldo : (int64_t)g.M, t);
-  g.nn = (int32_t)ceil_div(g.N, t);
-  if (kind == DLOGIT) g.nm = (int32_t)(g.ldd / t);  // D's zeros behind the vocabulary too
-  if (g.nz == 0) g.nz = 1;
-  if (g.gm == 0) g.gm = 4;
-  if ((int64_t)g.nm * g.nn * g.nz > 0x7fffffff) return hipErrorInvalidConfiguration;
-  if (kind == SCORES) {
-    const int64_t grid = (int64_t)g.nm * g.nn;
-    return tile == TILE256   ? launch(k_scores<T256>, grid, T256::THREADS, T256::LDS, st, g)
-           : tile == TILE128 ? launch(k_scores<T128>, grid, T128::THREADS, T128::LDS, st, g)
-                             : launch(k_scores<T64>, grid, T64::THREADS, T64::LDS, st, g);
-  }
-  if (elem == BF16)
-    return tile == TILE256 ? launch_kind<BF16, T256>(kind, g, st) : tile == TILE128 ? launch_kind<BF16, T128>(kind, g, st) : launch_kind<BF16, T64>(kind, g, st);
-  return tile == TILE256 ? launch_kind<F16, T256>(kind, g, st) : tile == TILE128 ? launch_kind<F16, T128>(kind, g, st) : launch_kind<F16, T64>(kind, g, st);
+  set_tiles(g, g.M, g.N, tile);
+  return elem == I8 ? launch_elem<I8>(kind, tile, g, st) : elem == BF16 ? launch_elem<BF16>(kind, tile, g, st) : launch_elem<F16>(kind, tile, g, st);
+}
+template <int E>
+hipError_t launch_grads_elem(int tile, const GradArgs& g, int64_t grid, hipStream_t st) {
+  return tile == TILE256   ? launch(k_grads<E, T256>, grid, T256::THREADS, T256::LDS, st, g)
+         : tile == TILE128 ? launch(k_grads<E, T128>, grid, T128::THREADS, T128::LDS, st, g)
+                           : launch(k_grads<E, T64>, grid, T64::THREADS, T64::LDS, st, g);
+}
+hipError_t launch_grads(int elem, int tile, GradArgs g, bool dx, bool dw, hipStream_t st) {
+  set_tiles(g.dx, g.dx.ldp, g.dx.N, tile);
+  set_tiles(g.dw, g.dw.M, g.dw.N, tile);
+  const int64_t a = dx ? (int64_t)g.dx.nm * g.dx.nn * g.dx.nz : 0, b = dw ? (int64_t)g.dw.nm * g.dw.nn * g.dw.nz : 0;
+  g.dx_tiles = (int32_t)std::min<int64_t>(a, 0x7fffffff);
+  return elem == BF16 ? launch_grads_elem<BF16>(tile, g, a + b, st) : launch_grads_elem<F16>(tile, g, a + b, st);
 }
 
 int cus_of(int device, int* cus) {
   HEADCHK(hipDeviceGetAttribute(cus, hipDeviceAttributeMultiprocessorCount, device));
   return PST_OK;
+}
+
+// ---- the choice of tiles
+// Times of a workgroup in us, fitted to single launches on the card (d = 128 ... 1024, 16 ... 8192 positions): a launch's
+// tiles run in rounds of `slots`, and a tile costs BASE + PER_STEP * K-steps when its compute unit is full.
+//   256: 1 a unit, 1.5 us a K-step of 64 (all of them 1.4 PFLOP/s);  128: 2 a unit, 1.1;  64: 4 a unit, 0.85
+constexpr double TILE_BASE[3] = {2.0, 3.0, 4.0}, TILE_STEP[3] = {0.85, 1.1, 1.5};
+constexpr int TILE_SLOTS[3] = {4, 2, 1};
+struct Work {
+  int64_t tiles;
+  int64_t steps;
+};
+// the estimate for one launch of up to two kinds of tiles
+double launch_us(int tile, Work a, Work b, int cus) {
+  const double slots = (double)cus * TILE_SLOTS[tile];
+  const double ta = TILE_BASE[tile] + TILE_STEP[tile] * a.steps, tb = b.tiles ? TILE_BASE[tile] + TILE_STEP[tile] * b.steps : 0;
+  const double longest = std::max(ta, tb), all = (a.tiles * ta + b.tiles * tb) / slots;
+  // whole rounds of one kind; two kinds even out
+  if (!b.tiles) return std::ceil(a.tiles / slots) * ta;
+  return all <= longest ? longest : all + 0.5 * longest;
+}
+int64_t tiles_of(int64_t m, int64_t n, int tile) { return ceil_div(m, TILE_M[tile]) * ceil_div(n, TILE_M[tile]); }
+int tile_for(int64_t m, int64_t n, int64_t steps, int cus) {
+  int best = TILE64;
+  double us = 1e30;
+  for (int t = TILE256; t >= TILE64; --t) {
+    const double e = launch_us(t, {tiles_of(m, n, t), steps}, {0, 0}, cus);
+    if (e < us) us = e, best = t;
+  }
+  return best;
 }
 
 // What a call on [rows, width] x [vocab, width] needs of its workspace; the same for the query and for the call.
@@ -725,11 +815,13 @@ struct Plan {
   bool pack_x, pack_w;
   int64_t amax = 0, unscale = 0, x = 0, w = 0;   // offsets
   int64_t part = 0, tlogit = 0;                  // loss
-  int64_t gscale = 0, D = 0, dxp = 0;            // gradient
+  int64_t gscale = 0, D = 0, dxp = 0, dwp = 0;   // gradient
   int64_t piece = 0;                             // vocabulary rows of a piece
-  int nz = 1;
+  int tile = 0, zx = 1, zw = 1;                  // of the two gradients' launch
   int64_t bytes = 0;
 };
+// the plans are made for the card's number of compute units, so that the query needs no device
+constexpr int CUS = 256;
 
 Plan plan_common(int type, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab, int64_t width, bool grad, Bump& b) {
   Plan p;
@@ -740,7 +832,7 @@ Plan plan_common(int type, const void* x, int64_t ldx, const void* w, int64_t ld
   p.vocab = vocab;
   p.width = width;
   p.width_pad = up(width, 64);
-  p.rows_pad = up(rows, 256);
+  p.rows_pad = grad ? up(rows, 64) : rows;
   const int e = size_of(type);
   p.pack_w = type == PST_F32 || !in_place(w, ldw * e, width * e);
   // x is the operand with zeros behind the last column; the gradient needs zeros behind the last row too
@@ -749,14 +841,15 @@ Plan plan_common(int type, const void* x, int64_t ldx, const void* w, int64_t ld
     p.amax = b.take(2 * AMAX_BLOCKS * 4);
     p.unscale = b.take(8);
   }
-  if (p.pack_x) p.x = b.take((grad ? p.rows_pad : rows) * p.width_pad * 2 * p.planes);
+  if (p.pack_x) p.x = b.take(p.rows_pad * p.width_pad * 2 * p.planes);
   if (p.pack_w) p.w = b.take(vocab * p.width_pad * 2 * p.planes);
   return p;
 }
 Plan plan_loss(int type, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab, int64_t width) {
   Bump b;
   Plan p = plan_common(type, x, ldx, w, ldw, rows, vocab, width, false, b);
-  p.part = b.take(ceil_div(vocab, 64) * rows * 8);
+  p.tile = tile_for(vocab, rows, p.width_pad / 64 * (p.planes == 2 ? 3 : 1), CUS);
+  p.part = b.take(ceil_div(vocab, TILE_M[p.tile]) * rows * 8);
   p.tlogit = b.take(rows * 4);
   p.bytes = b.n;
   return p;
@@ -767,14 +860,29 @@ Plan plan_grad(int type, const void* x, int64_t ldx, const void* w, int64_t ldw,
   Bump b;
   Plan p = plan_common(type, x, ldx, w, ldw, rows, vocab, width, true, b);
   p.gscale = b.take(8);
-  const int64_t most = std::max<int64_t>(256, PIECE_BYTES / (p.rows_pad * 2 * p.planes) / 256 * 256);
-  p.piece = up(ceil_div(vocab, ceil_div(vocab, most)), 256);
-  p.D = b.take(p.rows_pad * p.piece * 2 * p.planes);
-  // few tiles of dx: the pieces' K loops are split so that each compute unit has one
-  const int64_t tiles = ceil_div(p.width_pad, 64) * ceil_div(rows, 64);
-  p.nz = (int)std::max<int64_t>(1, std::min<int64_t>({8, p.piece / 64 / 4, 512 / std::max<int64_t>(1, tiles)}));
-  if (p.nz == 1 && ceil_div(p.width_pad, 256) * ceil_div(rows, 256) < 192) p.nz = 2;
-  p.dxp = b.take(p.nz * p.rows_pad * p.width_pad * 4);
+  const int64_t drows = up(rows, 256);
+  int64_t most = std::max<int64_t>(256, PIECE_BYTES / (drows * 2 * p.planes) / 256 * 256);
+  // several pieces: of a size that gives dW's largest tiles in whole rounds, where that is not much smaller
+  const int64_t round = CUS / std::max<int64_t>(1, ceil_div(p.width_pad, 256)) * 256;
+  if (vocab > most && round > 0 && most >= round) most = most / round * round;
+  p.piece = vocab > most ? most : up(vocab, 256);
+  p.D = b.take(drows * p.piece * 2 * p.planes);
+  // tiles and parts of the K loops: the least of the estimated launch and of the parts' way through memory (4 TB/s)
+  const int64_t nv = std::min(p.piece, vocab);
+  const int passes = p.planes == 2 ? 3 : 1;
+  double best = 1e30;
+  for (int t = TILE256; t >= TILE64; --t)
+    for (int zx = 1; zx <= 16; zx *= 2)
+      for (int zw = 1; zw <= (vocab > p.piece ? 1 : 16); zw *= 2) {
+        const int64_t sx = ceil_div(nv, 64) * passes, sw = ceil_div(rows, 64) * passes;
+        if ((zx > 1 && sx < 4 * zx) || (zw > 1 && sw < 4 * zw)) continue;
+        const double us = launch_us(t, {tiles_of(p.width_pad, rows, t) * zx, ceil_div(sx, zx)}, {tiles_of(width, nv, t) * zw, ceil_div(sw, zw)}, CUS);
+        const double bytes = 8.0 * p.width_pad * (rows * (double)zx + (zw > 1 ? vocab * (double)zw : 0.0));
+        const double e = us * ceil_div(vocab, p.piece) + bytes / 4e6;
+        if (e < best) best = e, p.tile = t, p.zx = zx, p.zw = zw;
+      }
+  p.dxp = b.take(p.zx * rows * p.width_pad * 4);
+  if (p.zw > 1) p.dwp = b.take(p.zw * vocab * p.width_pad * 4);
   p.bytes = b.n;
   return p;
 }
@@ -804,47 +912,40 @@ int check_ws(const void* ws, int64_t have, int64_t need) {
 // grids of the copying kernels: a few workgroups a compute unit
 unsigned copy_grid(int64_t groups, int cus) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(groups, 256), cus * 16ll)); }
 
-// the operands in a form that the products read: in place, or packed (and split) into the workspace
-int operands(const Plan& p, const void* x, int64_t ldx, const void* w, int64_t ldw, const Targets* zero_rows, char* ws, int cus, hipStream_t st,
-             Operand* X, Operand* W) {
-  const int64_t xrows = zero_rows ? p.rows_pad : p.rows;
-  float* part = (float*)(ws + p.amax);
-  float* unscale = (float*)(ws + p.unscale);
+// the operands in a form that the products read: in place, or packed (and split) into the workspace; for the gradient
+// (gloss) also the scale of D. One launch, two for 32-bit operands, none where there is nothing to do.
+int operands(const Plan& p, const void* x, int64_t ldx, const void* w, int64_t ldw, const Targets& t, const float* gloss, char* ws, int cus,
+             hipStream_t st, Operand* X, Operand* W) {
+  PackArgs a{};
+  a.width = (int32_t)p.width;
+  a.width_pad = (int32_t)p.width_pad;
+  a.type = p.type;
+  a.targets = t;
   if (p.type == PST_F32) {
-    AmaxArgs a{{(const float*)x, (const float*)w}, {ldx, ldw}, {p.rows, p.vocab}, (int32_t)p.width, part};
-    hipLaunchKernelGGL(k_amax, dim3(2 * AMAX_BLOCKS), dim3(256), 0, st, a);
+    AmaxArgs m{{(const float*)x, (const float*)w}, {ldx, ldw}, {p.rows, p.vocab}, (int32_t)p.width, (float*)(ws + p.amax)};
+    hipLaunchKernelGGL(k_amax, dim3(2 * AMAX_BLOCKS), dim3(1024), 0, st, m);
     HEADCHK(hipGetLastError());
   }
-  auto pack = [&](const void* src, int64_t ld, int64_t rows, int64_t rows_pad, int64_t at, int which, const Targets* t) {
-    PackArgs a{};
-    a.src = src;
-    a.ld = ld;
-    a.rows = rows;
-    a.rows_pad = rows_pad;
-    a.width = (int32_t)p.width;
-    a.width_pad = (int32_t)p.width_pad;
-    a.type = p.type;
-    a.dst = ws + at;
-    a.plane = rows_pad * p.width_pad * 2;
-    a.part = part + which * AMAX_BLOCKS;
-    a.unscale = unscale + which;
-    if (t) a.targets = *t;
-    hipLaunchKernelGGL(k_pack, dim3(copy_grid(rows_pad * (p.width_pad / 8), cus)), dim3(256), 0, st, a);
-  };
   const int e = size_of(p.type);
-  if (p.pack_x) {
-    pack(x, ldx, p.rows, xrows, p.x, 0, zero_rows);
-    HEADCHK(hipGetLastError());
-    *X = {ws + p.x, xrows * p.width_pad * 2, p.width_pad * 2, (int32_t)xrows, (int32_t)p.width_pad * 2};
-  } else {
-    *X = {(const char*)x, 0, ldx * e, (int32_t)p.rows, (int32_t)p.width * e};
+  auto job = [&](int which, const void* src, int64_t ld, int64_t rows, int64_t rows_pad, int64_t at) {
+    PackJob& j = a.job[which];
+    j = {src, ld, rows, rows_pad, ws + at, rows_pad * p.width_pad * 2, (float*)(ws + p.amax) + which * AMAX_BLOCKS, (float*)(ws + p.unscale) + which,
+         which == 0 && gloss, ((uintptr_t)src & 15) == 0 && ld * e % 16 == 0};
+    a.blocks[which] = (int32_t)copy_grid(rows_pad * (p.width_pad / 8), cus);
+    return Operand{ws + at, j.plane, p.width_pad * 2, (int32_t)rows_pad, (int32_t)p.width_pad * 2};
+  };
+  *X = p.pack_x ? job(0, x, ldx, p.rows, p.rows_pad, p.x) : Operand{(const char*)x, 0, ldx * e, (int32_t)p.rows, (int32_t)p.width * e};
+  *W = p.pack_w ? job(1, w, ldw, p.vocab, p.vocab, p.w) : Operand{(const char*)w, 0, ldw * e, (int32_t)p.vocab, (int32_t)p.width * e};
+  int blocks = a.blocks[0] + a.blocks[1];
+  if (gloss && p.type != PST_BF16) {
+    a.gloss = gloss;
+    a.n = p.rows;
+    a.gscale = (float*)(ws + p.gscale);
+    ++blocks;
   }
-  if (p.pack_w) {
-    pack(w, ldw, p.vocab, p.vocab, p.w, 1, nullptr);
+  if (blocks) {
+    hipLaunchKernelGGL(k_pack, dim3((unsigned)blocks), dim3(256), 0, st, a);
     HEADCHK(hipGetLastError());
-    *W = {ws + p.w, p.vocab * p.width_pad * 2, p.width_pad * 2, (int32_t)p.vocab, (int32_t)p.width_pad * 2};
-  } else {
-    *W = {(const char*)w, 0, ldw * e, (int32_t)p.vocab, (int32_t)p.width * e};
   }
   return PST_OK;
 }
@@ -869,7 +970,8 @@ int token_loss(int device, int type, const void* x, int64_t ldx, const void* w, 
   if (rc != PST_OK) return rc;
   char* ws = (char*)ws_;
   GemmArgs g{};
-  rc = operands(p, x, ldx, w, ldw, nullptr, ws, cus, st, &g.B, &g.A);
+  g.targets = {targets, ignore, tbits, (int32_t)vocab};
+  rc = operands(p, x, ldx, w, ldw, g.targets, nullptr, ws, cus, st, &g.B, &g.A);
   if (rc != PST_OK) return rc;
   g.k = passes(p.planes);
   g.M = (int32_t)vocab;
@@ -879,12 +981,10 @@ int token_loss(int device, int type, const void* x, int64_t ldx, const void* w, 
     g.ua = (float*)(ws + p.unscale) + 1;
     g.ub = (float*)(ws + p.unscale);
   }
-  g.targets = {targets, ignore, tbits, (int32_t)vocab};
   g.part = (float2*)(ws + p.part);
   g.tlogit = (float*)(ws + p.tlogit);
-  const int tile = tile_for(vocab, rows, cus);
-  HEADCHK(launch_gemm(LOSS, p.elem, tile, g, st));
-  JoinArgs j{g.part, g.tlogit, g.targets, loss, lse, (int32_t)rows, (int32_t)ceil_div(vocab, TILE_M[tile])};
+  HEADCHK(launch_gemm(LOSS, p.elem, p.tile, g, st));
+  JoinArgs j{g.part, g.tlogit, g.targets, loss, lse, (int32_t)rows, (int32_t)ceil_div(vocab, TILE_M[p.tile])};
   hipLaunchKernelGGL(k_join, dim3((unsigned)ceil_div(rows, 64)), dim3(1024), 0, st, j);
   HEADCHK(hipGetLastError());
   return PST_OK;
@@ -912,27 +1012,29 @@ int token_loss_grad(int device, int type, const void* x, int64_t ldx, const void
   if (rc != PST_OK) return rc;
   char* ws = (char*)ws_;
   const Targets t{targets, ignore, tbits, (int32_t)vocab};
-  // no positions: one of zeros stands for them, so that dW is written as the zeros that it is
+  // no positions: 64 of zeros stand for them, so that dW is written as the zeros that it is
   Plan q = p;
   q.rows = rows;
   Operand X, W;
-  rc = operands(q, x, ldx, w, ldw, &t, ws, cus, st, &X, &W);
+  static const float none = 0.0f;  // (never read: there are no rows)
+  rc = operands(q, x, ldx, w, ldw, t, rows ? gloss : &none, ws, cus, st, &X, &W);
   if (rc != PST_OK) return rc;
-  float* gs = (float*)(ws + p.gscale);
-  hipLaunchKernelGGL(k_gscale, dim3(1), dim3(1024), 0, st, gloss, t, rows, type, gs);
-  HEADCHK(hipGetLastError());
+  const float* gs = p.type == PST_BF16 ? nullptr : (float*)(ws + p.gscale);
+  const float* ungs = gs ? gs + 1 : nullptr;
   const float* ux = p.planes == 2 ? (float*)(ws + p.unscale) : nullptr;
   const float* uw = p.planes == 2 ? ux + 1 : nullptr;
   char* D = ws + p.D;
-  float* dxp = (float*)(ws + p.dxp);
+  const int64_t drows = up(std::max<int64_t>(rows, 1), 256);
+  const bool need_dx = dx && rows;
   for (int64_t v0 = 0; v0 < vocab; v0 += p.piece) {
-    const int64_t nv = std::min(p.piece, vocab - v0), nv_pad = up(nv, 256);
-    const int64_t dplane = p.rows_pad * nv_pad * 2;
+    const int64_t nv = std::min(p.piece, vocab - v0), ldd = up(nv, 256);
+    const Operand dop{D, drows * ldd * 2, ldd * 2, (int32_t)drows, (int32_t)ldd * 2};
+    Operand Wv = W;
+    Wv.p += v0 * W.ld;
+    Wv.rows = (int32_t)nv;
     GemmArgs g{};
     g.k = passes(p.planes);
-    g.A = W;
-    g.A.p += v0 * W.ld;
-    g.A.rows = (int32_t)nv;
+    g.A = Wv;
     g.B = X;
     g.M = (int32_t)nv;
     g.N = (int32_t)rows;
@@ -944,50 +1046,54 @@ int token_loss_grad(int device, int type, const void* x, int64_t ldx, const void
     g.gloss = gloss;
     g.gscale = gs;
     g.D = D;
-    g.dplane = dplane;
-    g.ldd = nv_pad;
+    g.dplane = dop.plane;
+    g.ldd = ldd;
     g.dtype = p.elem == BF16 ? PST_BF16 : PST_F16;
     g.dplanes = p.planes;
     g.v0 = (int32_t)v0;
-    if (rows) HEADCHK(launch_gemm(DLOGIT, p.elem, tile_for(nv, rows, cus), g, st));
-    if (dx && rows) {
-      GemmArgs d{};
-      d.k = passes(p.planes);
-      d.A = W;
-      d.A.p += v0 * W.ld;
-      d.A.rows = (int32_t)nv;
-      d.B = {D, dplane, nv_pad * 2, (int32_t)p.rows_pad, (int32_t)nv_pad * 2};
-      d.M = (int32_t)width;
-      d.N = (int32_t)rows;
-      d.steps = (int32_t)ceil_div(nv, 64);
-      d.nz = p.nz;
-      d.out = dxp;
-      d.ldo = p.width_pad;
-      d.zstride = p.rows_pad * p.width_pad;
-      d.add = v0 > 0;
-      HEADCHK(launch_gemm(DX, p.elem, tile_for(p.width_pad, rows * p.nz, cus), d, st));
+    if (rows) HEADCHK(launch_gemm(DLOGIT, p.elem, tile_for(nv, rows, g.steps * (p.planes == 2 ? 3 : 1), cus), g, st));
+    GradArgs b{};
+    b.dx.k = b.dw.k = g.k;
+    b.dx.A = Wv;
+    b.dx.B = b.dw.B = dop;
+    b.dx.M = b.dw.M = (int32_t)width;
+    b.dx.N = (int32_t)rows;
+    b.dx.steps = (int32_t)ceil_div(nv, 64);
+    b.dx.nz = p.zx;
+    b.dx.part_out = (float*)(ws + p.dxp);
+    b.dx.ldp = b.dw.ldp = p.width_pad;
+    b.dx.zstride = rows * p.width_pad;
+    b.dx.add = v0 > 0;
+    b.dw.A = X;
+    b.dw.N = (int32_t)nv;
+    b.dw.steps = (int32_t)ceil_div(rows, 64);
+    b.dw.nz = p.zw;
+    b.dw.ua = ungs;
+    b.dw.ub = ux;
+    b.dw.v0 = (int32_t)v0;
+    b.dw.out = dw;
+    b.dw.ldo = lddw;
+    b.dw.otype = type;
+    b.dw.wide = lddw % (16 / e) == 0 && ((uintptr_t)dw & 15) == 0;
+    if (p.zw > 1) {
+      b.dw.part_out = (float*)(ws + p.dwp);
+      b.dw.zstride = vocab * p.width_pad;
     }
-    if (dw) {
-      GemmArgs d{};
-      d.k = passes(p.planes);
-      d.A = X;
-      d.B = {D, dplane, nv_pad * 2, (int32_t)p.rows_pad, (int32_t)nv_pad * 2};
-      d.M = (int32_t)width;
-      d.N = (int32_t)nv;
-      d.steps = (int32_t)ceil_div(rows, 64);
-      d.ua = gs + 1;
-      d.ub = ux;
-      d.v0 = (int32_t)v0;
-      d.out = dw;
-      d.ldo = lddw;
-      d.otype = type;
-      d.wide = lddw % (16 / e) == 0 && ((uintptr_t)dw & 15) == 0;
-      HEADCHK(launch_gemm(DW, p.elem, tile_for(width, nv, cus), d, st));
-    }
+    HEADCHK(launch_grads(p.elem, p.tile, b, need_dx, dw != nullptr, st));
   }
-  if (dx && rows) {
-    FinishArgs f{dxp, p.width_pad, p.rows_pad * p.width_pad, p.nz, (int32_t)rows, (int32_t)width, type, dx, lddx, gs + 1, uw, t};
-    hipLaunchKernelGGL(k_finish, dim3(copy_grid(rows * ceil_div(width, 4), cus)), dim3(256), 0, st, f);
+  FinishArgs f{};
+  f.width = (int32_t)width;
+  f.otype = type;
+  f.targets = t;
+  auto job = [&](int which, int64_t part, int64_t n, int nz, void* out, int64_t ldo, const float* u) {
+    f.job[which] = {(const float*)(ws + part), p.width_pad, n * p.width_pad, n, nz, which == 0, out, ldo, ungs, u,
+                    ldo % 4 == 0 && ((uintptr_t)out & (type == PST_F32 ? 15 : 7)) == 0};
+    f.blocks[which] = (int32_t)copy_grid(n * ceil_div(width, 4), cus);
+  };
+  if (need_dx) job(0, p.dxp, rows, p.zx, dx, lddx, uw);
+  if (dw && p.zw > 1) job(1, p.dwp, vocab, p.zw, dw, lddw, ux);
+  if (f.blocks[0] + f.blocks[1]) {
+    hipLaunchKernelGGL(k_finish, dim3((unsigned)(f.blocks[0] + f.blocks[1])), dim3(256), 0, st, f);
     HEADCHK(hipGetLastError());
   }
   return PST_OK;
@@ -1075,7 +1181,7 @@ int token_scores_i8(int device, int type, const void* x, int64_t ldx, const int8
   g.wide = ldo % (16 / size_of(otype)) == 0 && ((uintptr_t)out & 15) == 0;
   g.sn = (const float*)(ws + p.scale);
   g.sm = wscale;
-  HEADCHK(launch_gemm(SCORES, I8, tile_for(vocab, rows, cus), g, st));
+  HEADCHK(launch_gemm(SCORES, I8, tile_for(vocab, rows, g.steps, cus), g, st));
   return PST_OK;
 }
 
