@@ -24,6 +24,20 @@
 namespace pst_head {
 namespace {
 
+// Tiles of the products. A remainder of up to 64 vocabulary rows behind the 256-row tiles (the marks behind a codebook of
+// 4096 or 64000), or of positions, goes to thin tiles of the same launch instead of a round of nearly empty ones.
+struct T256 : Tile<256, 256, 2, 4> {
+  static constexpr bool HAS_THIN = true;
+  struct Thin : Tile<64, 256, 2, 4> {};   // along m
+  struct ThinN : Tile<256, 64, 4, 2> {};  // along n
+};
+struct T128 : Tile<128, 128, 2, 2> {
+  static constexpr bool HAS_THIN = false;
+};
+struct T64 : Tile<64, 64, 2, 2> {
+  static constexpr bool HAS_THIN = false;
+};
+
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr int AMAX_BLOCKS = 256;
 
@@ -34,7 +48,7 @@ __device__ __forceinline__ float load1(const void* p, int type, int64_t i) {
   if (type == PST_BF16) return __uint_as_float((uint32_t)((const uint16_t*)p)[i] << 16);
   return (float)((const _Float16*)p)[i];
 }
-__device__ __forceinline__ uint32_t bits16(float v, int type) {
+__device__ __forceinline__ uint32_t bits16(float v, int type) {  // (type: a constant where it counts)
   if (type == PST_BF16) return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)v);
   return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v);
 }
@@ -168,18 +182,29 @@ __global__ __launch_bounds__(256) void k_pack(PackArgs a) {
     e = split_exp(block_max(p.part[threadIdx.x], sm));
     if (block == 0 && threadIdx.x == 0) *p.unscale = ldexpf(1.0f, -e);
   }
-  const int per = a.width_pad / 8;
+  const int by = p.wide ? 8 : 2, per = a.width_pad / by;  // neighbours a thread takes
   const int64_t groups = p.rows_pad * per;
   for (int64_t g = block * (int64_t)256 + threadIdx.x; g < groups; g += (int64_t)a.blocks[which] * 256) {
     const int64_t r = g / per;
-    const int c = (int)(g - r * per) * 8;
+    const int c = (int)(g - r * per) * by;
     bool keep = r < p.rows;
     if (keep && p.zero_rows) (void)target_of(a.targets, r, keep);
     char* d = p.dst + (r * a.width_pad + c) * 2;
-    if (!f32) {
+    if (!p.wide) {
+      const int64_t at = r * p.ld + c;
+      const bool k0 = keep && c < a.width, k1 = keep && c + 1 < a.width;
+      if (f32) {
+        const float x = k0 ? ldexpf(((const float*)p.src)[at], e) : 0.0f, y = k1 ? ldexpf(((const float*)p.src)[at + 1], e) : 0.0f;
+        *(uint32_t*)d = pack2(x, y, PST_F16);
+        *(uint32_t*)(d + p.plane) = pack2(rest16(x), rest16(y), PST_F16);
+      } else {
+        const uint32_t x = k0 ? ((const uint16_t*)p.src)[at] : 0, y = k1 ? ((const uint16_t*)p.src)[at + 1] : 0;
+        *(uint32_t*)d = x | y << 16;
+      }
+    } else if (!f32) {
       uint4 v = make_uint4(0, 0, 0, 0);
       const uint16_t* src = (const uint16_t*)p.src + r * p.ld + c;
-      if (keep && p.wide && c + 8 <= a.width) {
+      if (keep && c + 8 <= a.width) {
         v = *(const uint4*)src;
       } else if (keep) {
         uint32_t h[8];
@@ -191,7 +216,7 @@ __global__ __launch_bounds__(256) void k_pack(PackArgs a) {
     } else {
       float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
       const float* src = (const float*)p.src + r * p.ld + c;
-      if (keep && p.wide && c + 8 <= a.width) {
+      if (keep && c + 8 <= a.width) {
         const f32x4 lo = *(const f32x4*)src, hi = *(const f32x4*)(src + 4);
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = lo[j], v[4 + j] = hi[j];
@@ -217,7 +242,8 @@ struct GemmArgs {
   Operand A, B;
   KLoop k;
   int32_t M, N;        // rows of A and of B that exist
-  int32_t nm, nn, nz;  // tiles along m and n, pieces of the K loop
+  int32_t nm, nn, nz;  // tiles along m and n, parts of the K loop
+  int32_t blocks;      // workgroups that share the nm nn tiles; those behind them take the thin tiles of the last rows
   int32_t steps;       // K-steps of the whole range
   int32_t gm;
   // unscaling of 32-bit operands (device; null: 1)
@@ -230,7 +256,7 @@ struct GemmArgs {
   const float* gscale; // power of two on D (device; null: 1)
   char* D;             // [planes][rows][ldd] 16-bit
   int64_t dplane, ldd; // bytes, elements
-  int32_t dtype, dplanes, v0;
+  int32_t dplanes, v0;
   // matrix outputs
   void* out;
   int64_t ldo;
@@ -244,23 +270,27 @@ struct GemmArgs {
 
 struct GradArgs {
   GemmArgs dx, dw;
-  int32_t dx_tiles;
+  int32_t blocks[4];
 };
 
 enum Kind { LOSS, DLOGIT, SCORES };
 
+// Where a tile lies, and this wave and lane in it. `nm` x `nn` tiles start at row m_base and column n_base.
 template <class T>
 struct Place {
-  int m0, n0, z, lane, col, mwave, mw, nw;  // mwave, nw: this wave's first row and column, mw: this lane's first row
-  __device__ __forceinline__ Place(const GemmArgs& g, int block) {
+  static constexpr int BM = T::BM, BN = T::BN;
+  int m0, n0, z, mtile, lane, col, wrow, mwave, mw, nw;  // mwave, nw: this wave's first row and column, mw: this lane's first row
+  __device__ __forceinline__ Place(const GemmArgs& g, int tile, int nm, int nn, int m_base, int n_base) {
     int m, n;
-    place(block, g.nm * g.nn * g.nz, g.nm, g.nn, g.gm, m, n, z);
-    m0 = m * T::BM;
-    n0 = n * T::BN;
+    place(tile, nm * nn * g.nz, nm, nn, g.gm, m, n, z);
+    m0 = m_base + m * T::BM;
+    n0 = n_base + n * T::BN;
+    mtile = m_base ? g.nm : m;
     lane = threadIdx.x & 63;
     col = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    mwave = m0 + (wave / T::WN) * T::MI * 16;
+    wrow = wave / T::WN;
+    mwave = m0 + wrow * T::MI * 16;
     mw = mwave + 4 * (lane >> 4);
     nw = n0 + (wave % T::WN) * T::NI * 16;
   }
@@ -295,65 +325,128 @@ __device__ __forceinline__ float col_sum(float v) {
   return v + __shfl_xor(v, 32);
 }
 
-template <int E, class T>
-__global__ __launch_bounds__(T::THREADS) void k_loss(GemmArgs g) {
-  extern __shared__ char smem[];
-  const Place<T> p(g, blockIdx.x);
-  f32x4 acc[T::MI][T::NI];
-  multiply<E, T, false, false>(acc, g.A, g.B, g.k, p.m0, p.n0, 0, g.steps, smem);
-  if (g.ua) unscale<T>(acc, *g.ua * *g.ub);
-  if (p.mwave + T::MI * 16 > g.M) {  // rows behind the vocabulary's last
-#pragma unroll
-    for (int i = 0; i < T::MI; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (p.mw + 16 * i + r >= g.M) {
-#pragma unroll
-          for (int j = 0; j < T::NI; ++j) acc[i][j][r] = -__builtin_inff();
-        }
+// LDS behind a tile's stages: 4 KB for what an epilogue needs of the tile's rows and columns
+template <class T>
+__device__ __forceinline__ float* epilogue_lds(char* smem) {
+  return (float*)(smem + T::LDS);
+}
+constexpr int EPILOGUE_LDS = 4096;
+
+// A workgroup's tiles: tile, tile + stride, ... of the nm nn tiles of type T. The next tile's loads fly during the
+// epilogue of the last; what the epilogue needs from memory is loaded during the K loop (column and row of this thread),
+// since waiting for a load is waiting for all that were started before it.
+template <int E, class T, bool MANY, class Epilogue>
+__device__ __forceinline__ void tiles(const GemmArgs& g, int tile, int stride, int nm, int m_base, char* smem, Epilogue epilogue) {
+  Loop<E, T, false, false> loop(smem);
+  const int total = nm * g.nn;
+  if (tile >= total) return;
+  Place<T> p(g, tile, nm, g.nn, m_base, 0);
+  loop.begin(g.A, g.B, g.k, p.m0, p.n0, 0, g.steps);
+  for (;;) {
+    typename Mma<E>::Acc acc[T::MI][T::NI];
+    auto inputs = epilogue.load(g, p);
+    loop.run(acc);
+    epilogue.share(inputs, epilogue_lds<T>(smem));
+    const Place<T> done = p;
+    tile += stride;
+    const bool more = MANY && tile < total;
+    if (more) {
+      p = Place<T>(g, tile, nm, g.nn, m_base, 0);
+      loop.begin(g.A, g.B, g.k, p.m0, p.n0, 0, g.steps);
+    }
+    met();
+    epilogue.template store<T>(g, done, acc, epilogue_lds<T>(smem));
+    if (!more) return;
   }
-  float2* sm = (float2*)smem;  // [WM][BN]
-#pragma unroll
-  for (int j = 0; j < T::NI; ++j) {
-    const int n = p.nw + 16 * j + p.col;
-    float mx = acc[0][j][0];
-#pragma unroll
-    for (int i = 0; i < T::MI; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) mx = fmaxf(mx, acc[i][j][r]);
-    mx = col_max(mx);
-    const float base = mx == -__builtin_inff() ? 0.0f : mx * LOG2E;
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < T::MI; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) sum += exp2_fast(__builtin_fmaf(acc[i][j][r], LOG2E, -base));
-    sum = col_sum(sum);
-    // the target's logit, where it is among this wave's rows
-    bool counts = false;
-    const int t = n < g.N ? target_of(g.targets, n, counts) : -1;
-    if (__any(t >= p.mwave && t < p.mwave + T::MI * 16)) {
-      const int at = t < 0 ? -1 : t - p.mw;
+}
+
+struct LossEpilogue {
+  struct Inputs {
+    int target;
+  };
+  template <class P>
+  __device__ __forceinline__ Inputs load(const GemmArgs& g, const P& p) const {
+    bool counts;
+    const int n = p.n0 + (int)threadIdx.x;
+    return {(int)threadIdx.x < P::BN && n < g.N ? target_of(g.targets, n, counts) : -1};
+  }
+  __device__ __forceinline__ void share(const Inputs& in, float* lds) const {
+    asm volatile("" ::"v"(in.target));
+    if (threadIdx.x < 256) ((int*)lds)[threadIdx.x] = in.target;
+  }
+  template <class T>
+  __device__ __forceinline__ void store(const GemmArgs& g, const Place<T>& p, f32x4 (&acc)[T::MI][T::NI], float* lds) const {
+    if (g.ua) unscale<T>(acc, *g.ua * *g.ub);
+    if (p.mwave + T::MI * 16 > g.M) {  // rows behind the vocabulary's last
 #pragma unroll
       for (int i = 0; i < T::MI; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (at == 16 * i + r) g.tlogit[n] = acc[i][j][r];
+          if (p.mw + 16 * i + r >= g.M) {
+#pragma unroll
+            for (int j = 0; j < T::NI; ++j) acc[i][j][r] = -__builtin_inff();
+          }
     }
-    if (p.lane < 16) sm[((threadIdx.x >> 6) / T::WN) * T::BN + (n - p.n0)] = make_float2(mx, sum);
+    static_assert(256 * 4 + T::BN * 8 <= EPILOGUE_LDS, "epilogue's LDS");
+    float2* sm = (float2*)(lds + 256);  // [WM - 1][BN]: the other waves' maxima and sums
+    float mxs[T::NI], sums[T::NI];
+#pragma unroll
+    for (int j = 0; j < T::NI; ++j) {
+      const int n = p.nw + 16 * j + p.col;
+      float mx = acc[0][j][0];
+#pragma unroll
+      for (int i = 0; i < T::MI; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, acc[i][j][r]);
+      mx = col_max(mx);
+      const float base = mx == -__builtin_inff() ? 0.0f : mx * LOG2E;
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < T::MI; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum += exp2_fast(__builtin_fmaf(acc[i][j][r], LOG2E, -base));
+      sum = col_sum(sum);
+      mxs[j] = mx;
+      sums[j] = sum;
+      // the target's logit, where it is among this wave's rows
+      const int t = ((const int*)lds)[n - p.n0];
+      if (__any(t >= p.mwave && t < p.mwave + T::MI * 16)) {
+        const int at = t < 0 ? -1 : t - p.mw;
+#pragma unroll
+        for (int i = 0; i < T::MI; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (at == 16 * i + r) g.tlogit[n] = acc[i][j][r];
+      }
+    }
+    // the waves of a column join in wave row 0
+    static_assert(T::WM == 2, "two waves a column");
+    if (p.wrow == 1 && p.lane < 16) {
+#pragma unroll
+      for (int j = 0; j < T::NI; ++j) sm[p.nw - p.n0 + 16 * j + p.lane] = make_float2(mxs[j], sums[j]);
+    }
+    met();
+    if (p.wrow == 0 && p.lane < 16) {
+#pragma unroll
+      for (int j = 0; j < T::NI; ++j) {
+        const int n = p.nw + 16 * j + p.lane;
+        const float2 o = sm[n - p.n0];
+        const float mx = fmaxf(mxs[j], o.x);
+        const float safe = mx == -__builtin_inff() ? 0.0f : mx;
+        if (n < g.N)
+          g.part[(int64_t)p.mtile * g.N + n] = make_float2(mx, sums[j] * exp2_fast((mxs[j] - safe) * LOG2E) + o.y * exp2_fast((o.x - safe) * LOG2E));
+      }
+    }
   }
-  __syncthreads();
-  for (int c = threadIdx.x; c < T::BN; c += T::THREADS) {
-    if (p.n0 + c >= g.N) continue;
-    float2 a = sm[c];
-    for (int w = 1; w < T::WM; ++w) {
-      const float2 b = sm[w * T::BN + c];
-      const float mx = fmaxf(a.x, b.x);
-      const float safe = mx == -__builtin_inff() ? 0.0f : mx;
-      a.y = a.y * exp2_fast((a.x - safe) * LOG2E) + b.y * exp2_fast((b.x - safe) * LOG2E);
-      a.x = mx;
-    }
-    g.part[(int64_t)(p.m0 / T::BM) * g.N + p.n0 + c] = a;
+};
+
+template <int E, class T>
+__global__ __launch_bounds__(T::THREADS, 2) void k_loss(GemmArgs g) {
+  extern __shared__ char smem[];
+  if ((int)blockIdx.x < g.blocks) {
+    tiles<E, T, true>(g, blockIdx.x, g.blocks, g.nm, 0, smem, LossEpilogue{});
+  } else if constexpr (T::HAS_THIN) {
+    tiles<E, typename T::Thin, false>(g, blockIdx.x - g.blocks, 1 << 30, 1, g.nm * T::BM, smem, LossEpilogue{});
   }
 }
 
@@ -394,68 +487,100 @@ __global__ __launch_bounds__(1024) void k_join(JoinArgs a) {
 }
 
 // D of one piece of the vocabulary (columns v0 ...; zeros behind the last row and for positions that do not count)
-template <int E, class T>
-__global__ __launch_bounds__(T::THREADS) void k_dlogit(GemmArgs g) {
-  extern __shared__ char smem[];
-  const Place<T> p(g, blockIdx.x);
-  f32x4 acc[T::MI][T::NI];
-  multiply<E, T, false, false>(acc, g.A, g.B, g.k, p.m0, p.n0, 0, g.steps, smem);
-  if (g.ua) unscale<T>(acc, *g.ua * *g.ub);
-  const float gs = g.gscale ? *g.gscale : 1.0f;
-  const bool edge = p.mwave + T::MI * 16 > g.M;
+template <int E>
+struct DlogitEpilogue {
+  static constexpr int TYPE = E == BF16 ? PST_BF16 : PST_F16;
+  struct Inputs {
+    int target;  // less v0; a position that does not count has a factor of 0
+    float lse, c;
+  };
+  template <class P>
+  __device__ __forceinline__ Inputs load(const GemmArgs& g, const P& p) const {
+    const int n = p.n0 + (int)threadIdx.x;
+    Inputs in = {-1, 0.0f, 0.0f};
+    if ((int)threadIdx.x < P::BN && n < g.N) {
+      bool counts;
+      const int t = target_of(g.targets, n, counts);
+      in.target = t < 0 ? -1 : t - g.v0;
+      in.lse = counts ? g.lse[n] : 0.0f;
+      in.c = !counts ? 0.0f : t < 0 ? __builtin_nanf("") : g.gloss[n] * (g.gscale ? *g.gscale : 1.0f);
+    }
+    return in;
+  }
+  __device__ __forceinline__ void share(const Inputs& in, float* lds) const {
+    asm volatile("" ::"v"(in.target), "v"(in.lse), "v"(in.c));
+    if (threadIdx.x < 256) {
+      ((int*)lds)[threadIdx.x] = in.target;
+      lds[256 + threadIdx.x] = in.lse;
+      lds[512 + threadIdx.x] = in.c;
+    }
+  }
+  template <class T>
+  __device__ __forceinline__ void store(const GemmArgs& g, const Place<T>& p, f32x4 (&acc)[T::MI][T::NI], float* lds) const {
+    if (g.ua) unscale<T>(acc, *g.ua * *g.ub);
+    const bool edge = p.mwave + T::MI * 16 > g.M;
 #pragma unroll
-  for (int j = 0; j < T::NI; ++j) {
-    const int n = p.nw + 16 * j + p.col;
-    bool counts = false;
-    int t = -1;
-    float c = 0.0f, lse = 0.0f;
-    if (n < g.N) {
-      t = target_of(g.targets, n, counts);
-      if (counts) {
-        c = t < 0 ? __builtin_nanf("") : g.gloss[n] * gs;
-        lse = g.lse[n];
+    for (int j = 0; j < T::NI; ++j) {
+      const int n = p.nw + 16 * j + p.col;
+      const int t = ((const int*)lds)[n - p.n0];
+      const float lse = lds[256 + n - p.n0], c = lds[512 + n - p.n0];
+#pragma unroll
+      for (int i = 0; i < T::MI; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[i][j][r] = exp2_fast((acc[i][j][r] - lse) * LOG2E);
+      if (__any(t >= p.mwave && t < p.mwave + T::MI * 16)) {
+        const int at = t - p.mw;
+#pragma unroll
+        for (int i = 0; i < T::MI; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            acc[i][j][r] -= at == 16 * i + r ? 1.0f : 0.0f;
       }
-    }
-#pragma unroll
-    for (int i = 0; i < T::MI; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) acc[i][j][r] = exp2_fast((acc[i][j][r] - lse) * LOG2E);
-    t -= g.v0;
-    if (__any(t >= p.mwave && t < p.mwave + T::MI * 16)) {
-      const int at = t - p.mw;
 #pragma unroll
       for (int i = 0; i < T::MI; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (at == 16 * i + r) acc[i][j][r] -= 1.0f;
-    }
+        for (int r = 0; r < 4; ++r) acc[i][j][r] *= c;
+      // what does not count is zero whatever its hidden row holds
+      if (__any(c == 0.0f)) {
 #pragma unroll
-    for (int i = 0; i < T::MI; ++i)
+        for (int i = 0; i < T::MI; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) acc[i][j][r] = counts ? acc[i][j][r] * c : 0.0f;
-    if (edge) {
+          for (int r = 0; r < 4; ++r) acc[i][j][r] = c == 0.0f ? 0.0f : acc[i][j][r];
+      }
+      if (edge) {
 #pragma unroll
-      for (int i = 0; i < T::MI; ++i)
+        for (int i = 0; i < T::MI; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[i][j][r] = p.mw + 16 * i + r < g.M ? acc[i][j][r] : 0.0f;
-    }
-    char* to = g.D + ((int64_t)n * g.ldd + p.mwave) * 2;
+          for (int r = 0; r < 4; ++r) acc[i][j][r] = p.mw + 16 * i + r < g.M ? acc[i][j][r] : 0.0f;
+      }
+      char* to = g.D + ((int64_t)n * g.ldd + p.mwave) * 2;
 #pragma unroll
-    for (int i = 0; i < T::MI; i += 2) {
-      uint32_t w[2][2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int q = 0; q < 2; ++q) w[u][q] = pack2(acc[i + u][j][2 * q], acc[i + u][j][2 * q + 1], g.dtype);
-      store_pair(to + i * 32, w, p.lane);
-      if (g.dplanes == 2) {
+      for (int i = 0; i < T::MI; i += 2) {
+        uint32_t w[2][2];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int q = 0; q < 2; ++q) w[u][q] = pack2(rest16(acc[i + u][j][2 * q]), rest16(acc[i + u][j][2 * q + 1]), PST_F16);
-        store_pair(to + g.dplane + i * 32, w, p.lane);
+          for (int q = 0; q < 2; ++q) w[u][q] = pack2(acc[i + u][j][2 * q], acc[i + u][j][2 * q + 1], TYPE);
+        store_pair(to + i * 32, w, p.lane);
+        if (E == F16 && g.dplanes == 2) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) w[u][q] = pack2(rest16(acc[i + u][j][2 * q]), rest16(acc[i + u][j][2 * q + 1]), PST_F16);
+          store_pair(to + g.dplane + i * 32, w, p.lane);
+        }
       }
     }
+  }
+};
+
+template <int E, class T>
+__global__ __launch_bounds__(T::THREADS, 2) void k_dlogit(GemmArgs g) {
+  extern __shared__ char smem[];
+  if ((int)blockIdx.x < g.blocks) {
+    tiles<E, T, true>(g, blockIdx.x, g.blocks, g.nm, 0, smem, DlogitEpilogue<E>{});
+  } else if constexpr (T::HAS_THIN) {
+    tiles<E, typename T::Thin, false>(g, blockIdx.x - g.blocks, 1 << 30, 1, g.nm * T::BM, smem, DlogitEpilogue<E>{});
   }
 }
 
@@ -514,6 +639,7 @@ __global__ __launch_bounds__(256) void k_finish(FinishArgs a) {
     const int64_t n = g / per;
     const int c = (int)(g - n * per) * 4;
     f32x4 s = {0, 0, 0, 0};
+#pragma unroll 4
     for (int z = 0; z < f.nz; ++z) {
       const f32x4 v = *(const f32x4*)(f.part + z * f.zstride + n * f.ldp + c);
       s.x += v.x;
@@ -528,26 +654,34 @@ __global__ __launch_bounds__(256) void k_finish(FinishArgs a) {
   }
 }
 
-// A wave's blocks as rows of a matrix of 32- or 16-bit floats: column n of the product is row `row0 + n` of the output,
-// which has M columns. `wide`: rows and base allow 16-byte stores (of 16-bit values: two blocks make 16 bytes a lane).
-template <class T>
-__device__ __forceinline__ void store_rows(const f32x4 (&acc)[T::MI][T::NI], const GemmArgs& g, const Place<T>& p, int64_t row0) {
+// A wave's blocks as rows of a matrix of OT: column n of the product is row `row0 + n` of the output, which has M
+// columns. `wide`: rows and base allow 16-byte stores (of 16-bit values: two blocks make 16 bytes a lane).
+template <int OT, class T>
+__device__ __forceinline__ void store_rows_of(const f32x4 (&acc)[T::MI][T::NI], const GemmArgs& g, const Place<T>& p, int64_t row0) {
   const bool whole = g.wide && p.mwave + T::MI * 16 <= g.M;
 #pragma unroll
   for (int j = 0; j < T::NI; ++j) {
     const int n = p.nw + 16 * j + p.col;
     const bool row = n < g.N;
     const int64_t at = (row0 + n) * g.ldo;
-    if (whole && g.otype != PST_F32) {
-      char* to = (char*)g.out + (at + p.mwave) * 2;
+    if (whole) {
+      if (OT == PST_F32) {
+        float* to = (float*)g.out + at + p.mw;
+        if (row) {
 #pragma unroll
-      for (int i = 0; i < T::MI; i += 2) {
-        uint32_t w[2][2];
+          for (int i = 0; i < T::MI; ++i) *(f32x4*)(to + 16 * i) = acc[i][j];
+        }
+      } else {
+        char* to = (char*)g.out + (at + p.mwave) * 2;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int i = 0; i < T::MI; i += 2) {
+          uint32_t w[2][2];
 #pragma unroll
-          for (int q = 0; q < 2; ++q) w[u][q] = pack2(acc[i + u][j][2 * q], acc[i + u][j][2 * q + 1], g.otype);
-        store_pair(to + i * 32, w, p.lane, row);
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) w[u][q] = pack2(acc[i + u][j][2 * q], acc[i + u][j][2 * q + 1], OT);
+          store_pair(to + i * 32, w, p.lane, row);
+        }
       }
     } else if (row) {
 #pragma unroll
@@ -555,63 +689,92 @@ __device__ __forceinline__ void store_rows(const f32x4 (&acc)[T::MI][T::NI], con
         const int m = p.mw + 16 * i;
         if (m >= g.M) continue;
         const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-        store4(g.out, g.otype, at + m, v, g.M - m, g.wide);
+        store4(g.out, OT, at + m, v, g.M - m, g.wide);
       }
     }
   }
+}
+template <class T>
+__device__ __forceinline__ void store_rows(const f32x4 (&acc)[T::MI][T::NI], const GemmArgs& g, const Place<T>& p, int64_t row0) {
+  if (g.otype == PST_BF16) store_rows_of<PST_BF16, T>(acc, g, p, row0);
+  else if (g.otype == PST_F16) store_rows_of<PST_F16, T>(acc, g, p, row0);
+  else store_rows_of<PST_F32, T>(acc, g, p, row0);
 }
 
 // Both gradients of a piece of the vocabulary in one launch, since D feeds both and neither fills the card evenly:
 // dx's parts (m = column, n = position, k = vocabulary row of the piece, its K loop in nz parts) and rows v0 ... of dW
 // (m = column, n = vocabulary row, k = position; in one part straight to the output, or in parts as dx).
-template <int E, class T>
-__global__ __launch_bounds__(T::THREADS) void k_grads(GradArgs g) {
-  extern __shared__ char smem[];
-  const bool first = (int)blockIdx.x < g.dx_tiles;
+template <int E, class T, bool DX>
+__device__ __forceinline__ void grad_tile(const GemmArgs& g, int tile, int nn, int n_base, char* smem) {
+  const Place<T> p(g, tile, g.nm, nn, 0, n_base);
+  const int s0 = (int)((int64_t)g.steps * p.z / g.nz), s1 = (int)((int64_t)g.steps * (p.z + 1) / g.nz);
   f32x4 acc[T::MI][T::NI];
-  if (first) {
-    const Place<T> p(g.dx, blockIdx.x);
-    const int s0 = (int)((int64_t)g.dx.steps * p.z / g.dx.nz), s1 = (int)((int64_t)g.dx.steps * (p.z + 1) / g.dx.nz);
-    multiply<E, T, true, false>(acc, g.dx.A, g.dx.B, g.dx.k, p.m0, p.n0, s0, s1, smem);
-    store_part<T>(acc, g.dx, p);
+  Loop<E, T, true, !DX> loop(smem);
+  loop.begin(g.A, g.B, g.k, p.m0, p.n0, s0, s1);
+  loop.run(acc);
+  if (DX || g.part_out) {
+    store_part<T>(acc, g, p);
   } else {
-    const Place<T> p(g.dw, blockIdx.x - g.dx_tiles);
-    const int s0 = (int)((int64_t)g.dw.steps * p.z / g.dw.nz), s1 = (int)((int64_t)g.dw.steps * (p.z + 1) / g.dw.nz);
-    multiply<E, T, true, true>(acc, g.dw.A, g.dw.B, g.dw.k, p.m0, p.n0, s0, s1, smem);
-    if (g.dw.part_out) {
-      store_part<T>(acc, g.dw, p);
-    } else {
-      unscale<T>(acc, (g.dw.ua ? *g.dw.ua : 1.0f) * (g.dw.ub ? *g.dw.ub : 1.0f));
-      store_rows<T>(acc, g.dw, p, g.dw.v0);
-    }
+    unscale<T>(acc, (g.ua ? *g.ua : 1.0f) * (g.ub ? *g.ub : 1.0f));
+    store_rows<T>(acc, g, p, g.v0);
+  }
+}
+// workgroups: dx's tiles, dW's, then the thin ones of dx and of dW
+template <int E, class T>
+__global__ __launch_bounds__(T::THREADS, 2) void k_grads(GradArgs g) {
+  extern __shared__ char smem[];
+  int b = blockIdx.x;
+  if (b < g.blocks[0]) return grad_tile<E, T, true>(g.dx, b, g.dx.nn, 0, smem);
+  b -= g.blocks[0];
+  if (b < g.blocks[1]) return grad_tile<E, T, false>(g.dw, b, g.dw.nn, 0, smem);
+  if constexpr (T::HAS_THIN) {
+    b -= g.blocks[1];
+    if (b < g.blocks[2]) return grad_tile<E, typename T::ThinN, true>(g.dx, b, 1, g.dx.nn * T::BN, smem);
+    grad_tile<E, typename T::ThinN, false>(g.dw, b - g.blocks[2], 1, g.dw.nn * T::BN, smem);
   }
 }
 
 // 8-bit scores: m = vocabulary row, n = position
-template <class T>
-__global__ __launch_bounds__(T::THREADS) void k_scores(GemmArgs g) {
-  extern __shared__ char smem[];
-  const Place<T> p(g, blockIdx.x);
-  i32x4 sums[T::MI][T::NI];
-  multiply<I8, T, false, false>(sums, g.A, g.B, g.k, p.m0, p.n0, 0, g.steps, smem);
-  f32x4 acc[T::MI][T::NI];
-#pragma unroll
-  for (int j = 0; j < T::NI; ++j) {
-    const float sn = g.sn[min(p.nw + 16 * j + p.col, g.N - 1)];
-#pragma unroll
-    for (int i = 0; i < T::MI; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) acc[i][j][r] = (float)sums[i][j][r] * sn;
+struct ScoresEpilogue {
+  struct Inputs {
+    float sm, sn;
+  };
+  template <class P>
+  __device__ __forceinline__ Inputs load(const GemmArgs& g, const P& p) const {
+    const int i = (int)threadIdx.x & 255;
+    return {i < P::BM ? g.sm[min(p.m0 + i, g.M - 1)] : 0.0f, i < P::BN ? g.sn[min(p.n0 + i, g.N - 1)] : 0.0f};
   }
-#pragma unroll
-  for (int i = 0; i < T::MI; ++i)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const float sv = g.sm[min(p.mw + 16 * i + r, g.M - 1)];
-#pragma unroll
-      for (int j = 0; j < T::NI; ++j) acc[i][j][r] *= sv;
+  __device__ __forceinline__ void share(const Inputs& in, float* lds) const {
+    asm volatile("" ::"v"(in.sm), "v"(in.sn));
+    if (threadIdx.x < 256) {
+      lds[threadIdx.x] = in.sm;
+      lds[256 + threadIdx.x] = in.sn;
     }
-  store_rows<T>(acc, g, p, 0);
+  }
+  template <class T>
+  __device__ __forceinline__ void store(const GemmArgs& g, const Place<T>& p, i32x4 (&sums)[T::MI][T::NI], float* lds) const {
+    f32x4 acc[T::MI][T::NI];
+#pragma unroll
+    for (int i = 0; i < T::MI; ++i) {
+      const f32x4 sv = *(const f32x4*)(lds + p.mw - p.m0 + 16 * i);
+#pragma unroll
+      for (int j = 0; j < T::NI; ++j) {
+        const float sn = lds[256 + p.nw - p.n0 + 16 * j + p.col];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[i][j][r] = (float)sums[i][j][r] * sn * sv[r];
+      }
+    }
+    store_rows<T>(acc, g, p, 0);
+  }
+};
+template <class T>
+__global__ __launch_bounds__(T::THREADS, 2) void k_scores(GemmArgs g) {
+  extern __shared__ char smem[];
+  if ((int)blockIdx.x < g.blocks) {
+    tiles<I8, T, true>(g, blockIdx.x, g.blocks, g.nm, 0, smem, ScoresEpilogue{});
+  } else if constexpr (T::HAS_THIN) {
+    tiles<I8, typename T::Thin, false>(g, blockIdx.x - g.blocks, 1 << 30, 1, g.nm * T::BM, smem, ScoresEpilogue{});
+  }
 }
 
 struct QuantArgs {
@@ -621,19 +784,58 @@ struct QuantArgs {
   int32_t width, width_pad, type;  // columns width .. width_pad - 1 become zeros
   int8_t* q;
   float* scale;
+  int32_t wide_in, wide_out;       // rows allow 16-byte loads, 8-byte stores
 };
-// one wave a row: the largest magnitude, then rint(x / s). A row that holds an infinity or a NaN gets the scale
-// NaN and zeros, so that what is computed from it says so.
+// eight neighbours of a row from column c, zeros behind the last; `wide`: 16-byte loads
+__device__ __forceinline__ void load8(const QuantArgs& a, int64_t row, int c, float* v) {
+  if (a.wide_in && c + 8 <= a.width) {
+    if (a.type == PST_F32) {
+      const f32x4 lo = *(const f32x4*)((const float*)a.src + row + c), hi = *(const f32x4*)((const float*)a.src + row + c + 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = lo[j], v[4 + j] = hi[j];
+    } else {
+      const uint4 w = *(const uint4*)((const uint16_t*)a.src + row + c);
+      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint16_t h = (uint16_t)(u[j / 2] >> (16 * (j & 1)));
+        v[j] = a.type == PST_BF16 ? __uint_as_float((uint32_t)h << 16) : (float)__builtin_bit_cast(_Float16, h);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = c + j < a.width ? load1(a.src, a.type, row + c + j) : 0.0f;
+}
+// One wave a row: the largest magnitude, then rint(x / s), rows of up to 512 ITERS values read once. A row that holds
+// an infinity or a NaN gets the scale NaN and zeros, so that what is computed from it says so.
+// 8192 x 1024 bf16 -> 8 bits moves 25 MB.
+template <int ITERS>
 __global__ __launch_bounds__(256) void k_quantize(QuantArgs a) {
   const int lane = threadIdx.x & 63;
   const int64_t r = blockIdx.x * (int64_t)4 + (threadIdx.x >> 6);
   if (r >= a.rows) return;
+  const int64_t row = r * a.ld;
+  float held[ITERS ? ITERS : 1][8];
   float m = 0.0f;
   bool bad = false;
-  for (int k = lane; k < a.width; k += 64) {
-    const float v = fabsf(load1(a.src, a.type, r * a.ld + k));
-    bad |= !(v <= 3.4028234663852886e38f);
-    m = fmaxf(m, v);
+  auto look = [&](const float* v) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      bad |= !(fabsf(v[j]) <= 3.4028234663852886e38f);
+      m = fmaxf(m, fabsf(v[j]));
+    }
+  };
+  if (ITERS) {
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i) load8(a, row, i * 512 + lane * 8, held[i]);
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i) look(held[i]);
+  } else {
+    for (int c = lane * 8; c < a.width; c += 512) {
+      load8(a, row, c, held[0]);
+      look(held[0]);
+    }
   }
 #pragma unroll
   for (int s = 32; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
@@ -641,11 +843,29 @@ __global__ __launch_bounds__(256) void k_quantize(QuantArgs a) {
   const float s = m * (1.0f / 127.0f);
   if (lane == 0) a.scale[r] = bad ? __builtin_nanf("") : s;
   const bool zero = bad || !(s > 0.0f);
-  for (int k = lane; k < a.width_pad; k += 64) {
-    int q = 0;
-    // a subnormal scale can make the quotient pass 127
-    if (k < a.width && !zero) q = (int)fminf(fmaxf(rintf(load1(a.src, a.type, r * a.ld + k) / s), -127.0f), 127.0f);
-    a.q[r * a.ldq + k] = (int8_t)q;
+  auto write = [&](int c, const float* v) {
+    uint32_t q[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)  // (a subnormal scale can make the quotient pass 127)
+      q[j] = zero ? 0u : (uint32_t)(int)fminf(fmaxf(rintf(v[j] / s), -127.0f), 127.0f) & 255u;
+    int8_t* to = a.q + r * a.ldq + c;
+    if (a.wide_out && c + 8 <= a.width_pad) {
+      *(uint2*)to = make_uint2(q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24, q[4] | q[5] << 8 | q[6] << 16 | q[7] << 24);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + j < a.width_pad) to[j] = (int8_t)q[j];
+    }
+  };
+  if (ITERS) {
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i)
+      if (i * 512 + lane * 8 < a.width_pad) write(i * 512 + lane * 8, held[i]);
+  } else {
+    for (int c = lane * 8; c < a.width_pad; c += 512) {
+      load8(a, row, c, held[0]);
+      write(c, held[0]);
+    }
   }
 }
 // 8-bit rows into whole K-steps
@@ -717,14 +937,36 @@ bool in_place(const void* p, int64_t ld_bytes, int64_t row_bytes) {
   return ((uintptr_t)p & 15) == 0 && ld_bytes % 16 == 0 && row_bytes % 16 == 0;
 }
 
-#ifndef T256W
-#define T256W 2, 4
-#endif
-using T256 = Tile<256, 256, T256W>;
-using T128 = Tile<128, 128, 2, 2>;
-using T64 = Tile<64, 64, 2, 2>;
 enum TileId { TILE64 = 0, TILE128 = 1, TILE256 = 2 };
 constexpr int TILE_M[3] = {64, 128, 256};
+
+// ---- the choice of tiles
+// Times of a workgroup in us, fitted to single launches on the card (d = 128 ... 1024, 16 ... 8192 positions): a launch's
+// tiles run in rounds of `slots`, and a tile costs BASE + PER_STEP * K-steps when its compute unit is full.
+//   256: 1 a unit, 1.5 us a K-step of 64 (all of them 1.4 PFLOP/s);  128: 2 a unit, 1.1;  64: 4 a unit, 0.85
+constexpr int CUS = 256;  // the card's compute units, whatever device is asked: a workspace's size needs none
+constexpr double TILE_BASE[3] = {2.0, 3.0, 4.0}, TILE_STEP[3] = {0.85, 1.1, 1.5};
+constexpr int TILE_SLOTS[3] = {4, 2, 1};
+double tile_us(int tile, int64_t steps) { return TILE_BASE[tile] + TILE_STEP[tile] * steps; }
+int64_t tiles_of(int64_t m, int64_t n, int tile) { return ceil_div(m, TILE_M[tile]) * ceil_div(n, TILE_M[tile]); }
+// rows that thin tiles take
+int64_t thin_rows(int64_t m, int tile) {
+  const int64_t rest = m % TILE_M[TILE256];
+  return tile == TILE256 && m > rest && rest <= 64 ? rest : 0;
+}
+// m x n of the loss, the logits' gradient and the scores
+int tile_for(int64_t m, int64_t n, int64_t steps) {
+  int best = TILE64;
+  double us = 1e30;
+  for (int t = TILE256; t >= TILE64; --t) {
+    const int64_t thin = thin_rows(m, t), slots = (int64_t)CUS * TILE_SLOTS[t], full = tiles_of(m - thin, n, t);
+    double e = ceil_div(full, slots) * tile_us(t, steps);
+    // thin tiles take what the last round leaves free, or about half a round
+    if (thin && tiles_of(m, n, t) > ceil_div(full, slots) * slots) e += 0.5 * tile_us(t, steps);
+    if (e < us) us = e, best = t;
+  }
+  return best;
+}
 
 template <class F, class A>
 hipError_t launch(F* f, int64_t grid, int threads, int lds, hipStream_t st, const A& g) {
@@ -737,12 +979,12 @@ hipError_t launch(F* f, int64_t grid, int threads, int lds, hipStream_t st, cons
   return hipGetLastError();
 }
 template <int E, class T>
-hipError_t launch_kind(int kind, const GemmArgs& g, hipStream_t st) {
-  const int64_t grid = (int64_t)g.nm * g.nn;
+hipError_t launch_kind(int kind, const GemmArgs& g, int64_t grid, hipStream_t st) {
+  constexpr int LDS = T::LDS + EPILOGUE_LDS;
   if constexpr (E == I8) {
-    return launch(k_scores<T>, grid, T::THREADS, T::LDS, st, g);
+    return launch(k_scores<T>, grid, T::THREADS, LDS, st, g);
   } else {
-    return kind == LOSS ? launch(k_loss<E, T>, grid, T::THREADS, T::LDS, st, g) : launch(k_dlogit<E, T>, grid, T::THREADS, T::LDS, st, g);
+    return kind == LOSS ? launch(k_loss<E, T>, grid, T::THREADS, LDS, st, g) : launch(k_dlogit<E, T>, grid, T::THREADS, LDS, st, g);
   }
 }
 void set_tiles(GemmArgs& g, int64_t m, int64_t n, int tile) {
@@ -752,12 +994,21 @@ void set_tiles(GemmArgs& g, int64_t m, int64_t n, int tile) {
   g.gm = 4;
 }
 template <int E>
-hipError_t launch_elem(int kind, int tile, const GemmArgs& g, hipStream_t st) {
-  return tile == TILE256 ? launch_kind<E, T256>(kind, g, st) : tile == TILE128 ? launch_kind<E, T128>(kind, g, st) : launch_kind<E, T64>(kind, g, st);
+hipError_t launch_elem(int kind, int tile, const GemmArgs& g, int64_t grid, hipStream_t st) {
+  return tile == TILE256   ? launch_kind<E, T256>(kind, g, grid, st)
+         : tile == TILE128 ? launch_kind<E, T128>(kind, g, grid, st)
+                           : launch_kind<E, T64>(kind, g, grid, st);
 }
 hipError_t launch_gemm(int kind, int elem, int tile, GemmArgs g, hipStream_t st) {
-  set_tiles(g, g.M, g.N, tile);
-  return elem == I8 ? launch_elem<I8>(kind, tile, g, st) : elem == BF16 ? launch_elem<BF16>(kind, tile, g, st) : launch_elem<F16>(kind, tile, g, st);
+  const int64_t thin = thin_rows(g.M, tile);
+  set_tiles(g, g.M - thin, g.N, tile);
+  const int64_t tiles = (int64_t)g.nm * g.nn;
+  if (tiles > 0x3fffffff) return hipErrorInvalidConfiguration;
+  g.blocks = (int32_t)std::min<int64_t>(tiles, (int64_t)CUS * TILE_SLOTS[tile]);
+  const int64_t grid = g.blocks + (thin ? g.nn : 0);
+  return elem == I8     ? launch_elem<I8>(kind, tile, g, grid, st)
+         : elem == BF16 ? launch_elem<BF16>(kind, tile, g, grid, st)
+                        : launch_elem<F16>(kind, tile, g, grid, st);
 }
 template <int E>
 hipError_t launch_grads_elem(int tile, const GradArgs& g, int64_t grid, hipStream_t st) {
@@ -766,46 +1017,19 @@ hipError_t launch_grads_elem(int tile, const GradArgs& g, int64_t grid, hipStrea
                            : launch(k_grads<E, T64>, grid, T64::THREADS, T64::LDS, st, g);
 }
 hipError_t launch_grads(int elem, int tile, GradArgs g, bool dx, bool dw, hipStream_t st) {
-  set_tiles(g.dx, g.dx.ldp, g.dx.N, tile);
-  set_tiles(g.dw, g.dw.M, g.dw.N, tile);
-  const int64_t a = dx ? (int64_t)g.dx.nm * g.dx.nn * g.dx.nz : 0, b = dw ? (int64_t)g.dw.nm * g.dw.nn * g.dw.nz : 0;
-  g.dx_tiles = (int32_t)std::min<int64_t>(a, 0x7fffffff);
-  return elem == BF16 ? launch_grads_elem<BF16>(tile, g, a + b, st) : launch_grads_elem<F16>(tile, g, a + b, st);
-}
-
-int cus_of(int device, int* cus) {
-  HEADCHK(hipDeviceGetAttribute(cus, hipDeviceAttributeMultiprocessorCount, device));
-  return PST_OK;
-}
-
-// ---- the choice of tiles
-// Times of a workgroup in us, fitted to single launches on the card (d = 128 ... 1024, 16 ... 8192 positions): a launch's
-// tiles run in rounds of `slots`, and a tile costs BASE + PER_STEP * K-steps when its compute unit is full.
-//   256: 1 a unit, 1.5 us a K-step of 64 (all of them 1.4 PFLOP/s);  128: 2 a unit, 1.1;  64: 4 a unit, 0.85
-constexpr double TILE_BASE[3] = {2.0, 3.0, 4.0}, TILE_STEP[3] = {0.85, 1.1, 1.5};
-constexpr int TILE_SLOTS[3] = {4, 2, 1};
-struct Work {
-  int64_t tiles;
-  int64_t steps;
-};
-// the estimate for one launch of up to two kinds of tiles
-double launch_us(int tile, Work a, Work b, int cus) {
-  const double slots = (double)cus * TILE_SLOTS[tile];
-  const double ta = TILE_BASE[tile] + TILE_STEP[tile] * a.steps, tb = b.tiles ? TILE_BASE[tile] + TILE_STEP[tile] * b.steps : 0;
-  const double longest = std::max(ta, tb), all = (a.tiles * ta + b.tiles * tb) / slots;
-  // whole rounds of one kind; two kinds even out
-  if (!b.tiles) return std::ceil(a.tiles / slots) * ta;
-  return all <= longest ? longest : all + 0.5 * longest;
-}
-int64_t tiles_of(int64_t m, int64_t n, int tile) { return ceil_div(m, TILE_M[tile]) * ceil_div(n, TILE_M[tile]); }
-int tile_for(int64_t m, int64_t n, int64_t steps, int cus) {
-  int best = TILE64;
-  double us = 1e30;
-  for (int t = TILE256; t >= TILE64; --t) {
-    const double e = launch_us(t, {tiles_of(m, n, t), steps}, {0, 0}, cus);
-    if (e < us) us = e, best = t;
+  int64_t grid = 0;
+  for (int i = 0; i < 2; ++i) {
+    GemmArgs& q = i ? g.dw : g.dx;
+    const int64_t thin = thin_rows(q.N, tile);
+    set_tiles(q, i ? q.M : q.ldp, q.N - thin, tile);
+    const bool on = i ? dw : dx;
+    const int64_t blocks = on ? (int64_t)q.nm * q.nn * q.nz : 0, thins = on && thin ? (int64_t)q.nm * q.nz : 0;
+    grid += blocks + thins;
+    if (grid > 0x7fffffff) return hipErrorInvalidConfiguration;
+    g.blocks[i] = (int32_t)blocks;
+    g.blocks[2 + i] = (int32_t)thins;
   }
-  return best;
+  return elem == BF16 ? launch_grads_elem<BF16>(tile, g, grid, st) : launch_grads_elem<F16>(tile, g, grid, st);
 }
 
 // What a call on [rows, width] x [vocab, width] needs of its workspace; the same for the query and for the call.
@@ -820,9 +1044,6 @@ struct Plan {
   int tile = 0, zx = 1, zw = 1;                  // of the two gradients' launch
   int64_t bytes = 0;
 };
-// the plans are made for the card's number of compute units, so that the query needs no device
-constexpr int CUS = 256;
-
 Plan plan_common(int type, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab, int64_t width, bool grad, Bump& b) {
   Plan p;
   p.type = type;
@@ -848,7 +1069,7 @@ Plan plan_common(int type, const void* x, int64_t ldx, const void* w, int64_t ld
 Plan plan_loss(int type, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab, int64_t width) {
   Bump b;
   Plan p = plan_common(type, x, ldx, w, ldw, rows, vocab, width, false, b);
-  p.tile = tile_for(vocab, rows, p.width_pad / 64 * (p.planes == 2 ? 3 : 1), CUS);
+  p.tile = tile_for(vocab, rows, p.width_pad / 64 * (p.planes == 2 ? 3 : 1));
   p.part = b.take(ceil_div(vocab, TILE_M[p.tile]) * rows * 8);
   p.tlogit = b.take(rows * 4);
   p.bytes = b.n;
@@ -876,9 +1097,16 @@ Plan plan_grad(int type, const void* x, int64_t ldx, const void* w, int64_t ldw,
       for (int zw = 1; zw <= (vocab > p.piece ? 1 : 16); zw *= 2) {
         const int64_t sx = ceil_div(nv, 64) * passes, sw = ceil_div(rows, 64) * passes;
         if ((zx > 1 && sx < 4 * zx) || (zw > 1 && sw < 4 * zw)) continue;
-        const double us = launch_us(t, {tiles_of(p.width_pad, rows, t) * zx, ceil_div(sx, zx)}, {tiles_of(width, nv, t) * zw, ceil_div(sw, zw)}, CUS);
+        // both kinds share the slots; the last to start ends half its time behind the rest
+        const double tx = tile_us(t, ceil_div(sx, zx)), tw = tile_us(t, ceil_div(sw, zw)), longest = std::max(tx, tw);
+        const int64_t thin_x = thin_rows(rows, t), thin_w = thin_rows(nv, t);
+        const double nx = (double)tiles_of(p.width_pad, rows - thin_x, t) * zx, nw = (double)tiles_of(width, nv - thin_w, t) * zw;
+        const double thins = 0.5 * ((thin_x ? tiles_of(p.width_pad, 1, t) * zx * tx : 0) + (thin_w ? tiles_of(width, 1, t) * zw * tw : 0));
+        const double slots = (double)CUS * TILE_SLOTS[t];
+        double us = (nx * tx + nw * tw + thins) / slots;
+        us = nx + nw <= slots ? longest + (thins > 0 && nx + nw + thins / longest > slots ? 0.5 * longest : 0) : std::max(us + 0.5 * longest, longest);
         const double bytes = 8.0 * p.width_pad * (rows * (double)zx + (zw > 1 ? vocab * (double)zw : 0.0));
-        const double e = us * ceil_div(vocab, p.piece) + bytes / 4e6;
+        const double e = us * ceil_div(vocab, p.piece) + bytes / 4e6 + 0.2 * (zx + zw);
         if (e < best) best = e, p.tile = t, p.zx = zx, p.zw = zw;
       }
   p.dxp = b.take(p.zx * rows * p.width_pad * 4);
@@ -910,12 +1138,11 @@ int check_ws(const void* ws, int64_t have, int64_t need) {
 }
 
 // grids of the copying kernels: a few workgroups a compute unit
-unsigned copy_grid(int64_t groups, int cus) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(groups, 256), cus * 16ll)); }
+unsigned copy_grid(int64_t groups) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(groups, 256), CUS * 16ll)); }
 
 // the operands in a form that the products read: in place, or packed (and split) into the workspace; for the gradient
 // (gloss) also the scale of D. One launch, two for 32-bit operands, none where there is nothing to do.
-int operands(const Plan& p, const void* x, int64_t ldx, const void* w, int64_t ldw, const Targets& t, const float* gloss, char* ws, int cus,
-             hipStream_t st, Operand* X, Operand* W) {
+int operands(const Plan& p, const void* x, int64_t ldx, const void* w, int64_t ldw, const Targets& t, const float* gloss, char* ws, hipStream_t st, Operand* X, Operand* W) {
   PackArgs a{};
   a.width = (int32_t)p.width;
   a.width_pad = (int32_t)p.width_pad;
@@ -931,7 +1158,7 @@ int operands(const Plan& p, const void* x, int64_t ldx, const void* w, int64_t l
     PackJob& j = a.job[which];
     j = {src, ld, rows, rows_pad, ws + at, rows_pad * p.width_pad * 2, (float*)(ws + p.amax) + which * AMAX_BLOCKS, (float*)(ws + p.unscale) + which,
          which == 0 && gloss, ((uintptr_t)src & 15) == 0 && ld * e % 16 == 0};
-    a.blocks[which] = (int32_t)copy_grid(rows_pad * (p.width_pad / 8), cus);
+    a.blocks[which] = (int32_t)copy_grid(rows_pad * (p.width_pad / (j.wide ? 8 : 2)));
     return Operand{ws + at, j.plane, p.width_pad * 2, (int32_t)rows_pad, (int32_t)p.width_pad * 2};
   };
   *X = p.pack_x ? job(0, x, ldx, p.rows, p.rows_pad, p.x) : Operand{(const char*)x, 0, ldx * e, (int32_t)p.rows, (int32_t)p.width * e};
@@ -965,13 +1192,10 @@ int token_loss(int device, int type, const void* x, int64_t ldx, const void* w, 
   if (rc != PST_OK) return rc;
   OnDevice on(device);
   if (on.e != hipSuccess) return hip_fail("device " + std::to_string(device), on.e);
-  int cus = 0;
-  rc = cus_of(device, &cus);
-  if (rc != PST_OK) return rc;
   char* ws = (char*)ws_;
   GemmArgs g{};
   g.targets = {targets, ignore, tbits, (int32_t)vocab};
-  rc = operands(p, x, ldx, w, ldw, g.targets, nullptr, ws, cus, st, &g.B, &g.A);
+  rc = operands(p, x, ldx, w, ldw, g.targets, nullptr, ws, st, &g.B, &g.A);
   if (rc != PST_OK) return rc;
   g.k = passes(p.planes);
   g.M = (int32_t)vocab;
@@ -1007,9 +1231,6 @@ int token_loss_grad(int device, int type, const void* x, int64_t ldx, const void
   if (rc != PST_OK) return rc;
   OnDevice on(device);
   if (on.e != hipSuccess) return hip_fail("device " + std::to_string(device), on.e);
-  int cus = 0;
-  rc = cus_of(device, &cus);
-  if (rc != PST_OK) return rc;
   char* ws = (char*)ws_;
   const Targets t{targets, ignore, tbits, (int32_t)vocab};
   // no positions: 64 of zeros stand for them, so that dW is written as the zeros that it is
@@ -1017,7 +1238,7 @@ int token_loss_grad(int device, int type, const void* x, int64_t ldx, const void
   q.rows = rows;
   Operand X, W;
   static const float none = 0.0f;  // (never read: there are no rows)
-  rc = operands(q, x, ldx, w, ldw, t, rows ? gloss : &none, ws, cus, st, &X, &W);
+  rc = operands(q, x, ldx, w, ldw, t, rows ? gloss : &none, ws, st, &X, &W);
   if (rc != PST_OK) return rc;
   const float* gs = p.type == PST_BF16 ? nullptr : (float*)(ws + p.gscale);
   const float* ungs = gs ? gs + 1 : nullptr;
@@ -1048,10 +1269,9 @@ int token_loss_grad(int device, int type, const void* x, int64_t ldx, const void
     g.D = D;
     g.dplane = dop.plane;
     g.ldd = ldd;
-    g.dtype = p.elem == BF16 ? PST_BF16 : PST_F16;
     g.dplanes = p.planes;
     g.v0 = (int32_t)v0;
-    if (rows) HEADCHK(launch_gemm(DLOGIT, p.elem, tile_for(nv, rows, g.steps * (p.planes == 2 ? 3 : 1), cus), g, st));
+    if (rows) HEADCHK(launch_gemm(DLOGIT, p.elem, tile_for(nv, rows, g.steps * (p.planes == 2 ? 3 : 1)), g, st));
     GradArgs b{};
     b.dx.k = b.dw.k = g.k;
     b.dx.A = Wv;
@@ -1088,7 +1308,7 @@ int token_loss_grad(int device, int type, const void* x, int64_t ldx, const void
   auto job = [&](int which, int64_t part, int64_t n, int nz, void* out, int64_t ldo, const float* u) {
     f.job[which] = {(const float*)(ws + part), p.width_pad, n * p.width_pad, n, nz, which == 0, out, ldo, ungs, u,
                     ldo % 4 == 0 && ((uintptr_t)out & (type == PST_F32 ? 15 : 7)) == 0};
-    f.blocks[which] = (int32_t)copy_grid(n * ceil_div(width, 4), cus);
+    f.blocks[which] = (int32_t)copy_grid(n * ceil_div(width, 4));
   };
   if (need_dx) job(0, p.dxp, rows, p.zx, dx, lddx, uw);
   if (dw && p.zw > 1) job(1, p.dwp, vocab, p.zw, dw, lddw, ux);
@@ -1097,6 +1317,17 @@ int token_loss_grad(int device, int type, const void* x, int64_t ldx, const void
     HEADCHK(hipGetLastError());
   }
   return PST_OK;
+}
+
+hipError_t launch_quantize(QuantArgs a, hipStream_t st) {
+  a.wide_in = in_place(a.src, a.ld * size_of(a.type), 16);
+  a.wide_out = ((uintptr_t)a.q & 7) == 0 && a.ldq % 8 == 0;
+  const dim3 grid((unsigned)ceil_div(a.rows, 4)), block(256);
+  if (a.width_pad <= 512) hipLaunchKernelGGL(k_quantize<1>, grid, block, 0, st, a);
+  else if (a.width_pad <= 1024) hipLaunchKernelGGL(k_quantize<2>, grid, block, 0, st, a);
+  else if (a.width_pad <= 2048) hipLaunchKernelGGL(k_quantize<4>, grid, block, 0, st, a);
+  else hipLaunchKernelGGL(k_quantize<0>, grid, block, 0, st, a);
+  return hipGetLastError();
 }
 
 int quantize_rows(int device, int type, const void* x, int64_t ldx, int64_t rows, int64_t width, int8_t* q, int64_t ldq, float* scale, hipStream_t st) {
@@ -1108,9 +1339,7 @@ int quantize_rows(int device, int type, const void* x, int64_t ldx, int64_t rows
   if (!x || ((uintptr_t)x % size_of(type)) || !q || !scale || ((uintptr_t)scale & 3)) return fail(PST_E_INVALID, "a buffer is null or not aligned to its type");
   OnDevice on(device);
   if (on.e != hipSuccess) return hip_fail("device " + std::to_string(device), on.e);
-  QuantArgs a{x, ldx, ldq, rows, (int32_t)width, (int32_t)width, type, q, scale};
-  hipLaunchKernelGGL(k_quantize, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, st, a);
-  HEADCHK(hipGetLastError());
+  HEADCHK(launch_quantize({x, ldx, ldq, rows, (int32_t)width, (int32_t)width, type, q, scale, 0, 0}, st));
   return PST_OK;
 }
 
@@ -1154,17 +1383,12 @@ int token_scores_i8(int device, int type, const void* x, int64_t ldx, const int8
   if (rc != PST_OK) return rc;
   OnDevice on(device);
   if (on.e != hipSuccess) return hip_fail("device " + std::to_string(device), on.e);
-  int cus = 0;
-  rc = cus_of(device, &cus);
-  if (rc != PST_OK) return rc;
   char* ws = (char*)ws_;
-  QuantArgs a{x, ldx, p.width_pad, rows, (int32_t)width, (int32_t)p.width_pad, type, (int8_t*)(ws + p.q), (float*)(ws + p.scale)};
-  hipLaunchKernelGGL(k_quantize, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, st, a);
-  HEADCHK(hipGetLastError());
+  HEADCHK(launch_quantize({x, ldx, p.width_pad, rows, (int32_t)width, (int32_t)p.width_pad, type, (int8_t*)(ws + p.q), (float*)(ws + p.scale), 0, 0}, st));
   GemmArgs g{};
   g.k = passes(1);
   if (p.pack_w) {
-    hipLaunchKernelGGL(k_pack8, dim3(copy_grid(vocab * (p.width_pad / 16), cus)), dim3(256), 0, st, w, ldw, vocab, (int32_t)width, (int32_t)p.width_pad,
+    hipLaunchKernelGGL(k_pack8, dim3(copy_grid(vocab * (p.width_pad / 16))), dim3(256), 0, st, w, ldw, vocab, (int32_t)width, (int32_t)p.width_pad,
                        (int8_t*)(ws + p.w));
     HEADCHK(hipGetLastError());
     g.A = {ws + p.w, 0, p.width_pad, (int32_t)vocab, (int32_t)p.width_pad};
@@ -1181,7 +1405,7 @@ int token_scores_i8(int device, int type, const void* x, int64_t ldx, const int8
   g.wide = ldo % (16 / size_of(otype)) == 0 && ((uintptr_t)out & 15) == 0;
   g.sn = (const float*)(ws + p.scale);
   g.sm = wscale;
-  HEADCHK(launch_gemm(SCORES, I8, tile_for(vocab, rows, g.steps, cus), g, st));
+  HEADCHK(launch_gemm(SCORES, I8, tile_for(vocab, rows, g.steps), g, st));
   return PST_OK;
 }
 

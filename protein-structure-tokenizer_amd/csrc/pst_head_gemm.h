@@ -90,16 +90,15 @@ __device__ __forceinline__ void load_lds(const char* base, uint32_t off, uint32_
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory");
 }
 
-// Everything this wave has loaded has landed and everything it read from LDS has been read, then all waves meet.
-__device__ __forceinline__ void landed_and_met() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-}
-
-// The same with the last N loads still in flight.
+// All but the last N of this wave's loads have landed (they return in the order of their issue) and everything it read
+// from LDS has been read, then all waves meet.
 template <int N>
 __device__ __forceinline__ void landed_but() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
+
+// All waves meet, with what they wrote to LDS and whatever loads in flight.
+__device__ __forceinline__ void met() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // COLS: what the number of a 32-byte piece of LDS row k is xored with, rows of RT bytes. A read takes k-rows
 // 8 g + i (g, i = 0..3) and one piece of each: eight places of the 256-byte bank row, each twice.
@@ -195,57 +194,77 @@ template <int BM_, int BN_, int WM_, int WN_>
 struct Tile {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NW = WM_ * WN_, THREADS = NW * 64;
   static constexpr int MI = BM_ / WM_ / 16, NI = BN_ / WN_ / 16;  // a wave's 16x16 blocks
-  static constexpr int STAGE = (BM_ + BN_) * STEP, LDS = 2 * STAGE;
+  static constexpr int STAGE = (BM_ + BN_) * STEP, LDS = 2 * STAGE;  // (an epilogue's own LDS lies behind)
 };
 
-// The K loop: acc[MI][NI] of this wave. Two LDS stages: the loads of K-step t + 2 start when all waves have read the
-// last of step t, and fly while t + 1 is multiplied. A K-step is four parts, (k half, half of the wave's rows): each
-// part's fragments are read from LDS while the part before is multiplied, also across the one barrier of a K-step.
+// The K loop of one tile after another: begin() starts the loads of a tile's first two K-steps, run() leaves the tile's
+// sums in acc[MI][NI] of this wave. Between them a workgroup can store the tile before.
+// Two LDS stages: the loads of K-step t + 2 start when all waves have read the last of step t, and fly while t + 1 is
+// multiplied. A K-step is four parts, (k half, half of the wave's rows): each part's fragments are read from LDS while
+// the part before is multiplied, also across the one barrier of a K-step.
+// Measured at 8192 x 16128 x 1024 bf16 (216 us as it is): K-steps of 64 bytes in rings of 3, 4 and 5 stages 226 - 228 (twice
+// the barriers; deeper prefetch gains nothing), two 256 x 128 workgroups a unit 252 (half as much again through LDS),
+// four waves of 128 x 128 224, blocks of 32 x 32 227.
 template <int E, class T, bool ACOLS, bool BCOLS>
-__device__ __forceinline__ void multiply(typename Mma<E>::Acc (&acc)[T::MI][T::NI], const Operand& A, const Operand& B,
-                                         const KLoop& kl, int m0, int n0, int step0, int step1, char* smem) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave / T::WN, wn = wave % T::WN;
-  constexpr int HI = T::MI / 2;
+struct Loop {
+  typedef typename Mma<E>::Acc Acc;
+  static constexpr int HI = T::MI / 2;
   // blocks of a wave start at a multiple of their number, so that a COLS read can xor the block into its address
   static_assert((T::MI & (T::MI - 1)) == 0 && (T::NI & (T::NI - 1)) == 0 && T::MI >= 2 && T::NI >= 2, "wave tile");
+  static constexpr int LA = Stager<T::BM, ACOLS, T::NW>::NI, LB = Stager<T::BN, BCOLS, T::NW>::NI;
   Stager<T::BM, ACOLS, T::NW> sa;
   Stager<T::BN, BCOLS, T::NW> sb;
-  sa.init(A, m0, lane, wave);
-  sb.init(B, n0, lane, wave);
   Reader<T::BM, ACOLS> ra;
   Reader<T::BN, BCOLS> rb;
-  ra.init(wm * T::MI, lane);
-  rb.init(wn * T::NI, lane);
-#pragma unroll
-  for (int i = 0; i < T::MI; ++i)
-#pragma unroll
-    for (int j = 0; j < T::NI; ++j) acc[i][j] = {0, 0, 0, 0};
-  const uint32_t lds0 = lds_addr(smem);
-  const int steps = step1 - step0, total = steps * kl.segs;
-  int seg = 0, step = step0;  // what is loaded next
-  constexpr int LA = Stager<T::BM, ACOLS, T::NW>::NI, LB = Stager<T::BN, BCOLS, T::NW>::NI;
-  auto aim = [&](int stage) {
+  const char* smem;
+  uint32_t lds0;
+  int lane, wave;
+  int64_t plane_a, plane_b;
+  KLoop kl;
+  int step0, step1, total, seg, step;  // seg, step: what is loaded next
+
+  __device__ __forceinline__ explicit Loop(const char* smem_) : smem(smem_), lds0(lds_addr(smem_)) {
+    lane = threadIdx.x & 63;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    ra.init(wave / T::WN * T::MI, lane);
+    rb.init(wave % T::WN * T::NI, lane);
+  }
+  __device__ __forceinline__ void aim(int stage) {
     const uint32_t to = lds0 + stage * T::STAGE;
-    sa.aim((int64_t)((kl.seg_a >> (2 * seg)) & 3) * A.plane, step, to, lane, wave);
-    sb.aim((int64_t)((kl.seg_b >> (2 * seg)) & 3) * B.plane, step, to + T::BM * STEP, lane, wave);
+    sa.aim((int64_t)((kl.seg_a >> (2 * seg)) & 3) * plane_a, step, to, lane, wave);
+    sb.aim((int64_t)((kl.seg_b >> (2 * seg)) & 3) * plane_b, step, to + T::BM * STEP, lane, wave);
     if (++step == step1) {
       step = step0;
       ++seg;
     }
-  };
-  auto load = [&](int i) {
+  }
+  __device__ __forceinline__ void load(int i) const {
     if (i < LA) sa.one(i);
     else sb.one(i - LA);
-  };
-  auto issue = [&](int stage) {
+  }
+  __device__ __forceinline__ void issue(int stage) {
     aim(stage);
 #pragma unroll
     for (int i = 0; i < LA + LB; ++i) load(i);
-  };
+  }
+  // K-steps [from, to) of each pass; all waves have left the stages
+  __device__ __forceinline__ void begin(const Operand& A, const Operand& B, const KLoop& k, int m0, int n0, int from, int to) {
+    sa.init(A, m0, lane, wave);
+    sb.init(B, n0, lane, wave);
+    plane_a = A.plane;
+    plane_b = B.plane;
+    kl = k;
+    step0 = step = from;
+    step1 = to;
+    seg = 0;
+    total = (to - from) * k.segs;
+    if (total > 0) issue(0);
+    if (total > 1) issue(1);
+  }
+
   i32x4 a[2][HI], b[2][T::NI];
   // fragments of part p of the K-step in `stage`
-  auto fetch = [&](int stage, int p) {
+  __device__ __forceinline__ void fetch(int stage, int p) {
     const char* ta = smem + stage * T::STAGE;
     const char* tb = ta + T::BM * STEP;
 #pragma unroll
@@ -255,16 +274,17 @@ __device__ __forceinline__ void multiply(typename Mma<E>::Acc (&acc)[T::MI][T::N
       for (int j = 0; j < T::NI; ++j) b[p >> 1][j] = rb.get(tb, j, p >> 1);
     }
     __builtin_amdgcn_sched_barrier(0);
-  };
-  // multiplies part p; with `more` the loads of a K-step spread between the multiplications, since the unit that takes
-  // them accepts one in 16 clocks of the whole workgroup and a wave behind it would wait with idle matrix cores
-  auto mult = [&](int p, auto more) {
+  }
+  // multiplies part p; MORE: with the loads of a K-step spread between the multiplications, since the unit that takes them
+  // accepts one in 16 clocks of the whole workgroup and a wave behind it would wait with idle matrix cores
+  template <bool MORE>
+  __device__ __forceinline__ void mult(Acc (&acc)[T::MI][T::NI], int p) {
     constexpr int TOTAL = HI * T::NI;
 #pragma unroll
     for (int q = 0; q < TOTAL; ++q) {
       const int i = q / T::NI, j = q % T::NI;
       acc[(p & 1) * HI + i][j] = Mma<E>::mma(a[p & 1][i], b[p >> 1][j], acc[(p & 1) * HI + i][j]);
-      if constexpr (more.value) {
+      if constexpr (MORE) {
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int l = q * (LA + LB) / TOTAL; l < (q + 1) * (LA + LB) / TOTAL; ++l) load(l);
@@ -272,38 +292,45 @@ __device__ __forceinline__ void multiply(typename Mma<E>::Acc (&acc)[T::MI][T::N
       }
     }
     __builtin_amdgcn_sched_barrier(0);
-  };
-  if (total > 0) {
-    issue(0);
-    if (total > 1) {
-      issue(1);
-      landed_but<LA + LB>();
-    } else {
-      landed_and_met();
-    }
-    fetch(0, 0);
   }
-  auto body = [&](int t, auto more, auto next) {
+  // one K-step; MORE: another one is loaded into its stage, NEXT: another one follows
+  template <bool MORE, bool NEXT>
+  __device__ __forceinline__ void body(Acc (&acc)[T::MI][T::NI], int t) {
     fetch(t & 1, 1);
-    mult(0, std::false_type{});
+    mult<false>(acc, 0);
     fetch(t & 1, 2);
-    mult(1, std::false_type{});
+    mult<false>(acc, 1);
     fetch(t & 1, 3);
-    mult(2, std::false_type{});
+    mult<false>(acc, 2);
     // the last fragments of step t are in registers: its stage is free once all waves are here
-    if constexpr (next.value) {
-      landed_and_met();
+    if constexpr (NEXT) {
+      landed_but<0>();
       fetch((t + 1) & 1, 0);
     }
-    if constexpr (more.value) aim(t & 1);
-    mult(3, more);
-  };
-  int t = 0;
-  for (; t + 2 < total; ++t) body(t, std::true_type{}, std::true_type{});
-  if (t + 1 < total) body(t++, std::false_type{}, std::true_type{});
-  if (t < total) body(t, std::false_type{}, std::false_type{});
-  landed_and_met();  // the stages are free for the epilogue
-}
+    if constexpr (MORE) aim(t & 1);
+    mult<MORE>(acc, 3);
+  }
+  __device__ __forceinline__ void run(Acc (&acc)[T::MI][T::NI]) {
+#pragma unroll
+    for (int i = 0; i < T::MI; ++i)
+#pragma unroll
+      for (int j = 0; j < T::NI; ++j) acc[i][j] = {0, 0, 0, 0};
+    if (total > 0) {
+      // (what this wave stored since begin() counts as loads in flight do, so this may wait for some of it)
+      if (total > 1) {
+        landed_but<LA + LB>();
+      } else {
+        landed_but<0>();
+      }
+      fetch(0, 0);
+    }
+    int t = 0;
+    for (; t + 2 < total; ++t) body<true, true>(acc, t);
+    if (t + 1 < total) body<false, true>(acc, t++);
+    if (t < total) body<false, false>(acc, t);
+    landed_but<0>();  // the stages are free
+  }
+};
 
 // Tiles of a grid in the order that keeps an XCD's L2 warm: workgroup b runs on XCD b % 8, each XCD takes one
 // contiguous range of the tiles, and within it `gm` tiles along m share each tile along n.

@@ -18,7 +18,7 @@ import functools
 from . import _native
 
 _TYPES = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}  # PST_F32, PST_BF16, PST_F16
-_TARGET_BITS = {"torch.int64": 64, "torch.int32": 32}
+_target_bits = {}  # torch.dtype -> bits
 _type_of = {}  # torch.dtype -> code, filled on first use (a dtype's text costs more to make than to look up)
 
 
@@ -31,13 +31,20 @@ def _code(t, name):
     return _type_of[d]
 
 
+_torch_module = None
+
+
 def _torch():
-    import torch
-    if not _native.shares_torch_runtime:
+    global _torch_module
+    if _torch_module is None:
+        import torch
         _native.lib()
         if not _native.shares_torch_runtime:
             raise _native.PstError("import torch before pst_amd loads libpst: the two hold different HIP runtimes")
-    return torch
+        _torch_module = torch
+        for bits in (32, 64):
+            _target_bits[getattr(torch, f"int{bits}")] = bits
+    return _torch_module
 
 
 def _check(rc):
@@ -51,12 +58,10 @@ def _device(t, name):
     return t.device
 
 
-def _matrix(t, name, device=None, shape=None):
+def _matrix(t, name, device=None):
     """(pointer, row stride) of a matrix with unit column stride."""
     if t.dim() != 2:
         raise ValueError(f"{name} has {t.dim()} dimensions: 2 are needed")
-    if shape is not None and tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name} has shape {tuple(t.shape)}: {tuple(shape)} is needed")
     if device is not None and t.device != device:
         raise ValueError(f"{name} is on {t.device}: {device} is needed")
     rows, cols = t.shape
@@ -88,14 +93,14 @@ def _workspace_bytes(fn, *key):
 
 
 def _workspace(torch, device, fn, ctype, x, ldx, w, ldw, rows, vocab, width):
+    """A call's workspace (torch's allocations are aligned to 512 bytes) and its size."""
     # a pointer counts by its alignment alone
     n = _workspace_bytes(fn, ctype, 256 + (x & 15), ldx, 256 + (w & 15), ldw, rows, vocab, width)
-    ws = torch.empty(n + 256, dtype=torch.uint8, device=device)
-    return ws, (ws.data_ptr() + 255) & ~255, n
+    return torch.empty(n, dtype=torch.uint8, device=device), n
 
 
 def _stream(torch, device):
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)  # torch.cuda.current_stream without the object
 
 
 def _head(torch, hidden, weight):
@@ -113,7 +118,7 @@ def _head(torch, hidden, weight):
 
 
 def _targets(targets, rows, device):
-    bits = _TARGET_BITS.get(str(targets.dtype))
+    bits = _target_bits.get(targets.dtype)
     if bits is None:
         raise ValueError(f"targets are {targets.dtype}: int64 or int32 is needed")
     return _vector(targets, "targets", rows, device), bits
@@ -130,12 +135,12 @@ def token_loss(hidden, weight, targets, *, ignore_index=-100):
     rows, width = hidden.shape
     vocab = weight.shape[0]
     t, bits = _targets(targets, rows, device)
-    out = torch.empty((2, rows), dtype=torch.float32, device=device)
-    loss, lse = out[0], out[1]
+    loss = torch.empty(rows, dtype=torch.float32, device=device)
+    lse = torch.empty(rows, dtype=torch.float32, device=device)
     if rows:
-        ws, wp, wn = _workspace(torch, device, "pst_token_loss_workspace", code, x, ldx, w, ldw, rows, vocab, width)
+        ws, wn = _workspace(torch, device, "pst_token_loss_workspace", code, x, ldx, w, ldw, rows, vocab, width)
         _check(_native.lib().pst_token_loss(device.index, code, x, ldx, w, ldw, rows, vocab, width, t, bits, ignore_index,
-                                            loss.data_ptr(), lse.data_ptr(), wp, wn, _stream(torch, device)))
+                                            loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), wn, _stream(torch, device)))
     return loss, lse
 
 
@@ -155,10 +160,10 @@ def token_loss_grad(hidden, weight, targets, lse, grad_loss, *, ignore_index=-10
     dx = torch.empty((rows, width), dtype=hidden.dtype, device=device) if need_hidden else None
     dw = torch.empty((vocab, width), dtype=weight.dtype, device=device) if need_weight else None
     if dw is not None or (dx is not None and rows):
-        ws, wp, wn = _workspace(torch, device, "pst_token_loss_grad_workspace", code, x, ldx, w, ldw, rows, vocab, width)
+        ws, wn = _workspace(torch, device, "pst_token_loss_grad_workspace", code, x, ldx, w, ldw, rows, vocab, width)
         _check(_native.lib().pst_token_loss_grad(
             device.index, code, x, ldx, w, ldw, rows, vocab, width, t, bits, ignore_index, sp, gp,
-            dx.data_ptr() if dx is not None else None, width, dw.data_ptr() if dw is not None else None, width, wp, wn,
+            dx.data_ptr() if dx is not None else None, width, dw.data_ptr() if dw is not None else None, width, ws.data_ptr(), wn,
             _stream(torch, device)))
     return dx, dw
 
@@ -205,7 +210,7 @@ def token_scores_int8(hidden, qweight, scale, *, out_dtype=None):
     out_code = _code(held, "out_dtype")
     out = held[:, :vocab]
     if rows:
-        ws, wp, wn = _workspace(torch, device, "pst_token_scores_i8_workspace", code, x, ldx, w, ldw, rows, vocab, width)
+        ws, wn = _workspace(torch, device, "pst_token_scores_i8_workspace", code, x, ldx, w, ldw, rows, vocab, width)
         _check(_native.lib().pst_token_scores_i8(device.index, code, x, ldx, w, ldw, sp, rows, vocab, width, out_code,
-                                                 out.data_ptr(), ldo, wp, wn, _stream(torch, device)))
+                                                 out.data_ptr(), ldo, ws.data_ptr(), wn, _stream(torch, device)))
     return out
