@@ -26,15 +26,14 @@ namespace {
 
 // Tiles of the products. A remainder of up to 64 vocabulary rows behind the 256-row tiles (the marks behind a codebook of
 // 4096 or 64000), or of positions, goes to thin tiles of the same launch instead of a round of nearly empty ones.
-struct T256 : Tile<256, 256, 2, 4> {
+struct T256 : Tile<256, 256, 2, 4, 2> {
   static constexpr bool HAS_THIN = true;
-  struct Thin : Tile<64, 256, 2, 4> {};   // along m
-  struct ThinN : Tile<256, 64, 4, 2> {};  // along n
+  struct Thin : Tile<64, 64, 2, 4, 4> {};
 };
-struct T128 : Tile<128, 128, 2, 2> {
+struct T128 : Tile<128, 128, 2, 2, 2> {
   static constexpr bool HAS_THIN = false;
 };
-struct T64 : Tile<64, 64, 2, 2> {
+struct T64 : Tile<64, 64, 2, 2, 2> {
   static constexpr bool HAS_THIN = false;
 };
 
@@ -126,6 +125,20 @@ __global__ __launch_bounds__(1024) void k_amax(AmaxArgs a) {
   }
 }
 
+// The pieces of a matrix's rows over workgroups of 256 threads, without a division: a power of two of threads, at most 64,
+// takes a row.
+struct Spread {
+  int64_t row, rows;  // this thread's first row, and how far its next is
+  int piece, pieces;  // the same of the pieces within a row
+  __device__ __forceinline__ Spread(int block, int blocks, int per_row) {
+    const int shift = per_row >= 64 ? 6 : per_row <= 1 ? 0 : 32 - __builtin_clz(per_row - 1);
+    row = ((int64_t)block * 256 + threadIdx.x) >> shift;
+    rows = ((int64_t)blocks * 256) >> shift;
+    pieces = 1 << shift;
+    piece = threadIdx.x & (pieces - 1);
+  }
+};
+
 // A matrix copied into rows of whole K-steps with zeros behind, 32-bit values split into two planes
 struct PackJob {
   const void* src;         // null: nothing to do
@@ -182,11 +195,10 @@ __global__ __launch_bounds__(256) void k_pack(PackArgs a) {
     e = split_exp(block_max(p.part[threadIdx.x], sm));
     if (block == 0 && threadIdx.x == 0) *p.unscale = ldexpf(1.0f, -e);
   }
-  const int by = p.wide ? 8 : 2, per = a.width_pad / by;  // neighbours a thread takes
-  const int64_t groups = p.rows_pad * per;
-  for (int64_t g = block * (int64_t)256 + threadIdx.x; g < groups; g += (int64_t)a.blocks[which] * 256) {
-    const int64_t r = g / per;
-    const int c = (int)(g - r * per) * by;
+  const int by = p.wide ? 8 : 2;  // neighbours a thread takes
+  const Spread at_row(block, a.blocks[which], a.width_pad / by);
+  for (int64_t r = at_row.row; r < p.rows_pad; r += at_row.rows)
+  for (int c = at_row.piece * by; c < a.width_pad; c += at_row.pieces * by) {
     bool keep = r < p.rows;
     if (keep && p.zero_rows) (void)target_of(a.targets, r, keep);
     char* d = p.dst + (r * a.width_pad + c) * 2;
@@ -243,7 +255,8 @@ struct GemmArgs {
   KLoop k;
   int32_t M, N;        // rows of A and of B that exist
   int32_t nm, nn, nz;  // tiles along m and n, parts of the K loop
-  int32_t blocks;      // workgroups that share the nm nn tiles; those behind them take the thin tiles of the last rows
+  int32_t blocks;      // workgroups that share the nm nn tiles; those behind them take the `thins` thin tiles of the last rows
+  int32_t thins;
   int32_t steps;       // K-steps of the whole range
   int32_t gm;
   // unscaling of 32-bit operands (device; null: 1)
@@ -332,15 +345,15 @@ __device__ __forceinline__ float* epilogue_lds(char* smem) {
 }
 constexpr int EPILOGUE_LDS = 4096;
 
-// A workgroup's tiles: tile, tile + stride, ... of the nm nn tiles of type T. The next tile's loads fly during the
+// A workgroup's tiles: tile, tile + stride, ... of the nm x nn of type T from row m_base. The next tile's loads fly during the
 // epilogue of the last; what the epilogue needs from memory is loaded during the K loop (column and row of this thread),
 // since waiting for a load is waiting for all that were started before it.
 template <int E, class T, bool MANY, class Epilogue>
-__device__ __forceinline__ void tiles(const GemmArgs& g, int tile, int stride, int nm, int m_base, char* smem, Epilogue epilogue) {
+__device__ __forceinline__ void tiles(const GemmArgs& g, int tile, int stride, int nm, int nn, int m_base, char* smem, Epilogue epilogue) {
   Loop<E, T, false, false> loop(smem);
-  const int total = nm * g.nn;
+  const int total = nm * nn;
   if (tile >= total) return;
-  Place<T> p(g, tile, nm, g.nn, m_base, 0);
+  Place<T> p(g, tile, nm, nn, m_base, 0);
   loop.begin(g.A, g.B, g.k, p.m0, p.n0, 0, g.steps);
   for (;;) {
     typename Mma<E>::Acc acc[T::MI][T::NI];
@@ -351,7 +364,7 @@ __device__ __forceinline__ void tiles(const GemmArgs& g, int tile, int stride, i
     tile += stride;
     const bool more = MANY && tile < total;
     if (more) {
-      p = Place<T>(g, tile, nm, g.nn, m_base, 0);
+      p = Place<T>(g, tile, nm, nn, m_base, 0);
       loop.begin(g.A, g.B, g.k, p.m0, p.n0, 0, g.steps);
     }
     met();
@@ -444,9 +457,9 @@ template <int E, class T>
 __global__ __launch_bounds__(T::THREADS, 2) void k_loss(GemmArgs g) {
   extern __shared__ char smem[];
   if ((int)blockIdx.x < g.blocks) {
-    tiles<E, T, true>(g, blockIdx.x, g.blocks, g.nm, 0, smem, LossEpilogue{});
+    tiles<E, T, true>(g, blockIdx.x, g.blocks, g.nm, g.nn, 0, smem, LossEpilogue{});
   } else if constexpr (T::HAS_THIN) {
-    tiles<E, typename T::Thin, false>(g, blockIdx.x - g.blocks, 1 << 30, 1, g.nm * T::BM, smem, LossEpilogue{});
+    tiles<E, typename T::Thin, false>(g, blockIdx.x - g.blocks, 1 << 30, 1, g.thins, g.nm * T::BM, smem, LossEpilogue{});
   }
 }
 
@@ -578,9 +591,9 @@ template <int E, class T>
 __global__ __launch_bounds__(T::THREADS, 2) void k_dlogit(GemmArgs g) {
   extern __shared__ char smem[];
   if ((int)blockIdx.x < g.blocks) {
-    tiles<E, T, true>(g, blockIdx.x, g.blocks, g.nm, 0, smem, DlogitEpilogue<E>{});
+    tiles<E, T, true>(g, blockIdx.x, g.blocks, g.nm, g.nn, 0, smem, DlogitEpilogue<E>{});
   } else if constexpr (T::HAS_THIN) {
-    tiles<E, typename T::Thin, false>(g, blockIdx.x - g.blocks, 1 << 30, 1, g.nm * T::BM, smem, DlogitEpilogue<E>{});
+    tiles<E, typename T::Thin, false>(g, blockIdx.x - g.blocks, 1 << 30, 1, g.thins, g.nm * T::BM, smem, DlogitEpilogue<E>{});
   }
 }
 
@@ -632,12 +645,10 @@ __global__ __launch_bounds__(256) void k_finish(FinishArgs a) {
   const int which = (int)blockIdx.x < a.blocks[0] ? 0 : 1;
   const int block = (int)blockIdx.x - (which ? a.blocks[0] : 0);
   const FinishJob& f = a.job[which];
-  const int per = (a.width + 3) / 4;
-  const int64_t total = f.rows * per;
+  const Spread at_row(block, a.blocks[which], (a.width + 3) / 4);
   const float mul = (f.u0 ? *f.u0 : 1.0f) * (f.u1 ? *f.u1 : 1.0f);
-  for (int64_t g = block * (int64_t)256 + threadIdx.x; g < total; g += (int64_t)a.blocks[which] * 256) {
-    const int64_t n = g / per;
-    const int c = (int)(g - n * per) * 4;
+  for (int64_t n = at_row.row; n < f.rows; n += at_row.rows)
+  for (int c = at_row.piece * 4; c < a.width; c += at_row.pieces * 4) {
     f32x4 s = {0, 0, 0, 0};
 #pragma unroll 4
     for (int z = 0; z < f.nz; ++z) {
@@ -705,8 +716,8 @@ __device__ __forceinline__ void store_rows(const f32x4 (&acc)[T::MI][T::NI], con
 // dx's parts (m = column, n = position, k = vocabulary row of the piece, its K loop in nz parts) and rows v0 ... of dW
 // (m = column, n = vocabulary row, k = position; in one part straight to the output, or in parts as dx).
 template <int E, class T, bool DX>
-__device__ __forceinline__ void grad_tile(const GemmArgs& g, int tile, int nn, int n_base, char* smem) {
-  const Place<T> p(g, tile, g.nm, nn, 0, n_base);
+__device__ __forceinline__ void grad_tile(const GemmArgs& g, int tile, int nm, int nn, int n_base, char* smem) {
+  const Place<T> p(g, tile, nm, nn, 0, n_base);
   const int s0 = (int)((int64_t)g.steps * p.z / g.nz), s1 = (int)((int64_t)g.steps * (p.z + 1) / g.nz);
   f32x4 acc[T::MI][T::NI];
   Loop<E, T, true, !DX> loop(smem);
@@ -724,13 +735,13 @@ template <int E, class T>
 __global__ __launch_bounds__(T::THREADS, 2) void k_grads(GradArgs g) {
   extern __shared__ char smem[];
   int b = blockIdx.x;
-  if (b < g.blocks[0]) return grad_tile<E, T, true>(g.dx, b, g.dx.nn, 0, smem);
+  if (b < g.blocks[0]) return grad_tile<E, T, true>(g.dx, b, g.dx.nm, g.dx.nn, 0, smem);
   b -= g.blocks[0];
-  if (b < g.blocks[1]) return grad_tile<E, T, false>(g.dw, b, g.dw.nn, 0, smem);
+  if (b < g.blocks[1]) return grad_tile<E, T, false>(g.dw, b, g.dw.nm, g.dw.nn, 0, smem);
   if constexpr (T::HAS_THIN) {
     b -= g.blocks[1];
-    if (b < g.blocks[2]) return grad_tile<E, typename T::ThinN, true>(g.dx, b, 1, g.dx.nn * T::BN, smem);
-    grad_tile<E, typename T::ThinN, false>(g.dw, b - g.blocks[2], 1, g.dw.nn * T::BN, smem);
+    if (b < g.blocks[2]) return grad_tile<E, typename T::Thin, true>(g.dx, b, g.dx.thins, 1, g.dx.nn * T::BN, smem);
+    grad_tile<E, typename T::Thin, false>(g.dw, b - g.blocks[2], g.dw.thins, 1, g.dw.nn * T::BN, smem);
   }
 }
 
@@ -771,9 +782,9 @@ template <class T>
 __global__ __launch_bounds__(T::THREADS, 2) void k_scores(GemmArgs g) {
   extern __shared__ char smem[];
   if ((int)blockIdx.x < g.blocks) {
-    tiles<I8, T, true>(g, blockIdx.x, g.blocks, g.nm, 0, smem, ScoresEpilogue{});
+    tiles<I8, T, true>(g, blockIdx.x, g.blocks, g.nm, g.nn, 0, smem, ScoresEpilogue{});
   } else if constexpr (T::HAS_THIN) {
-    tiles<I8, typename T::Thin, false>(g, blockIdx.x - g.blocks, 1 << 30, 1, g.nm * T::BM, smem, ScoresEpilogue{});
+    tiles<I8, typename T::Thin, false>(g, blockIdx.x - g.blocks, 1 << 30, 1, g.thins, g.nm * T::BM, smem, ScoresEpilogue{});
   }
 }
 
@@ -941,13 +952,17 @@ enum TileId { TILE64 = 0, TILE128 = 1, TILE256 = 2 };
 constexpr int TILE_M[3] = {64, 128, 256};
 
 // ---- the choice of tiles
-// Times of a workgroup in us, fitted to single launches on the card (d = 128 ... 1024, 16 ... 8192 positions): a launch's
-// tiles run in rounds of `slots`, and a tile costs BASE + PER_STEP * K-steps when its compute unit is full.
-//   256: 1 a unit, 1.5 us a K-step of 64 (all of them 1.4 PFLOP/s);  128: 2 a unit, 1.1;  64: 4 a unit, 0.85
+// Times of a workgroup in us, fitted to single launches on the card (d = 128 ... 1024, 16 ... 8192 positions): BASE and, for
+// each K-step of 64, STEP + MORE for each workgroup that shares the compute unit, up to `slots` of them. The largest
+// tiles reach 1.3 PFLOP/s, those of 128 about 0.95, those of 64 about 0.65; the smaller ones fill the card sooner.
 constexpr int CUS = 256;  // the card's compute units, whatever device is asked: a workspace's size needs none
-constexpr double TILE_BASE[3] = {2.0, 3.0, 4.0}, TILE_STEP[3] = {0.85, 1.1, 1.5};
+constexpr double TILE_BASE[3] = {2.0, 3.0, 4.0}, TILE_STEP[3] = {0.45, 0.55, 1.5}, TILE_MORE[3] = {0.1, 0.27, 0.0};
 constexpr int TILE_SLOTS[3] = {4, 2, 1};
-double tile_us(int tile, int64_t steps) { return TILE_BASE[tile] + TILE_STEP[tile] * steps; }
+constexpr double THIN = 0.35;  // a thin tile's time
+double tile_us(int tile, double tiles, int64_t steps) {
+  const double share = std::min<double>(TILE_SLOTS[tile], std::max(1.0, tiles / CUS));
+  return TILE_BASE[tile] + (TILE_STEP[tile] + TILE_MORE[tile] * share) * steps;
+}
 int64_t tiles_of(int64_t m, int64_t n, int tile) { return ceil_div(m, TILE_M[tile]) * ceil_div(n, TILE_M[tile]); }
 // rows that thin tiles take
 int64_t thin_rows(int64_t m, int tile) {
@@ -960,9 +975,9 @@ int tile_for(int64_t m, int64_t n, int64_t steps) {
   double us = 1e30;
   for (int t = TILE256; t >= TILE64; --t) {
     const int64_t thin = thin_rows(m, t), slots = (int64_t)CUS * TILE_SLOTS[t], full = tiles_of(m - thin, n, t);
-    double e = ceil_div(full, slots) * tile_us(t, steps);
-    // thin tiles take what the last round leaves free, or about half a round
-    if (thin && tiles_of(m, n, t) > ceil_div(full, slots) * slots) e += 0.5 * tile_us(t, steps);
+    const double one = tile_us(t, full, steps);
+    double e = ceil_div(full, slots) * one;
+    if (thin && full + ceil_div(n, 64) > ceil_div(full, slots) * slots) e += THIN * one;  // not into what the last round leaves free
     if (e < us) us = e, best = t;
   }
   return best;
@@ -1005,7 +1020,8 @@ hipError_t launch_gemm(int kind, int elem, int tile, GemmArgs g, hipStream_t st)
   const int64_t tiles = (int64_t)g.nm * g.nn;
   if (tiles > 0x3fffffff) return hipErrorInvalidConfiguration;
   g.blocks = (int32_t)std::min<int64_t>(tiles, (int64_t)CUS * TILE_SLOTS[tile]);
-  const int64_t grid = g.blocks + (thin ? g.nn : 0);
+  g.thins = (int32_t)ceil_div(g.N, 64);
+  const int64_t grid = g.blocks + (thin ? g.thins : 0);
   return elem == I8     ? launch_elem<I8>(kind, tile, g, grid, st)
          : elem == BF16 ? launch_elem<BF16>(kind, tile, g, grid, st)
                         : launch_elem<F16>(kind, tile, g, grid, st);
@@ -1023,7 +1039,8 @@ hipError_t launch_grads(int elem, int tile, GradArgs g, bool dx, bool dw, hipStr
     const int64_t thin = thin_rows(q.N, tile);
     set_tiles(q, i ? q.M : q.ldp, q.N - thin, tile);
     const bool on = i ? dw : dx;
-    const int64_t blocks = on ? (int64_t)q.nm * q.nn * q.nz : 0, thins = on && thin ? (int64_t)q.nm * q.nz : 0;
+    q.thins = (int32_t)ceil_div(i ? q.M : q.ldp, 64);
+    const int64_t blocks = on ? (int64_t)q.nm * q.nn * q.nz : 0, thins = on && thin ? (int64_t)q.thins * q.nz : 0;
     grid += blocks + thins;
     if (grid > 0x7fffffff) return hipErrorInvalidConfiguration;
     g.blocks[i] = (int32_t)blocks;
@@ -1075,6 +1092,48 @@ Plan plan_loss(int type, const void* x, int64_t ldx, const void* w, int64_t ldw,
   p.bytes = b.n;
   return p;
 }
+// The tiles of the two gradients' launch and the parts zx, zw of their K loops: the least of the estimated launch and of
+// the parts' way back through memory (4.5 TB/s). The last choice is kept, by the sizes alone.
+void split_grads(Plan& p, int64_t nv, bool pieces) {
+  struct Last {
+    int64_t rows = -1, nv, width;
+    int planes, tile, zx, zw;
+    bool pieces;
+  };
+  thread_local Last last;
+  if (last.rows != p.rows || last.nv != nv || last.width != p.width || last.planes != p.planes || last.pieces != pieces) {
+    constexpr int Z[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
+    const int passes = p.planes == 2 ? 3 : 1;
+    const int64_t sx = ceil_div(nv, 64) * passes, sw = ceil_div(p.rows, 64) * passes;
+    double best = 1e30;
+    for (int t = TILE256; t >= TILE64; --t) {
+      const int64_t thin_x = thin_rows(p.rows, t), thin_w = thin_rows(nv, t);
+      const double slots = (double)CUS * TILE_SLOTS[t];
+      const double one_x = tiles_of(p.width_pad, p.rows - thin_x, t), one_w = tiles_of(p.width, nv - thin_w, t);
+      const double thins_x = thin_x ? ceil_div(p.width_pad, 64) : 0, thins_w = thin_w ? ceil_div(p.width, 64) : 0;
+      for (int zx : Z)
+        for (int zw : Z) {
+          if ((zx > 1 && sx < 4 * zx) || (zw > 1 && (pieces || sw < 4 * zw))) continue;
+          const double n = one_x * zx + one_w * zw, thins = thins_x * zx + thins_w * zw;
+          const double tx = tile_us(t, n, ceil_div(sx, zx)), tw = tile_us(t, n, ceil_div(sw, zw)), longest = std::max(tx, tw);
+          double us = longest;
+          // both kinds share the slots; the last to start ends half its time behind the rest
+          if (n > slots) us = std::max((one_x * zx * tx + one_w * zw * tw) / slots + 0.5 * longest, longest + std::min(tx, tw));
+          if (n + thins > ceil_div((int64_t)n, (int64_t)slots) * slots) us += THIN * longest;
+          us += 4.0 * p.width_pad * (p.rows * (double)zx + (zw > 1 ? nv * (double)zw : 0.0)) / 4.5e6 + 0.1 * (zx + zw);
+          if (us < best) best = us, last.tile = t, last.zx = zx, last.zw = zw;
+        }
+    }
+    last.rows = p.rows;
+    last.nv = nv;
+    last.width = p.width;
+    last.planes = p.planes;
+    last.pieces = pieces;
+  }
+  p.tile = last.tile;
+  p.zx = last.zx;
+  p.zw = last.zw;
+}
 // bytes of D that a piece of the vocabulary may take: about what the last-level cache (256 MB) holds
 constexpr int64_t PIECE_BYTES = 288ll << 20;
 Plan plan_grad(int type, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab, int64_t width) {
@@ -1088,27 +1147,7 @@ Plan plan_grad(int type, const void* x, int64_t ldx, const void* w, int64_t ldw,
   if (vocab > most && round > 0 && most >= round) most = most / round * round;
   p.piece = vocab > most ? most : up(vocab, 256);
   p.D = b.take(drows * p.piece * 2 * p.planes);
-  // tiles and parts of the K loops: the least of the estimated launch and of the parts' way through memory (4 TB/s)
-  const int64_t nv = std::min(p.piece, vocab);
-  const int passes = p.planes == 2 ? 3 : 1;
-  double best = 1e30;
-  for (int t = TILE256; t >= TILE64; --t)
-    for (int zx = 1; zx <= 16; zx *= 2)
-      for (int zw = 1; zw <= (vocab > p.piece ? 1 : 16); zw *= 2) {
-        const int64_t sx = ceil_div(nv, 64) * passes, sw = ceil_div(rows, 64) * passes;
-        if ((zx > 1 && sx < 4 * zx) || (zw > 1 && sw < 4 * zw)) continue;
-        // both kinds share the slots; the last to start ends half its time behind the rest
-        const double tx = tile_us(t, ceil_div(sx, zx)), tw = tile_us(t, ceil_div(sw, zw)), longest = std::max(tx, tw);
-        const int64_t thin_x = thin_rows(rows, t), thin_w = thin_rows(nv, t);
-        const double nx = (double)tiles_of(p.width_pad, rows - thin_x, t) * zx, nw = (double)tiles_of(width, nv - thin_w, t) * zw;
-        const double thins = 0.5 * ((thin_x ? tiles_of(p.width_pad, 1, t) * zx * tx : 0) + (thin_w ? tiles_of(width, 1, t) * zw * tw : 0));
-        const double slots = (double)CUS * TILE_SLOTS[t];
-        double us = (nx * tx + nw * tw + thins) / slots;
-        us = nx + nw <= slots ? longest + (thins > 0 && nx + nw + thins / longest > slots ? 0.5 * longest : 0) : std::max(us + 0.5 * longest, longest);
-        const double bytes = 8.0 * p.width_pad * (rows * (double)zx + (zw > 1 ? vocab * (double)zw : 0.0));
-        const double e = us * ceil_div(vocab, p.piece) + bytes / 4e6 + 0.2 * (zx + zw);
-        if (e < best) best = e, p.tile = t, p.zx = zx, p.zw = zw;
-      }
+  split_grads(p, std::min(p.piece, vocab), vocab > p.piece);
   p.dxp = b.take(p.zx * rows * p.width_pad * 4);
   if (p.zw > 1) p.dwp = b.take(p.zw * vocab * p.width_pad * 4);
   p.bytes = b.n;

@@ -190,17 +190,17 @@ struct Reader {
   }
 };
 
-template <int BM_, int BN_, int WM_, int WN_>
+template <int BM_, int BN_, int WM_, int WN_, int STAGES_>
 struct Tile {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NW = WM_ * WN_, THREADS = NW * 64;
   static constexpr int MI = BM_ / WM_ / 16, NI = BN_ / WN_ / 16;  // a wave's 16x16 blocks
-  static constexpr int STAGE = (BM_ + BN_) * STEP, LDS = 2 * STAGE;  // (an epilogue's own LDS lies behind)
+  static constexpr int STAGES = STAGES_, STAGE = (BM_ + BN_) * STEP, LDS = STAGES * STAGE;  // (an epilogue's own LDS lies behind)
 };
 
-// The K loop of one tile after another: begin() starts the loads of a tile's first two K-steps, run() leaves the tile's
-// sums in acc[MI][NI] of this wave. Between them a workgroup can store the tile before.
-// Two LDS stages: the loads of K-step t + 2 start when all waves have read the last of step t, and fly while t + 1 is
-// multiplied. A K-step is four parts, (k half, half of the wave's rows): each part's fragments are read from LDS while
+// The K loop of one tile after another: begin() starts the loads of a tile's first K-steps, run() leaves the tile's sums in
+// acc[MI][NI] of this wave. Between them a workgroup can store the tile before.
+// A ring of S LDS stages: the loads of K-step t + S start when all waves have read the last of step t, and fly while the
+// steps between are multiplied. 256-row tiles have room for two; a smaller tile's step is shorter than a load's way. A K-step is four parts, (k half, half of the wave's rows): each part's fragments are read from LDS while
 // the part before is multiplied, also across the one barrier of a K-step.
 // Measured at 8192 x 16128 x 1024 bf16 (216 us as it is): K-steps of 64 bytes in rings of 3, 4 and 5 stages 226 - 228 (twice
 // the barriers; deeper prefetch gains nothing), two 256 x 128 workgroups a unit 252 (half as much again through LDS),
@@ -210,8 +210,9 @@ struct Loop {
   typedef typename Mma<E>::Acc Acc;
   static constexpr int HI = T::MI / 2;
   // blocks of a wave start at a multiple of their number, so that a COLS read can xor the block into its address
-  static_assert((T::MI & (T::MI - 1)) == 0 && (T::NI & (T::NI - 1)) == 0 && T::MI >= 2 && T::NI >= 2, "wave tile");
-  static constexpr int LA = Stager<T::BM, ACOLS, T::NW>::NI, LB = Stager<T::BN, BCOLS, T::NW>::NI;
+  static_assert((T::MI & (T::MI - 1)) == 0 && (T::NI & (T::NI - 1)) == 0 && T::MI >= 2, "wave tile");
+  static constexpr int S = T::STAGES, LA = Stager<T::BM, ACOLS, T::NW>::NI, LB = Stager<T::BN, BCOLS, T::NW>::NI, L = LA + LB;
+  static_assert((S & (S - 1)) == 0 && S >= 2, "ring of stages");
   Stager<T::BM, ACOLS, T::NW> sa;
   Stager<T::BN, BCOLS, T::NW> sb;
   Reader<T::BM, ACOLS> ra;
@@ -245,7 +246,7 @@ struct Loop {
   __device__ __forceinline__ void issue(int stage) {
     aim(stage);
 #pragma unroll
-    for (int i = 0; i < LA + LB; ++i) load(i);
+    for (int i = 0; i < L; ++i) load(i);
   }
   // K-steps [from, to) of each pass; all waves have left the stages
   __device__ __forceinline__ void begin(const Operand& A, const Operand& B, const KLoop& k, int m0, int n0, int from, int to) {
@@ -258,8 +259,33 @@ struct Loop {
     step1 = to;
     seg = 0;
     total = (to - from) * k.segs;
-    if (total > 0) issue(0);
-    if (total > 1) issue(1);
+    for (int t = 0; t < min(S, total); ++t) issue(t);
+  }
+
+  // at most `steps` K-steps' loads are in flight behind this
+  template <int MOST = S - 1>
+  __device__ __forceinline__ void landed_but_steps(int steps) const {
+    if constexpr (MOST == 0) {
+      landed_but<0>();
+    } else {
+      if (steps >= MOST) return landed_but<MOST * L>();
+      landed_but_steps<MOST - 1>(steps);
+    }
+  }
+  __device__ __forceinline__ void clear(Acc (&acc)[T::MI][T::NI]) {
+#pragma unroll
+    for (int i = 0; i < T::MI; ++i)
+#pragma unroll
+      for (int j = 0; j < T::NI; ++j) acc[i][j] = {0, 0, 0, 0};
+  }
+  // the loads of a K-step between `count` multiplications, behind the q-th: the unit that takes them accepts one in 16
+  // clocks of the whole workgroup, and a wave behind it would wait with idle matrix cores
+  template <int COUNT>
+  __device__ __forceinline__ void load_behind(int q) const {
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int l = q * L / COUNT; l < (q + 1) * L / COUNT; ++l) load(l);
+    __builtin_amdgcn_sched_barrier(0);
   }
 
   i32x4 a[2][HI], b[2][T::NI];
@@ -275,59 +301,55 @@ struct Loop {
     }
     __builtin_amdgcn_sched_barrier(0);
   }
-  // multiplies part p; MORE: with the loads of a K-step spread between the multiplications, since the unit that takes them
-  // accepts one in 16 clocks of the whole workgroup and a wave behind it would wait with idle matrix cores
+  // multiplies part p; MORE: with the loads of a K-step
   template <bool MORE>
   __device__ __forceinline__ void mult(Acc (&acc)[T::MI][T::NI], int p) {
-    constexpr int TOTAL = HI * T::NI;
+    constexpr int COUNT = HI * T::NI;
 #pragma unroll
-    for (int q = 0; q < TOTAL; ++q) {
+    for (int q = 0; q < COUNT; ++q) {
       const int i = q / T::NI, j = q % T::NI;
       acc[(p & 1) * HI + i][j] = Mma<E>::mma(a[p & 1][i], b[p >> 1][j], acc[(p & 1) * HI + i][j]);
-      if constexpr (MORE) {
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int l = q * (LA + LB) / TOTAL; l < (q + 1) * (LA + LB) / TOTAL; ++l) load(l);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+      if constexpr (MORE) load_behind<COUNT>(q);
     }
     __builtin_amdgcn_sched_barrier(0);
   }
-  // one K-step; MORE: another one is loaded into its stage, NEXT: another one follows
-  template <bool MORE, bool NEXT>
-  __device__ __forceinline__ void body(Acc (&acc)[T::MI][T::NI], int t) {
-    fetch(t & 1, 1);
+  // the first three parts of K-step t, and the fragments of its last
+  __device__ __forceinline__ void most(Acc (&acc)[T::MI][T::NI], int t) {
+    const int stage = t & (S - 1);
+    fetch(stage, 1);
     mult<false>(acc, 0);
-    fetch(t & 1, 2);
+    fetch(stage, 2);
     mult<false>(acc, 1);
-    fetch(t & 1, 3);
+    fetch(stage, 3);
     mult<false>(acc, 2);
-    // the last fragments of step t are in registers: its stage is free once all waves are here
-    if constexpr (NEXT) {
-      landed_but<0>();
-      fetch((t + 1) & 1, 0);
-    }
-    if constexpr (MORE) aim(t & 1);
-    mult<MORE>(acc, 3);
   }
+
   __device__ __forceinline__ void run(Acc (&acc)[T::MI][T::NI]) {
-#pragma unroll
-    for (int i = 0; i < T::MI; ++i)
-#pragma unroll
-      for (int j = 0; j < T::NI; ++j) acc[i][j] = {0, 0, 0, 0};
+    clear(acc);
+    int t = 0;
+    // (what this wave stored since begin() counts as loads in flight do, so the first wait may be for some of it)
     if (total > 0) {
-      // (what this wave stored since begin() counts as loads in flight do, so this may wait for some of it)
-      if (total > 1) {
-        landed_but<LA + LB>();
-      } else {
-        landed_but<0>();
-      }
+      landed_but_steps(min(S, total) - 1);
       fetch(0, 0);
     }
-    int t = 0;
-    for (; t + 2 < total; ++t) body<true, true>(acc, t);
-    if (t + 1 < total) body<false, true>(acc, t++);
-    if (t < total) body<false, false>(acc, t);
+    for (; t + S < total; ++t) {
+      most(acc, t);
+      // the last fragments of step t are in registers: its stage is free once all waves are here
+      landed_but<(S - 2) * L>();
+      fetch((t + 1) & (S - 1), 0);
+      aim(t & (S - 1));
+      mult<true>(acc, 3);
+    }
+    for (; t + 1 < total; ++t) {
+      most(acc, t);
+      landed_but_steps(total - t - 2);
+      fetch((t + 1) & (S - 1), 0);
+      mult<false>(acc, 3);
+    }
+    if (t < total) {
+      most(acc, t);
+      mult<false>(acc, 3);
+    }
     landed_but<0>();  // the stages are free
   }
 };
