@@ -9,8 +9,7 @@
 // in a workspace that the last-level cache holds, and multiplies it in both directions from there.
 //
 // 32-bit inputs: each value is split into two 16-bit floats (hi + lo, 22 bits of mantissa) after a scaling of
-// the whole tensor by a power of two, and a product is the three passes lo hi + hi lo + hi hi on the 16-bit
-// matrix cores: about 2^-22 of the operands' product, at three sixteenths of the 32-bit instructions' time.
+// the whole tensor by a power of two, and a product is lo hi + hi lo + hi hi on the 16-bit matrix cores: about 2^-22 of the operands' product, at three sixteenths of the 32-bit instructions' time.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -24,17 +23,26 @@
 namespace pst_head {
 namespace {
 
-// Tiles of the products. A remainder of up to 64 vocabulary rows behind the 256-row tiles (the marks behind a codebook of
-// 4096 or 64000), or of positions, goes to thin tiles of the same launch instead of a round of nearly empty ones.
+// Tiles of the products. A remainder of up to 64 vocabulary rows (the marks behind a codebook of 4096 or 64000) or
+// positions behind the whole tiles goes to thin tiles of the same launch instead of a round of nearly empty ones.
+struct T64 : Tile<64, 64, 2, 2, 2> {
+  static constexpr bool HAS_THIN = false;
+};
+struct T128 : Tile<128, 128, 2, 2, 2> {
+  static constexpr bool HAS_THIN = true;
+  typedef T64 Thin;
+};
 struct T256 : Tile<256, 256, 2, 4, 2> {
   static constexpr bool HAS_THIN = true;
   struct Thin : Tile<64, 64, 2, 4, 4> {};
 };
-struct T128 : Tile<128, 128, 2, 2, 2> {
+// of split 32-bit values: a K-step brings both planes of both operands, and three products are made of them
+struct S64 : Tile<64, 64, 2, 2, 2, 2> {
   static constexpr bool HAS_THIN = false;
 };
-struct T64 : Tile<64, 64, 2, 2, 2> {
-  static constexpr bool HAS_THIN = false;
+struct S128 : Tile<128, 128, 2, 2, 2, 2> {
+  static constexpr bool HAS_THIN = true;
+  typedef S64 Thin;
 };
 
 constexpr float LOG2E = 1.44269504088896340736f;
@@ -252,7 +260,6 @@ __global__ __launch_bounds__(256) void k_pack(PackArgs a) {
 // ------------------------------------------------------------------ products with their epilogues
 struct GemmArgs {
   Operand A, B;
-  KLoop k;
   int32_t M, N;        // rows of A and of B that exist
   int32_t nm, nn, nz;  // tiles along m and n, parts of the K loop
   int32_t blocks;      // workgroups that share the nm nn tiles; those behind them take the `thins` thin tiles of the last rows
@@ -269,7 +276,7 @@ struct GemmArgs {
   const float* gscale; // power of two on D (device; null: 1)
   char* D;             // [planes][rows][ldd] 16-bit
   int64_t dplane, ldd; // bytes, elements
-  int32_t dplanes, v0;
+  int32_t v0;
   // matrix outputs
   void* out;
   int64_t ldo;
@@ -354,7 +361,7 @@ __device__ __forceinline__ void tiles(const GemmArgs& g, int tile, int stride, i
   const int total = nm * nn;
   if (tile >= total) return;
   Place<T> p(g, tile, nm, nn, m_base, 0);
-  loop.begin(g.A, g.B, g.k, p.m0, p.n0, 0, g.steps);
+  loop.begin(g.A, g.B, p.m0, p.n0, 0, g.steps);
   for (;;) {
     typename Mma<E>::Acc acc[T::MI][T::NI];
     auto inputs = epilogue.load(g, p);
@@ -365,7 +372,7 @@ __device__ __forceinline__ void tiles(const GemmArgs& g, int tile, int stride, i
     const bool more = MANY && tile < total;
     if (more) {
       p = Place<T>(g, tile, nm, nn, m_base, 0);
-      loop.begin(g.A, g.B, g.k, p.m0, p.n0, 0, g.steps);
+      loop.begin(g.A, g.B, p.m0, p.n0, 0, g.steps);
     }
     met();
     epilogue.template store<T>(g, done, acc, epilogue_lds<T>(smem));
@@ -389,7 +396,7 @@ struct LossEpilogue {
   }
   template <class T>
   __device__ __forceinline__ void store(const GemmArgs& g, const Place<T>& p, f32x4 (&acc)[T::MI][T::NI], float* lds) const {
-    if (g.ua) unscale<T>(acc, *g.ua * *g.ub);
+    if (T::PLANES == 2) unscale<T>(acc, *g.ua * *g.ub);
     if (p.mwave + T::MI * 16 > g.M) {  // rows behind the vocabulary's last
 #pragma unroll
       for (int i = 0; i < T::MI; ++i)
@@ -530,7 +537,7 @@ struct DlogitEpilogue {
   }
   template <class T>
   __device__ __forceinline__ void store(const GemmArgs& g, const Place<T>& p, f32x4 (&acc)[T::MI][T::NI], float* lds) const {
-    if (g.ua) unscale<T>(acc, *g.ua * *g.ub);
+    if (T::PLANES == 2) unscale<T>(acc, *g.ua * *g.ub);
     const bool edge = p.mwave + T::MI * 16 > g.M;
 #pragma unroll
     for (int j = 0; j < T::NI; ++j) {
@@ -575,7 +582,7 @@ struct DlogitEpilogue {
 #pragma unroll
           for (int q = 0; q < 2; ++q) w[u][q] = pack2(acc[i + u][j][2 * q], acc[i + u][j][2 * q + 1], TYPE);
         store_pair(to + i * 32, w, p.lane);
-        if (E == F16 && g.dplanes == 2) {
+        if (T::PLANES == 2) {
 #pragma unroll
           for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -721,7 +728,7 @@ __device__ __forceinline__ void grad_tile(const GemmArgs& g, int tile, int nm, i
   const int s0 = (int)((int64_t)g.steps * p.z / g.nz), s1 = (int)((int64_t)g.steps * (p.z + 1) / g.nz);
   f32x4 acc[T::MI][T::NI];
   Loop<E, T, true, !DX> loop(smem);
-  loop.begin(g.A, g.B, g.k, p.m0, p.n0, s0, s1);
+  loop.begin(g.A, g.B, p.m0, p.n0, s0, s1);
   loop.run(acc);
   if (DX || g.part_out) {
     store_part<T>(acc, g, p);
@@ -948,17 +955,18 @@ bool in_place(const void* p, int64_t ld_bytes, int64_t row_bytes) {
   return ((uintptr_t)p & 15) == 0 && ld_bytes % 16 == 0 && row_bytes % 16 == 0;
 }
 
-enum TileId { TILE64 = 0, TILE128 = 1, TILE256 = 2 };
-constexpr int TILE_M[3] = {64, 128, 256};
+enum TileId { TILE64 = 0, TILE128 = 1, TILE256 = 2, SPLIT64 = 3, SPLIT128 = 4 };
+constexpr int TILE_M[5] = {64, 128, 256, 64, 128};
 
 // ---- the choice of tiles
 // Times of a workgroup in us, fitted to single launches on the card (d = 128 ... 1024, 16 ... 8192 positions): BASE and, for
 // each K-step of 64, STEP + MORE for each workgroup that shares the compute unit, up to `slots` of them. The largest
-// tiles reach 1.3 PFLOP/s, those of 128 about 0.95, those of 64 about 0.65; the smaller ones fill the card sooner.
+// tiles reach 1.3 PFLOP/s, those of 128 about 0.95, those of 64 about 0.65; the smaller ones fill the card sooner. The two
+// of split values make three products a step.
 constexpr int CUS = 256;  // the card's compute units, whatever device is asked: a workspace's size needs none
-constexpr double TILE_BASE[3] = {2.0, 3.0, 4.0}, TILE_STEP[3] = {0.45, 0.55, 1.5}, TILE_MORE[3] = {0.1, 0.27, 0.0};
-constexpr int TILE_SLOTS[3] = {4, 2, 1};
-constexpr double THIN = 0.35;  // a thin tile's time
+constexpr double TILE_BASE[5] = {2.0, 3.0, 4.0, 2.5, 4.0}, TILE_STEP[5] = {0.45, 0.55, 1.5, 0.5, 1.0}, TILE_MORE[5] = {0.1, 0.27, 0.0, 0.2, 0.0};
+constexpr int TILE_SLOTS[5] = {4, 2, 1, 2, 1};
+constexpr double THIN[5] = {0.0, 0.6, 0.35, 0.0, 0.6};  // a thin tile's time, of a whole one's
 double tile_us(int tile, double tiles, int64_t steps) {
   const double share = std::min<double>(TILE_SLOTS[tile], std::max(1.0, tiles / CUS));
   return TILE_BASE[tile] + (TILE_STEP[tile] + TILE_MORE[tile] * share) * steps;
@@ -966,18 +974,18 @@ double tile_us(int tile, double tiles, int64_t steps) {
 int64_t tiles_of(int64_t m, int64_t n, int tile) { return ceil_div(m, TILE_M[tile]) * ceil_div(n, TILE_M[tile]); }
 // rows that thin tiles take
 int64_t thin_rows(int64_t m, int tile) {
-  const int64_t rest = m % TILE_M[TILE256];
-  return tile == TILE256 && m > rest && rest <= 64 ? rest : 0;
+  const int64_t rest = m % TILE_M[tile];
+  return THIN[tile] > 0 && m > rest && rest <= 64 ? rest : 0;
 }
 // m x n of the loss, the logits' gradient and the scores
-int tile_for(int64_t m, int64_t n, int64_t steps) {
+int tile_for(int64_t m, int64_t n, int64_t steps, int planes = 1) {
   int best = TILE64;
   double us = 1e30;
-  for (int t = TILE256; t >= TILE64; --t) {
+  for (int t = planes == 2 ? SPLIT128 : TILE256; t >= (planes == 2 ? SPLIT64 : TILE64); --t) {
     const int64_t thin = thin_rows(m, t), slots = (int64_t)CUS * TILE_SLOTS[t], full = tiles_of(m - thin, n, t);
     const double one = tile_us(t, full, steps);
     double e = ceil_div(full, slots) * one;
-    if (thin && full + ceil_div(n, 64) > ceil_div(full, slots) * slots) e += THIN * one;  // not into what the last round leaves free
+    if (thin && full + ceil_div(n, 64) > ceil_div(full, slots) * slots) e += THIN[t] * one;  // not into what the last round leaves free
     if (e < us) us = e, best = t;
   }
   return best;
@@ -1010,6 +1018,10 @@ void set_tiles(GemmArgs& g, int64_t m, int64_t n, int tile) {
 }
 template <int E>
 hipError_t launch_elem(int kind, int tile, const GemmArgs& g, int64_t grid, hipStream_t st) {
+  if constexpr (E == F16) {
+    if (tile == SPLIT128) return launch_kind<E, S128>(kind, g, grid, st);
+    if (tile == SPLIT64) return launch_kind<E, S64>(kind, g, grid, st);
+  }
   return tile == TILE256   ? launch_kind<E, T256>(kind, g, grid, st)
          : tile == TILE128 ? launch_kind<E, T128>(kind, g, grid, st)
                            : launch_kind<E, T64>(kind, g, grid, st);
@@ -1028,6 +1040,10 @@ hipError_t launch_gemm(int kind, int elem, int tile, GemmArgs g, hipStream_t st)
 }
 template <int E>
 hipError_t launch_grads_elem(int tile, const GradArgs& g, int64_t grid, hipStream_t st) {
+  if constexpr (E == F16) {
+    if (tile == SPLIT128) return launch(k_grads<E, S128>, grid, S128::THREADS, S128::LDS, st, g);
+    if (tile == SPLIT64) return launch(k_grads<E, S64>, grid, S64::THREADS, S64::LDS, st, g);
+  }
   return tile == TILE256   ? launch(k_grads<E, T256>, grid, T256::THREADS, T256::LDS, st, g)
          : tile == TILE128 ? launch(k_grads<E, T128>, grid, T128::THREADS, T128::LDS, st, g)
                            : launch(k_grads<E, T64>, grid, T64::THREADS, T64::LDS, st, g);
@@ -1086,7 +1102,7 @@ Plan plan_common(int type, const void* x, int64_t ldx, const void* w, int64_t ld
 Plan plan_loss(int type, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab, int64_t width) {
   Bump b;
   Plan p = plan_common(type, x, ldx, w, ldw, rows, vocab, width, false, b);
-  p.tile = tile_for(vocab, rows, p.width_pad / 64 * (p.planes == 2 ? 3 : 1));
+  p.tile = tile_for(vocab, rows, p.width_pad / 64, p.planes);
   p.part = b.take(ceil_div(vocab, TILE_M[p.tile]) * rows * 8);
   p.tlogit = b.take(rows * 4);
   p.bytes = b.n;
@@ -1103,24 +1119,23 @@ void split_grads(Plan& p, int64_t nv, bool pieces) {
   thread_local Last last;
   if (last.rows != p.rows || last.nv != nv || last.width != p.width || last.planes != p.planes || last.pieces != pieces) {
     constexpr int Z[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
-    const int passes = p.planes == 2 ? 3 : 1;
-    const int64_t sx = ceil_div(nv, 64) * passes, sw = ceil_div(p.rows, 64) * passes;
+    const int64_t sx = ceil_div(nv, 64), sw = ceil_div(p.rows, 64), least = p.planes == 2 ? 2 : 4;
     double best = 1e30;
-    for (int t = TILE256; t >= TILE64; --t) {
+    for (int t = p.planes == 2 ? SPLIT128 : TILE256; t >= (p.planes == 2 ? SPLIT64 : TILE64); --t) {
       const int64_t thin_x = thin_rows(p.rows, t), thin_w = thin_rows(nv, t);
       const double slots = (double)CUS * TILE_SLOTS[t];
       const double one_x = tiles_of(p.width_pad, p.rows - thin_x, t), one_w = tiles_of(p.width, nv - thin_w, t);
       const double thins_x = thin_x ? ceil_div(p.width_pad, 64) : 0, thins_w = thin_w ? ceil_div(p.width, 64) : 0;
       for (int zx : Z)
         for (int zw : Z) {
-          if ((zx > 1 && sx < 4 * zx) || (zw > 1 && (pieces || sw < 4 * zw))) continue;
+          if ((zx > 1 && sx < least * zx) || (zw > 1 && (pieces || sw < least * zw))) continue;
           const double n = one_x * zx + one_w * zw, thins = thins_x * zx + thins_w * zw;
           const double tx = tile_us(t, n, ceil_div(sx, zx)), tw = tile_us(t, n, ceil_div(sw, zw)), longest = std::max(tx, tw);
           double us = longest;
           // both kinds share the slots; the last to start ends half its time behind the rest
           if (n > slots) us = std::max((one_x * zx * tx + one_w * zw * tw) / slots + 0.5 * longest, longest + std::min(tx, tw));
-          if (n + thins > ceil_div((int64_t)n, (int64_t)slots) * slots) us += THIN * longest;
-          us += 4.0 * p.width_pad * (p.rows * (double)zx + (zw > 1 ? nv * (double)zw : 0.0)) / 4.5e6 + 0.1 * (zx + zw);
+          if (n + thins > ceil_div((int64_t)n, (int64_t)slots) * slots) us += THIN[t] * longest;
+          us += 4.0 * p.width_pad * (p.rows * (double)zx + (zw > 1 ? nv * (double)zw : 0.0)) / 4.5e6 + 0.3 * (zx + zw);
           if (us < best) best = us, last.tile = t, last.zx = zx, last.zw = zw;
         }
     }
@@ -1134,14 +1149,15 @@ void split_grads(Plan& p, int64_t nv, bool pieces) {
   p.zx = last.zx;
   p.zw = last.zw;
 }
-// bytes of D that a piece of the vocabulary may take: about what the last-level cache (256 MB) holds
-constexpr int64_t PIECE_BYTES = 288ll << 20;
+// Vocabulary rows of a piece: D takes about what the last-level cache (256 MB) holds, but a piece has 4096 rows at least,
+// since each adds to all of dx's sums in memory.
+constexpr int64_t PIECE_BYTES = 288ll << 20, PIECE_LEAST = 4096;
 Plan plan_grad(int type, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab, int64_t width) {
   Bump b;
   Plan p = plan_common(type, x, ldx, w, ldw, rows, vocab, width, true, b);
   p.gscale = b.take(8);
   const int64_t drows = up(rows, 256);
-  int64_t most = std::max<int64_t>(256, PIECE_BYTES / (drows * 2 * p.planes) / 256 * 256);
+  int64_t most = std::max<int64_t>(PIECE_LEAST, PIECE_BYTES / (drows * 2 * p.planes) / 256 * 256);
   // several pieces: of a size that gives dW's largest tiles in whole rounds, where that is not much smaller
   const int64_t round = CUS / std::max<int64_t>(1, ceil_div(p.width_pad, 256)) * 256;
   if (vocab > most && round > 0 && most >= round) most = most / round * round;
@@ -1216,9 +1232,6 @@ int operands(const Plan& p, const void* x, int64_t ldx, const void* w, int64_t l
   return PST_OK;
 }
 
-// the passes of a product of split operands, the small terms first: (lo, hi), (hi, lo), (hi, hi)
-KLoop passes(int planes) { return planes == 2 ? KLoop{3, 0x01, 0x04} : KLoop{1, 0, 0}; }
-
 int token_loss(int device, int type, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab, int64_t width,
                const void* targets, int tbits, int64_t ignore, float* loss, float* lse, void* ws_, int64_t ws_bytes, hipStream_t st) {
   int rc = check_sizes(type, x, ldx, w, ldw, rows, vocab, width);
@@ -1236,7 +1249,6 @@ int token_loss(int device, int type, const void* x, int64_t ldx, const void* w, 
   g.targets = {targets, ignore, tbits, (int32_t)vocab};
   rc = operands(p, x, ldx, w, ldw, g.targets, nullptr, ws, st, &g.B, &g.A);
   if (rc != PST_OK) return rc;
-  g.k = passes(p.planes);
   g.M = (int32_t)vocab;
   g.N = (int32_t)rows;
   g.steps = (int32_t)(p.width_pad / 64);
@@ -1293,8 +1305,7 @@ int token_loss_grad(int device, int type, const void* x, int64_t ldx, const void
     Wv.p += v0 * W.ld;
     Wv.rows = (int32_t)nv;
     GemmArgs g{};
-    g.k = passes(p.planes);
-    g.A = Wv;
+      g.A = Wv;
     g.B = X;
     g.M = (int32_t)nv;
     g.N = (int32_t)rows;
@@ -1308,11 +1319,9 @@ int token_loss_grad(int device, int type, const void* x, int64_t ldx, const void
     g.D = D;
     g.dplane = dop.plane;
     g.ldd = ldd;
-    g.dplanes = p.planes;
     g.v0 = (int32_t)v0;
-    if (rows) HEADCHK(launch_gemm(DLOGIT, p.elem, tile_for(nv, rows, g.steps * (p.planes == 2 ? 3 : 1)), g, st));
+    if (rows) HEADCHK(launch_gemm(DLOGIT, p.elem, tile_for(nv, rows, g.steps, p.planes), g, st));
     GradArgs b{};
-    b.dx.k = b.dw.k = g.k;
     b.dx.A = Wv;
     b.dx.B = b.dw.B = dop;
     b.dx.M = b.dw.M = (int32_t)width;
@@ -1425,7 +1434,6 @@ int token_scores_i8(int device, int type, const void* x, int64_t ldx, const int8
   char* ws = (char*)ws_;
   HEADCHK(launch_quantize({x, ldx, p.width_pad, rows, (int32_t)width, (int32_t)p.width_pad, type, (int8_t*)(ws + p.q), (float*)(ws + p.scale), 0, 0}, st));
   GemmArgs g{};
-  g.k = passes(1);
   if (p.pack_w) {
     hipLaunchKernelGGL(k_pack8, dim3(copy_grid(vocab * (p.width_pad / 16))), dim3(256), 0, st, w, ldw, vocab, (int32_t)width, (int32_t)p.width_pad,
                        (int8_t*)(ws + p.w));

@@ -61,21 +61,14 @@ struct Mma<I8> {
 };
 
 // One operand in memory. ROWS: `rows` rows of `bytes` valid bytes (a multiple of 16). COLS: `rows` k-rows of
-// `bytes` valid bytes. ld in bytes, a multiple of 16 (and p 16-byte aligned). Plane q (a 32-bit float split
-// into 16-bit ones has two) starts at p + q * plane.
+// `bytes` valid bytes. ld in bytes, a multiple of 16 (and p 16-byte aligned). Split 32-bit floats have two planes of
+// 16-bit ones, hi at p and lo at p + plane.
 struct Operand {
   const char* p;
   int64_t plane;
   int64_t ld;
   int32_t rows;
   int32_t bytes;
-};
-
-// The product's K loop: `segs` passes over the same k range with the operands' planes seg_a / seg_b (2 bits a
-// pass), K-steps [step0, step1) of each.
-struct KLoop {
-  int32_t segs;
-  uint32_t seg_a, seg_b;
 };
 
 constexpr int STEP = 128;  // bytes of k in a K-step
@@ -115,15 +108,18 @@ struct Stager {
   static constexpr int PER = 1024 / RT;            // LDS rows an instruction fills
   static_assert(NI >= 1 && NI * NW * 1024 == R * STEP, "tile and waves do not fit");
   uint32_t off[NI];
-  const char* base;  // of the current plane's tile
+  const char* base;  // of the tile
   int32_t k_bytes;   // ROWS: valid bytes of a row; COLS: valid k-rows
   int64_t ld;
+  int64_t plane;
   const char* src;   // the K-step being loaded, what is valid of it, and where it goes
-  int32_t left = 1 << 30;
+  int32_t left;
   uint32_t to;
 
   __device__ __forceinline__ void init(const Operand& o, int row0, int lane, int wave) {
     ld = o.ld;
+    plane = o.plane;
+    left = 1 << 30;
     // a tile behind the last row (a column of zeros in the output) reads the last one
     const int first = COLS ? min(row0 * 2, o.bytes - 16) : min(row0, o.rows - 1);
     base = o.p + (COLS ? (int64_t)first : (int64_t)first * o.ld);
@@ -140,26 +136,27 @@ struct Stager {
       }
     }
   }
-  // K-step `step` of plane `plane_off` goes to the LDS tile at `lds`, by one(0) ... one(NI - 1)
-  __device__ __forceinline__ void aim(int64_t plane_off, int step, uint32_t lds, int lane, int wave) {
+  // K-step `step` goes to the LDS tile at `lds` (its lo plane to the tile behind), by one(0) ... one(NI - 1) a plane
+  __device__ __forceinline__ void aim(int step, uint32_t lds, int lane, int wave) {
     constexpr int WHOLE = COLS ? 64 : STEP;
-    if (left < WHOLE) shift(left, 1, lane, wave);  // a pass behind the first: undo the last K-step's
-    src = base + plane_off + (COLS ? (int64_t)min(step * 64, k_bytes - 1) * ld : (int64_t)step * STEP);
+    src = base + (COLS ? (int64_t)min(step * 64, k_bytes - 1) * ld : (int64_t)step * STEP);
     left = COLS ? k_bytes - step * 64 : k_bytes - step * STEP;
-    if (left < WHOLE) shift(left, -1, lane, wave);
+    if (left < WHOLE) shift(left, lane, wave);  // the last step of all
     to = __builtin_amdgcn_readfirstlane(lds + (uint32_t)wave * (NI * 1024));
   }
   // a K-step of which `valid` (k-rows or bytes) exist: what lies behind reads the last of them
-  __device__ __forceinline__ void shift(int valid, int sign, int lane, int wave) {
+  __device__ __forceinline__ void shift(int valid, int lane, int wave) {
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
       const int r = (wave * NI + j) * PER + lane / (RT / 16);
       const int c = lane % (RT / 16);
-      const uint32_t d = COLS ? (uint32_t)((int64_t)max(0, r - max(0, valid - 1)) * ld) : (uint32_t)max(0, ((c ^ (r >> 1 & 7)) << 4) - (valid - 16));
-      off[j] += sign > 0 ? d : 0u - d;
+      off[j] -= COLS ? (uint32_t)((int64_t)max(0, r - max(0, valid - 1)) * ld) : (uint32_t)max(0, ((c ^ (r >> 1 & 7)) << 4) - (valid - 16));
     }
   }
-  __device__ __forceinline__ void one(int j) const { load_lds(src, off[j], to + j * 1024); }
+  __device__ __forceinline__ void one(int j) const {
+    const int q = j / NI, i = j % NI;
+    load_lds(q ? src + plane : src, off[i], to + q * (R * STEP) + i * 1024);
+  }
 };
 
 // Fragments of one wave, 16 rows x 64 bytes of k each: block b (from block blk0 of the tile), half s of the K-step
@@ -190,11 +187,11 @@ struct Reader {
   }
 };
 
-template <int BM_, int BN_, int WM_, int WN_, int STAGES_>
+template <int BM_, int BN_, int WM_, int WN_, int STAGES_, int PLANES_ = 1>
 struct Tile {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NW = WM_ * WN_, THREADS = NW * 64;
   static constexpr int MI = BM_ / WM_ / 16, NI = BN_ / WN_ / 16;  // a wave's 16x16 blocks
-  static constexpr int STAGES = STAGES_, STAGE = (BM_ + BN_) * STEP, LDS = STAGES * STAGE;  // (an epilogue's own LDS lies behind)
+  static constexpr int STAGES = STAGES_, PLANES = PLANES_, STAGE = (BM_ + BN_) * STEP * PLANES_, LDS = STAGES * STAGE;  // (an epilogue's own LDS lies behind)
 };
 
 // The K loop of one tile after another: begin() starts the loads of a tile's first K-steps, run() leaves the tile's sums in
@@ -211,7 +208,8 @@ struct Loop {
   static constexpr int HI = T::MI / 2;
   // blocks of a wave start at a multiple of their number, so that a COLS read can xor the block into its address
   static_assert((T::MI & (T::MI - 1)) == 0 && (T::NI & (T::NI - 1)) == 0 && T::MI >= 2, "wave tile");
-  static constexpr int S = T::STAGES, LA = Stager<T::BM, ACOLS, T::NW>::NI, LB = Stager<T::BN, BCOLS, T::NW>::NI, L = LA + LB;
+  static constexpr int S = T::STAGES, PL = T::PLANES;
+  static constexpr int LA = Stager<T::BM, ACOLS, T::NW>::NI * PL, LB = Stager<T::BN, BCOLS, T::NW>::NI * PL, L = LA + LB;
   static_assert((S & (S - 1)) == 0 && S >= 2, "ring of stages");
   Stager<T::BM, ACOLS, T::NW> sa;
   Stager<T::BN, BCOLS, T::NW> sb;
@@ -220,9 +218,7 @@ struct Loop {
   const char* smem;
   uint32_t lds0;
   int lane, wave;
-  int64_t plane_a, plane_b;
-  KLoop kl;
-  int step0, step1, total, seg, step;  // seg, step: what is loaded next
+  int step, total;  // step: what is loaded next
 
   __device__ __forceinline__ explicit Loop(const char* smem_) : smem(smem_), lds0(lds_addr(smem_)) {
     lane = threadIdx.x & 63;
@@ -232,12 +228,9 @@ struct Loop {
   }
   __device__ __forceinline__ void aim(int stage) {
     const uint32_t to = lds0 + stage * T::STAGE;
-    sa.aim((int64_t)((kl.seg_a >> (2 * seg)) & 3) * plane_a, step, to, lane, wave);
-    sb.aim((int64_t)((kl.seg_b >> (2 * seg)) & 3) * plane_b, step, to + T::BM * STEP, lane, wave);
-    if (++step == step1) {
-      step = step0;
-      ++seg;
-    }
+    sa.aim(step, to, lane, wave);
+    sb.aim(step, to + T::BM * STEP * PL, lane, wave);
+    ++step;
   }
   __device__ __forceinline__ void load(int i) const {
     if (i < LA) sa.one(i);
@@ -248,17 +241,12 @@ struct Loop {
 #pragma unroll
     for (int i = 0; i < L; ++i) load(i);
   }
-  // K-steps [from, to) of each pass; all waves have left the stages
-  __device__ __forceinline__ void begin(const Operand& A, const Operand& B, const KLoop& k, int m0, int n0, int from, int to) {
+  // K-steps [from, to); all waves have left the stages
+  __device__ __forceinline__ void begin(const Operand& A, const Operand& B, int m0, int n0, int from, int to) {
     sa.init(A, m0, lane, wave);
     sb.init(B, n0, lane, wave);
-    plane_a = A.plane;
-    plane_b = B.plane;
-    kl = k;
-    step0 = step = from;
-    step1 = to;
-    seg = 0;
-    total = (to - from) * k.segs;
+    step = from;
+    total = to - from;
     for (int t = 0; t < min(S, total); ++t) issue(t);
   }
 
@@ -288,27 +276,32 @@ struct Loop {
     __builtin_amdgcn_sched_barrier(0);
   }
 
-  i32x4 a[2][HI], b[2][T::NI];
+  i32x4 a[2][PL][HI], b[2][PL][T::NI];
   // fragments of part p of the K-step in `stage`
   __device__ __forceinline__ void fetch(int stage, int p) {
     const char* ta = smem + stage * T::STAGE;
-    const char* tb = ta + T::BM * STEP;
+    const char* tb = ta + T::BM * STEP * PL;
 #pragma unroll
-    for (int i = 0; i < HI; ++i) a[p & 1][i] = ra.get(ta, (p & 1) * HI + i, p >> 1);
-    if ((p & 1) == 0) {
+    for (int q = 0; q < PL; ++q) {
 #pragma unroll
-      for (int j = 0; j < T::NI; ++j) b[p >> 1][j] = rb.get(tb, j, p >> 1);
+      for (int i = 0; i < HI; ++i) a[p & 1][q][i] = ra.get(ta + q * (T::BM * STEP), (p & 1) * HI + i, p >> 1);
+      if ((p & 1) == 0) {
+#pragma unroll
+        for (int j = 0; j < T::NI; ++j) b[p >> 1][q][j] = rb.get(tb + q * (T::BN * STEP), j, p >> 1);
+      }
     }
     __builtin_amdgcn_sched_barrier(0);
   }
-  // multiplies part p; MORE: with the loads of a K-step
+  // multiplies part p; MORE: with the loads of a K-step. Of split values the three products that count, the small ones
+  // first: lo hi + hi lo + hi hi.
   template <bool MORE>
   __device__ __forceinline__ void mult(Acc (&acc)[T::MI][T::NI], int p) {
-    constexpr int COUNT = HI * T::NI;
+    constexpr int ONE = HI * T::NI, COUNT = ONE * (PL == 2 ? 3 : 1);
 #pragma unroll
     for (int q = 0; q < COUNT; ++q) {
-      const int i = q / T::NI, j = q % T::NI;
-      acc[(p & 1) * HI + i][j] = Mma<E>::mma(a[p & 1][i], b[p >> 1][j], acc[(p & 1) * HI + i][j]);
+      const int i = q % ONE / T::NI, j = q % T::NI, c = q / ONE;
+      const int qa = PL == 2 && c == 0, qb = PL == 2 && c == 1;
+      acc[(p & 1) * HI + i][j] = Mma<E>::mma(a[p & 1][qa][i], b[p >> 1][qb][j], acc[(p & 1) * HI + i][j]);
       if constexpr (MORE) load_behind<COUNT>(q);
     }
     __builtin_amdgcn_sched_barrier(0);

@@ -69,7 +69,7 @@ def _matrix(t, name, device=None):
     if cols > 1 and s1 != 1:
         raise ValueError(f"{name} has a column stride of {s1}: 1 is needed")
     if rows <= 1:
-        s0 = max(s0, cols)
+        s0 = cols
     elif s0 < cols:
         raise ValueError(f"{name} has overlapping rows (row stride {s0} of {cols} columns)")
     return t.data_ptr(), s0

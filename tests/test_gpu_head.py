@@ -113,6 +113,23 @@ def test_several_pieces_of_the_vocabulary():
     check_grad(x, w, t, gl)
 
 
+def test_pieces_for_many_positions():
+    x, w, t, gl = make(40000, 9000, 32, torch.bfloat16, seed=3)
+    check_grad(x, w, t, gl)
+
+
+# whole tiles of 256 and 128 with a few rows, columns or positions behind them, and just past what thin tiles take
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("rows,vocab,width", [(2049, 4097, 64), (2112, 4160, 72), (2113, 4161, 64), (1090, 1795, 520)])
+def test_remainders(rows, vocab, width, dtype):
+    x, w, t, gl = make(rows, vocab, width, dtype, seed=7)
+    t[:4] = torch.arange(vocab - 4, vocab, device=DEV)
+    _, lse = check_loss(x, w, t)
+    check_grad(x, w, t, gl, lse)
+    q, s = head.quantize_rows(w)
+    assert torch.equal(head.token_scores_int8(x, q, s, out_dtype=torch.float32), defined_scores(x, q, s, torch.float32))
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("pad,wpad", [(8, 16), (1, 0), (0, 3), (24, 1)])
 def test_strides(pad, wpad, dtype):
@@ -140,6 +157,13 @@ def test_rows_far_apart():
     q, s = head.quantize_rows(w)
     far = held.view(torch.int8).as_strided((1100, 64), (1 << 22, 1)).copy_(q)
     assert torch.equal(head.token_scores_int8(x, far, s), head.token_scores_int8(x, q, s))
+
+
+def test_one_row_of_a_wide_buffer():
+    held = torch.randn(2, 1 << 22, device=DEV).bfloat16()
+    x, w, t, gl = make(1, 20, 64, torch.bfloat16, ignored=0)
+    check_loss(held[:1, :64], w, t)
+    check_grad(held[1:, :64], w, t, gl)
 
 
 def test_int32_targets_and_another_ignored_value():
@@ -343,10 +367,10 @@ def step(x, w, t, gl, q, s):
 
 
 def test_captured_and_replayed():
-    """Two graphs and eager calls of other sizes between their replays: each has its own workspace."""
+    """Graphs and eager calls of other sizes between their replays: each has its own workspace."""
     sets, graphs, outs = [], [], []
-    for k, (rows, vocab) in enumerate(((100, 700), (64, 1500))):
-        x, w, t, gl = make(rows, vocab, 136, (torch.float32, torch.bfloat16)[k], seed=k)
+    for k, (rows, vocab) in enumerate(((100, 700), (64, 1500), (2048, 8200), (1100, 4099))):
+        x, w, t, gl = make(rows, vocab, 136, (torch.float32, torch.bfloat16, torch.bfloat16, torch.float32)[k], seed=k)
         sets.append((x, w, t, gl) + head.quantize_rows(w))
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
