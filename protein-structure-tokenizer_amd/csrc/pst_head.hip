@@ -40,9 +40,9 @@ struct T256 : Tile<256, 256, 2, 4, 2> {
 struct S64 : Tile<64, 64, 2, 2, 2, 2> {
   static constexpr bool HAS_THIN = false;
 };
-struct S128 : Tile<128, 128, 2, 2, 2, 2> {
+struct S128 : Tile<128, 128, 2, 4, 2, 2> {
   static constexpr bool HAS_THIN = true;
-  typedef S64 Thin;
+  struct Thin : Tile<64, 64, 2, 4, 2, 2> {};
 };
 
 constexpr float LOG2E = 1.44269504088896340736f;
@@ -461,7 +461,7 @@ struct LossEpilogue {
 };
 
 template <int E, class T>
-__global__ __launch_bounds__(T::THREADS, 2) void k_loss(GemmArgs g) {
+__global__ __launch_bounds__(T::THREADS, T::WAVES) void k_loss(GemmArgs g) {
   extern __shared__ char smem[];
   if ((int)blockIdx.x < g.blocks) {
     tiles<E, T, true>(g, blockIdx.x, g.blocks, g.nm, g.nn, 0, smem, LossEpilogue{});
@@ -595,7 +595,7 @@ struct DlogitEpilogue {
 };
 
 template <int E, class T>
-__global__ __launch_bounds__(T::THREADS, 2) void k_dlogit(GemmArgs g) {
+__global__ __launch_bounds__(T::THREADS, T::WAVES) void k_dlogit(GemmArgs g) {
   extern __shared__ char smem[];
   if ((int)blockIdx.x < g.blocks) {
     tiles<E, T, true>(g, blockIdx.x, g.blocks, g.nm, g.nn, 0, smem, DlogitEpilogue<E>{});
@@ -739,7 +739,7 @@ __device__ __forceinline__ void grad_tile(const GemmArgs& g, int tile, int nm, i
 }
 // workgroups: dx's tiles, dW's, then the thin ones of dx and of dW
 template <int E, class T>
-__global__ __launch_bounds__(T::THREADS, 2) void k_grads(GradArgs g) {
+__global__ __launch_bounds__(T::THREADS, T::WAVES) void k_grads(GradArgs g) {
   extern __shared__ char smem[];
   int b = blockIdx.x;
   if (b < g.blocks[0]) return grad_tile<E, T, true>(g.dx, b, g.dx.nm, g.dx.nn, 0, smem);
@@ -786,7 +786,7 @@ struct ScoresEpilogue {
   }
 };
 template <class T>
-__global__ __launch_bounds__(T::THREADS, 2) void k_scores(GemmArgs g) {
+__global__ __launch_bounds__(T::THREADS, T::WAVES) void k_scores(GemmArgs g) {
   extern __shared__ char smem[];
   if ((int)blockIdx.x < g.blocks) {
     tiles<I8, T, true>(g, blockIdx.x, g.blocks, g.nm, g.nn, 0, smem, ScoresEpilogue{});
@@ -964,9 +964,9 @@ constexpr int TILE_M[5] = {64, 128, 256, 64, 128};
 // tiles reach 1.3 PFLOP/s, those of 128 about 0.95, those of 64 about 0.65; the smaller ones fill the card sooner. The two
 // of split values make three products a step.
 constexpr int CUS = 256;  // the card's compute units, whatever device is asked: a workspace's size needs none
-constexpr double TILE_BASE[5] = {2.0, 3.0, 4.0, 2.5, 4.0}, TILE_STEP[5] = {0.45, 0.55, 1.5, 0.5, 1.0}, TILE_MORE[5] = {0.1, 0.27, 0.0, 0.2, 0.0};
+constexpr double TILE_BASE[5] = {2.0, 3.0, 4.0, 2.5, 4.0}, TILE_STEP[5] = {0.45, 0.55, 1.5, 0.3, 1.1}, TILE_MORE[5] = {0.1, 0.27, 0.0, 0.28, 0.0};
 constexpr int TILE_SLOTS[5] = {4, 2, 1, 2, 1};
-constexpr double THIN[5] = {0.0, 0.6, 0.35, 0.0, 0.6};  // a thin tile's time, of a whole one's
+constexpr double THIN[5] = {0.0, 0.6, 0.35, 0.0, 0.5};  // a thin tile's time, of a whole one's
 double tile_us(int tile, double tiles, int64_t steps) {
   const double share = std::min<double>(TILE_SLOTS[tile], std::max(1.0, tiles / CUS));
   return TILE_BASE[tile] + (TILE_STEP[tile] + TILE_MORE[tile] * share) * steps;

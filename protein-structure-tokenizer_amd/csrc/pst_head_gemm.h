@@ -191,6 +191,7 @@ template <int BM_, int BN_, int WM_, int WN_, int STAGES_, int PLANES_ = 1>
 struct Tile {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NW = WM_ * WN_, THREADS = NW * 64;
   static constexpr int MI = BM_ / WM_ / 16, NI = BN_ / WN_ / 16;  // a wave's 16x16 blocks
+  static constexpr int WAVES = 2;  // on each SIMD at least: what a workgroup's registers leave room for
   static constexpr int STAGES = STAGES_, PLANES = PLANES_, STAGE = (BM_ + BN_) * STEP * PLANES_, LDS = STAGES * STAGE;  // (an epilogue's own LDS lies behind)
 };
 
