@@ -886,18 +886,17 @@ __global__ __launch_bounds__(256) void k_quantize(QuantArgs a) {
     }
   }
 }
-// 8-bit rows into whole K-steps
+// 8-bit rows into whole K-steps, four neighbours a thread
 __global__ __launch_bounds__(256) void k_pack8(const int8_t* src, int64_t ld, int64_t rows, int32_t width, int32_t width_pad, int8_t* dst) {
-  const int per = width_pad / 16;
-  const int64_t total = rows * per;
-  for (int64_t g = blockIdx.x * (int64_t)256 + threadIdx.x; g < total; g += (int64_t)gridDim.x * 256) {
-    const int64_t r = g / per;
-    const int c = (int)(g - r * per) * 16;
-    int8_t v[16];
+  const Spread at_row(blockIdx.x, gridDim.x, width_pad / 4);
+  for (int64_t r = at_row.row; r < rows; r += at_row.rows)
+    for (int c = at_row.piece * 4; c < width_pad; c += at_row.pieces * 4) {
+      uint32_t v = 0;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = c + j < width ? src[r * ld + c + j] : (int8_t)0;
-    *(uint4*)(dst + r * width_pad + c) = __builtin_bit_cast(uint4, *(i32x4*)v);
-  }
+      for (int j = 0; j < 4; ++j)
+        if (c + j < width) v |= (uint32_t)(uint8_t)src[r * ld + c + j] << (8 * j);
+      *(uint32_t*)(dst + r * width_pad + c) = v;
+    }
 }
 
 // ------------------------------------------------------------------ host
@@ -977,13 +976,14 @@ int64_t thin_rows(int64_t m, int tile) {
   const int64_t rest = m % TILE_M[tile];
   return THIN[tile] > 0 && m > rest && rest <= 64 ? rest : 0;
 }
-// m x n of the loss, the logits' gradient and the scores
-int tile_for(int64_t m, int64_t n, int64_t steps, int planes = 1) {
+// m x n of the loss, the logits' gradient and the scores; a compute unit stores about 20 KB in a us (5 TB/s of all)
+int tile_for(int64_t m, int64_t n, int64_t steps, int planes, int out_bytes) {
   int best = TILE64;
   double us = 1e30;
   for (int t = planes == 2 ? SPLIT128 : TILE256; t >= (planes == 2 ? SPLIT64 : TILE64); --t) {
     const int64_t thin = thin_rows(m, t), slots = (int64_t)CUS * TILE_SLOTS[t], full = tiles_of(m - thin, n, t);
-    const double one = tile_us(t, full, steps);
+    const double share = std::min<double>(TILE_SLOTS[t], std::max(1.0, (double)full / CUS));
+    const double one = tile_us(t, full, steps) + (double)TILE_M[t] * TILE_M[t] * out_bytes * share / 20e3;
     double e = ceil_div(full, slots) * one;
     if (thin && full + ceil_div(n, 64) > ceil_div(full, slots) * slots) e += THIN[t] * one;  // not into what the last round leaves free
     if (e < us) us = e, best = t;
@@ -1102,7 +1102,7 @@ Plan plan_common(int type, const void* x, int64_t ldx, const void* w, int64_t ld
 Plan plan_loss(int type, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab, int64_t width) {
   Bump b;
   Plan p = plan_common(type, x, ldx, w, ldw, rows, vocab, width, false, b);
-  p.tile = tile_for(vocab, rows, p.width_pad / 64, p.planes);
+  p.tile = tile_for(vocab, rows, p.width_pad / 64, p.planes, 0);
   p.part = b.take(ceil_div(vocab, TILE_M[p.tile]) * rows * 8);
   p.tlogit = b.take(rows * 4);
   p.bytes = b.n;
@@ -1192,8 +1192,12 @@ int check_ws(const void* ws, int64_t have, int64_t need) {
   return PST_OK;
 }
 
-// grids of the copying kernels: a few workgroups a compute unit
-unsigned copy_grid(int64_t groups) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(groups, 256), CUS * 16ll)); }
+// workgroups of the kernels that go through rows by a Spread: each thread one row, up to a few workgroups a compute unit
+int32_t row_grid(int64_t rows, int64_t per_row) {
+  int shift = 0;
+  while (shift < 6 && (1 << shift) < per_row) ++shift;
+  return (int32_t)std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows << shift, 256), CUS * 16ll));
+}
 
 // the operands in a form that the products read: in place, or packed (and split) into the workspace; for the gradient
 // (gloss) also the scale of D. One launch, two for 32-bit operands, none where there is nothing to do.
@@ -1213,7 +1217,7 @@ int operands(const Plan& p, const void* x, int64_t ldx, const void* w, int64_t l
     PackJob& j = a.job[which];
     j = {src, ld, rows, rows_pad, ws + at, rows_pad * p.width_pad * 2, (float*)(ws + p.amax) + which * AMAX_BLOCKS, (float*)(ws + p.unscale) + which,
          which == 0 && gloss, ((uintptr_t)src & 15) == 0 && ld * e % 16 == 0};
-    a.blocks[which] = (int32_t)copy_grid(rows_pad * (p.width_pad / (j.wide ? 8 : 2)));
+    a.blocks[which] = row_grid(rows_pad, p.width_pad / (j.wide ? 8 : 2));
     return Operand{ws + at, j.plane, p.width_pad * 2, (int32_t)rows_pad, (int32_t)p.width_pad * 2};
   };
   *X = p.pack_x ? job(0, x, ldx, p.rows, p.rows_pad, p.x) : Operand{(const char*)x, 0, ldx * e, (int32_t)p.rows, (int32_t)p.width * e};
@@ -1320,7 +1324,7 @@ int token_loss_grad(int device, int type, const void* x, int64_t ldx, const void
     g.dplane = dop.plane;
     g.ldd = ldd;
     g.v0 = (int32_t)v0;
-    if (rows) HEADCHK(launch_gemm(DLOGIT, p.elem, tile_for(nv, rows, g.steps, p.planes), g, st));
+    if (rows) HEADCHK(launch_gemm(DLOGIT, p.elem, tile_for(nv, rows, g.steps, p.planes, p.planes), g, st));
     GradArgs b{};
     b.dx.A = Wv;
     b.dx.B = b.dw.B = dop;
@@ -1356,7 +1360,7 @@ int token_loss_grad(int device, int type, const void* x, int64_t ldx, const void
   auto job = [&](int which, int64_t part, int64_t n, int nz, void* out, int64_t ldo, const float* u) {
     f.job[which] = {(const float*)(ws + part), p.width_pad, n * p.width_pad, n, nz, which == 0, out, ldo, ungs, u,
                     ldo % 4 == 0 && ((uintptr_t)out & (type == PST_F32 ? 15 : 7)) == 0};
-    f.blocks[which] = (int32_t)copy_grid(n * ceil_div(width, 4));
+    f.blocks[which] = row_grid(n, ceil_div(width, 4));
   };
   if (need_dx) job(0, p.dxp, rows, p.zx, dx, lddx, uw);
   if (dw && p.zw > 1) job(1, p.dwp, vocab, p.zw, dw, lddw, ux);
@@ -1435,7 +1439,7 @@ int token_scores_i8(int device, int type, const void* x, int64_t ldx, const int8
   HEADCHK(launch_quantize({x, ldx, p.width_pad, rows, (int32_t)width, (int32_t)p.width_pad, type, (int8_t*)(ws + p.q), (float*)(ws + p.scale), 0, 0}, st));
   GemmArgs g{};
   if (p.pack_w) {
-    hipLaunchKernelGGL(k_pack8, dim3(copy_grid(vocab * (p.width_pad / 16))), dim3(256), 0, st, w, ldw, vocab, (int32_t)width, (int32_t)p.width_pad,
+    hipLaunchKernelGGL(k_pack8, dim3(row_grid(vocab, p.width_pad / 4)), dim3(256), 0, st, w, ldw, vocab, (int32_t)width, (int32_t)p.width_pad,
                        (int8_t*)(ws + p.w));
     HEADCHK(hipGetLastError());
     g.A = {ws + p.w, 0, p.width_pad, (int32_t)vocab, (int32_t)p.width_pad};
@@ -1452,7 +1456,7 @@ int token_scores_i8(int device, int type, const void* x, int64_t ldx, const int8
   g.wide = ldo % (16 / size_of(otype)) == 0 && ((uintptr_t)out & 15) == 0;
   g.sn = (const float*)(ws + p.scale);
   g.sm = wscale;
-  HEADCHK(launch_gemm(SCORES, I8, tile_for(vocab, rows, g.steps), g, st));
+  HEADCHK(launch_gemm(SCORES, I8, tile_for(vocab, rows, g.steps, 1, size_of(otype)), g, st));
   return PST_OK;
 }
 
