@@ -9,7 +9,10 @@
 // in a workspace that the last-level cache holds, and multiplies it in both directions from there.
 //
 // 32-bit inputs: each value is split into two 16-bit floats (hi + lo, 22 bits of mantissa) after a scaling of
-// the whole tensor by a power of two, and a product is lo hi + hi lo + hi hi on the 16-bit matrix cores: about 2^-22 of the operands' product, at three sixteenths of the 32-bit instructions' time.
+// the whole tensor by a power of two, and a product is lo hi + hi lo + hi hi on the 16-bit matrix cores: off by about
+// 2^-22 of the operands' product, at 0.41 - 0.49 PFLOP/s of such products where the 32-bit instructions reach 0.154.
+//
+// Times in this file: one MI355X, median of 40 - 600 calls in a row.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -112,7 +115,8 @@ struct AmaxArgs {
   int32_t width;
   float* part;  // [2][AMAX_BLOCKS]
 };
-// the largest finite magnitude of each of two matrices, in AMAX_BLOCKS parts; a wave a row
+// the largest finite magnitude of each of two matrices, in AMAX_BLOCKS parts; a wave a row. A pass of its own, since a
+// split by the largest value of each row would have to put the rows' scales into D. 1023 + 4099 rows of 333: 4.7 us.
 __global__ __launch_bounds__(1024) void k_amax(AmaxArgs a) {
   const int t = blockIdx.x / AMAX_BLOCKS, b = blockIdx.x % AMAX_BLOCKS;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -147,7 +151,8 @@ struct Spread {
   }
 };
 
-// A matrix copied into rows of whole K-steps with zeros behind, 32-bit values split into two planes
+// A matrix copied into rows of whole K-steps with zeros behind, 32-bit values split into two planes. Bound by its bytes
+// where they are many: 8192 x 1024 bf16 8.2 us, 1000 + 4096 rows of 512 f32 6.3 us; odd rows, two values a thread, 9 us.
 struct PackJob {
   const void* src;         // null: nothing to do
   int64_t ld;
@@ -380,6 +385,11 @@ __device__ __forceinline__ void tiles(const GemmArgs& g, int tile, int stride, i
   }
 }
 
+// The loss: m = vocabulary row, n = position, so a lane holds 32 logits of each of its columns: their maximum and the sum of
+// exp(l - maximum) in registers, then over the column's four lanes and the two wave rows, and 8 bytes a tile and position
+// go to memory. One exponential a logit (16 clocks of a SIMD for 64 of them) is 1/8 of the matrix work at d = 1024;
+// persistent workgroups load the next tile meanwhile.
+// 8192 x 64003 x 1024 bf16: 829 us, 1.30 PFLOP/s (the library's product of that shape alone, logits to memory: 961 us).
 struct LossEpilogue {
   struct Inputs {
     int target;
@@ -477,7 +487,7 @@ struct JoinArgs {
   float *loss, *lse;
   int32_t n, tiles;
 };
-// 16 waves share the vocabulary tiles of 64 positions
+// 16 waves share the vocabulary tiles of 64 positions; 8192 positions of 251 tiles (16 MB): 7.7 us
 __global__ __launch_bounds__(1024) void k_join(JoinArgs a) {
   __shared__ float2 sm[16][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -506,7 +516,10 @@ __global__ __launch_bounds__(1024) void k_join(JoinArgs a) {
   a.loss[n] = !counts ? 0.0f : t < 0 ? __builtin_nanf("") : lse - a.tlogit[n];
 }
 
-// D of one piece of the vocabulary (columns v0 ...; zeros behind the last row and for positions that do not count)
+// D of one piece of the vocabulary (columns v0 ...; zeros behind the last row and for positions that do not count), in
+// 16 bits: the type the matrix cores take, and the 2^-8 (2^-11) it costs, relative, is what the operands' own rounding did. exp(l - lse) as
+// 2^((l - lse) log2 e): the difference first, so that large logits lose nothing in the product.
+// Stores of 16 bytes a lane. 8192 x 16384 x 1024 bf16: 240 us, 1.14 PFLOP/s.
 template <int E>
 struct DlogitEpilogue {
   static constexpr int TYPE = E == BF16 ? PST_BF16 : PST_F16;
@@ -630,7 +643,7 @@ __device__ __forceinline__ void store_part(const f32x4 (&acc)[T::MI][T::NI], con
   }
 }
 
-// a gradient from its parts' sums
+// a gradient from its parts' sums; 2 x 3 parts of 4096 x 512 (50 MB, in the cache): 11 us
 struct FinishJob {
   const float* part;
   int64_t ldp, zstride;
@@ -719,7 +732,8 @@ __device__ __forceinline__ void store_rows(const f32x4 (&acc)[T::MI][T::NI], con
   else store_rows_of<PST_F32, T>(acc, g, p, row0);
 }
 
-// Both gradients of a piece of the vocabulary in one launch, since D feeds both and neither fills the card evenly:
+// Both gradients of a piece of the vocabulary in one launch, since D feeds both and neither fills the card evenly (8192 x
+// 16384 x 1024 bf16: 426 us, 1.29 PFLOP/s; 4096 x 4099 x 512: 43 us together, 31 and 45 in launches of their own):
 // dx's parts (m = column, n = position, k = vocabulary row of the piece, its K loop in nz parts) and rows v0 ... of dW
 // (m = column, n = vocabulary row, k = position; in one part straight to the output, or in parts as dx).
 template <int E, class T, bool DX>
@@ -752,7 +766,9 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES) void k_grads(GradArgs g) {
   }
 }
 
-// 8-bit scores: m = vocabulary row, n = position
+// 8-bit scores: m = vocabulary row, n = position. Few positions are bound by the table's bytes: 16 x 64003 x 1024 12.8 us,
+// 5.3 TB/s with the scores; many by power, as the other products, and by their stores: 8192 x 64003 x 1024 to bf16 618 us,
+// 1.74 POP/s and 1.7 TB/s.
 struct ScoresEpilogue {
   struct Inputs {
     float sm, sn;
@@ -826,8 +842,8 @@ __device__ __forceinline__ void load8(const QuantArgs& a, int64_t row, int c, fl
   for (int j = 0; j < 8; ++j) v[j] = c + j < a.width ? load1(a.src, a.type, row + c + j) : 0.0f;
 }
 // One wave a row: the largest magnitude, then rint(x / s), rows of up to 512 ITERS values read once. A row that holds
-// an infinity or a NaN gets the scale NaN and zeros, so that what is computed from it says so.
-// 8192 x 1024 bf16 -> 8 bits moves 25 MB.
+// an infinity or a NaN gets the scale NaN and zeros, so that what is computed from it says so. 16 x 1024 4 us, 8192 x 1024
+// f16 15 us (25 MB: its launch and two passes of latency; through a reciprocal instead of the division it took as long).
 template <int ITERS>
 __global__ __launch_bounds__(256) void k_quantize(QuantArgs a) {
   const int lane = threadIdx.x & 63;
@@ -1201,7 +1217,8 @@ int32_t row_grid(int64_t rows, int64_t per_row) {
 
 // the operands in a form that the products read: in place, or packed (and split) into the workspace; for the gradient
 // (gloss) also the scale of D. One launch, two for 32-bit operands, none where there is nothing to do.
-int operands(const Plan& p, const void* x, int64_t ldx, const void* w, int64_t ldw, const Targets& t, const float* gloss, char* ws, hipStream_t st, Operand* X, Operand* W) {
+int operands(const Plan& p, const void* x, int64_t ldx, const void* w, int64_t ldw, const Targets& t, const float* gloss, char* ws,
+             hipStream_t st, Operand* X, Operand* W) {
   PackArgs a{};
   a.width = (int32_t)p.width;
   a.width_pad = (int32_t)p.width_pad;
@@ -1279,7 +1296,8 @@ int token_loss_grad(int device, int type, const void* x, int64_t ldx, const void
   if ((dx && lddx < width) || (dw && lddw < width)) return fail(PST_E_INVALID, "a gradient's row stride is smaller than the width");
   if (((uintptr_t)dx % e) || ((uintptr_t)dw % e)) return fail(PST_E_INVALID, "a gradient is not aligned to its type");
   if (!dx && !dw) return PST_OK;
-  if (rows && (!lse || !gloss || ((uintptr_t)lse & 3) || ((uintptr_t)gloss & 3))) return fail(PST_E_INVALID, "lse or grad_loss is null or not aligned");
+  if (rows && (!lse || !gloss || ((uintptr_t)lse & 3) || ((uintptr_t)gloss & 3)))
+    return fail(PST_E_INVALID, "lse or grad_loss is null or not aligned");
   if (rows == 0 && !dw) return PST_OK;
   const Plan p = plan_grad(type, x, ldx, w, ldw, std::max<int64_t>(rows, 1), vocab, width);
   rc = check_ws(ws_, ws_bytes, p.bytes);
@@ -1382,13 +1400,15 @@ hipError_t launch_quantize(QuantArgs a, hipStream_t st) {
   return hipGetLastError();
 }
 
-int quantize_rows(int device, int type, const void* x, int64_t ldx, int64_t rows, int64_t width, int8_t* q, int64_t ldq, float* scale, hipStream_t st) {
+int quantize_rows(int device, int type, const void* x, int64_t ldx, int64_t rows, int64_t width, int8_t* q, int64_t ldq, float* scale,
+                  hipStream_t st) {
   if (!is_type(type)) return fail(PST_E_INVALID, "unknown type");
   if (rows < 0 || width < 1) return fail(PST_E_INVALID, "rows >= 0 and width >= 1 are needed");
   if (rows > (1ll << 30) || width > (1 << 20)) return fail(PST_E_TOO_LARGE, "rows over 2^30, or width over 2^20");
   if (ldx < width || ldq < width) return fail(PST_E_INVALID, "a row stride is smaller than the width");
   if (rows == 0) return PST_OK;
-  if (!x || ((uintptr_t)x % size_of(type)) || !q || !scale || ((uintptr_t)scale & 3)) return fail(PST_E_INVALID, "a buffer is null or not aligned to its type");
+  if (!x || ((uintptr_t)x % size_of(type)) || !q || !scale || ((uintptr_t)scale & 3))
+    return fail(PST_E_INVALID, "a buffer is null or not aligned to its type");
   OnDevice on(device);
   if (on.e != hipSuccess) return hip_fail("device " + std::to_string(device), on.e);
   HEADCHK(launch_quantize({x, ldx, ldq, rows, (int32_t)width, (int32_t)width, type, q, scale, 0, 0}, st));
@@ -1429,14 +1449,16 @@ int token_scores_i8(int device, int type, const void* x, int64_t ldx, const int8
   if (!is_type(otype)) return fail(PST_E_INVALID, "unknown output type");
   if (rows == 0) return PST_OK;
   if (ldo < vocab) return fail(PST_E_INVALID, "the scores' row stride is smaller than the vocabulary");
-  if (!wscale || ((uintptr_t)wscale & 3) || !out || ((uintptr_t)out % size_of(otype))) return fail(PST_E_INVALID, "scale or scores is null or not aligned");
+  if (!wscale || ((uintptr_t)wscale & 3) || !out || ((uintptr_t)out % size_of(otype)))
+    return fail(PST_E_INVALID, "scale or scores is null or not aligned");
   const ScorePlan p = plan_scores(w, ldw, rows, vocab, width);
   rc = check_ws(ws_, ws_bytes, p.bytes);
   if (rc != PST_OK) return rc;
   OnDevice on(device);
   if (on.e != hipSuccess) return hip_fail("device " + std::to_string(device), on.e);
   char* ws = (char*)ws_;
-  HEADCHK(launch_quantize({x, ldx, p.width_pad, rows, (int32_t)width, (int32_t)p.width_pad, type, (int8_t*)(ws + p.q), (float*)(ws + p.scale), 0, 0}, st));
+  HEADCHK(launch_quantize(
+      {x, ldx, p.width_pad, rows, (int32_t)width, (int32_t)p.width_pad, type, (int8_t*)(ws + p.q), (float*)(ws + p.scale), 0, 0}, st));
   GemmArgs g{};
   if (p.pack_w) {
     hipLaunchKernelGGL(k_pack8, dim3(row_grid(vocab, p.width_pad / 4)), dim3(256), 0, st, w, ldw, vocab, (int32_t)width, (int32_t)p.width_pad,

@@ -7,7 +7,10 @@
 //
 // What bounds the large products is power: with operands of random bits the card sustains 2.06 PFLOP/s of bf16
 // 16x16x32 and 1.77 of 32x32x16 (whose sums move twice the bits for each product; 8-bit: 4.04 and 3.40), all from
-// registers. So the small block is used, and bytes are moved as rarely as the registers allow: 128 x 64 a wave.
+// registers. So the small block is used, and bytes are moved as rarely as the registers allow: 128 x 64 a wave. At 1.29
+// PFLOP/s the matrix cores are busy 2/3 of the time at 1.87 GHz; without the loads to LDS (leaving all else) the same
+// instructions take 155 us instead of 216, without the LDS reads 195: what remains is moving operands. 80 % of the loads
+// hit L2, whose share of the rest is what the tile order leaves: each matrix once from behind it.
 //
 // A K-step is 128 bytes of k (64 16-bit values, 128 8-bit ones) of every tile row. Operands are staged by
 // global_load_lds_dwordx4 (global memory to LDS without registers: lane i of the instruction fills 16 bytes
@@ -22,8 +25,6 @@
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
-
-#include <type_traits>
 
 namespace pst_head {
 
@@ -192,17 +193,18 @@ struct Tile {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NW = WM_ * WN_, THREADS = NW * 64;
   static constexpr int MI = BM_ / WM_ / 16, NI = BN_ / WN_ / 16;  // a wave's 16x16 blocks
   static constexpr int WAVES = 2;  // on each SIMD at least: what a workgroup's registers leave room for
-  static constexpr int STAGES = STAGES_, PLANES = PLANES_, STAGE = (BM_ + BN_) * STEP * PLANES_, LDS = STAGES * STAGE;  // (an epilogue's own LDS lies behind)
+  static constexpr int STAGES = STAGES_, PLANES = PLANES_;
+  static constexpr int STAGE = (BM_ + BN_) * STEP * PLANES_, LDS = STAGES * STAGE;  // (an epilogue's own LDS lies behind)
 };
 
 // The K loop of one tile after another: begin() starts the loads of a tile's first K-steps, run() leaves the tile's sums in
 // acc[MI][NI] of this wave. Between them a workgroup can store the tile before.
 // A ring of S LDS stages: the loads of K-step t + S start when all waves have read the last of step t, and fly while the
-// steps between are multiplied. 256-row tiles have room for two; a smaller tile's step is shorter than a load's way. A K-step is four parts, (k half, half of the wave's rows): each part's fragments are read from LDS while
-// the part before is multiplied, also across the one barrier of a K-step.
-// Measured at 8192 x 16128 x 1024 bf16 (216 us as it is): K-steps of 64 bytes in rings of 3, 4 and 5 stages 226 - 228 (twice
-// the barriers; deeper prefetch gains nothing), two 256 x 128 workgroups a unit 252 (half as much again through LDS),
-// four waves of 128 x 128 224, blocks of 32 x 32 227.
+// steps between are multiplied. A K-step is four parts, (k half, half of the wave's rows): each part's fragments are read
+// from LDS while the part before is multiplied, also across the one barrier of a K-step.
+// Measured at 8192 x 16128 x 1024 bf16 (dW, 210 - 216 us as it is): K-steps of 64 bytes in rings of 3, 4 and 5 stages
+// 226 - 228 (twice the barriers; deeper prefetch gains nothing), two 256 x 128 workgroups a unit 252 (half as much again
+// through LDS), four waves of 128 x 128 224, blocks of 32 x 32 227, loads in one burst 222.
 template <int E, class T, bool ACOLS, bool BCOLS>
 struct Loop {
   typedef typename Mma<E>::Acc Acc;

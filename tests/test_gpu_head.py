@@ -461,3 +461,30 @@ def test_refusals_on_the_gpu():
         head.token_scores_int8(x, q, s[:29])
     with pytest.raises(ValueError, match="out_dtype"):
         head.token_scores_int8(x, q, s, out_dtype=torch.float64)
+
+
+class TokenLoss(torch.autograd.Function):
+    """The operators under autograd, as the integration notes give them."""
+
+    @staticmethod
+    def forward(ctx, hidden, weight, targets):
+        loss, lse = head.token_loss(hidden, weight, targets)
+        ctx.save_for_backward(hidden, weight, targets, lse)
+        return loss
+
+    @staticmethod
+    def backward(ctx, grad_loss):
+        hidden, weight, targets, lse = ctx.saved_tensors
+        return (*head.token_loss_grad(hidden, weight, targets, lse, grad_loss.contiguous()), None)
+
+
+def test_under_autograd():
+    x, w, t, _ = make(60, 432, 48, torch.float32, seed=9)
+    x.requires_grad_(), w.requires_grad_()
+    n = (t != -100).sum()
+    TokenLoss.apply(x, w, t).sum().div(n).backward()
+    a, b = x.detach().double().requires_grad_(), w.detach().double().requires_grad_()
+    torch.nn.functional.cross_entropy(a @ b.T, t, ignore_index=-100).backward()
+    # 60 and 432 terms, split products of 2^-21, exponents off by a few of 2^-24: far below 1e-5 of the norm
+    assert (x.grad.double() - a.grad).norm() <= 1e-5 * a.grad.norm()
+    assert (w.grad.double() - b.grad).norm() <= 1e-5 * b.grad.norm()
