@@ -487,33 +487,40 @@ struct JoinArgs {
   float *loss, *lse;
   int32_t n, tiles;
 };
-// 16 waves share the vocabulary tiles of 64 positions; 8192 positions of 251 tiles (16 MB): 7.7 us
+// 1024 threads share the vocabulary tiles of COLS positions; 8192 positions of 251 tiles (16 MB): 7.7 us
+template <int COLS>
 __global__ __launch_bounds__(1024) void k_join(JoinArgs a) {
-  __shared__ float2 sm[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int n = blockIdx.x * 64 + lane;
-  float mx = -__builtin_inff(), sum = 0.0f;
-  if (n < a.n)
-    for (int t = wave; t < a.tiles; t += 16) {
-      const float2 q = a.part[(int64_t)t * a.n + n];
-      const float m2 = fmaxf(mx, q.x);
-      const float safe = m2 == -__builtin_inff() ? 0.0f : m2;
-      sum = sum * exp2_fast((mx - safe) * LOG2E) + q.y * exp2_fast((q.x - safe) * LOG2E);
-      mx = m2;
-    }
-  sm[wave][lane] = make_float2(mx, sum);
-  __syncthreads();
-  if (wave != 0 || n >= a.n) return;
-  float top = sm[0][lane].x;
-  for (int w = 1; w < 16; ++w) top = fmaxf(top, sm[w][lane].x);
-  const float safe = top == -__builtin_inff() ? 0.0f : top;
-  float s = 0.0f;
-  for (int w = 0; w < 16; ++w) s += sm[w][lane].y * exp2_fast((sm[w][lane].x - safe) * LOG2E);
-  const float lse = safe + logf(s);
+  constexpr int ROWS = 1024 / COLS;
+  __shared__ float2 sm[ROWS][COLS];
+  const int col = threadIdx.x % COLS, row = threadIdx.x / COLS;
+  const int n = blockIdx.x * COLS + col;
+  auto join = [](float2 p, float2 q) {
+    const float mx = fmaxf(p.x, q.x);
+    const float safe = mx == -__builtin_inff() ? 0.0f : mx;
+    return make_float2(mx, p.y * exp2_fast((p.x - safe) * LOG2E) + q.y * exp2_fast((q.x - safe) * LOG2E));
+  };
+  float2 mine = make_float2(-__builtin_inff(), 0.0f);
+  if (n < a.n) {
+#pragma unroll 4
+    for (int t = row; t < a.tiles; t += ROWS) mine = join(mine, a.part[(int64_t)t * a.n + n]);
+  }
+  sm[row][col] = mine;
+#pragma unroll
+  for (int half = ROWS / 2; half >= 1; half >>= 1) {
+    __syncthreads();
+    if (row < half) sm[row][col] = join(sm[row][col], sm[row + half][col]);
+  }
+  if (row != 0 || n >= a.n) return;
+  const float2 all = sm[0][col];
+  const float lse = (all.x == -__builtin_inff() ? 0.0f : all.x) + logf(all.y);
   bool counts;
   const int t = target_of(a.targets, n, counts);
   a.lse[n] = lse;
   a.loss[n] = !counts ? 0.0f : t < 0 ? __builtin_nanf("") : lse - a.tlogit[n];
+}
+void launch_join(const JoinArgs& j, hipStream_t st) {
+  if (j.n <= 1024) hipLaunchKernelGGL(k_join<16>, dim3((unsigned)((j.n + 15) / 16)), dim3(1024), 0, st, j);
+  else hipLaunchKernelGGL(k_join<64>, dim3((unsigned)((j.n + 63) / 64)), dim3(1024), 0, st, j);
 }
 
 // D of one piece of the vocabulary (columns v0 ...; zeros behind the last row and for positions that do not count), in
@@ -811,6 +818,102 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES) void k_scores(GemmArgs g) {
   }
 }
 
+// ------------------------------------------------------------------ the loss of few positions, 32 bits
+// With few positions the way of a 32-bit table through memory is all that counts, and the products above would split it
+// first: read it twice, write as much and read that. This kernel reads it once for 16 NB positions, at any alignment, and
+// multiplies in 32 bits (v_mfma_f32_16x16x4: 32 clocks of a SIMD for 256 bytes of the table, 17 TB/s of them all). us with
+// the split, and so: 1 x 64000 x 1024 205, 51 (5.1 TB/s); 32 x 64000 x 1024 206, 99; 16 x 4096 x 2048 50, 19; 64 x 432 x 64
+// 25, 19; but 64 x 64000 x 333 92, 160 and 256 x 4096 x 1024 35, 46: many positions read the table again and again.
+struct FewArgs {
+  const float *x, *w;
+  int64_t ldx, ldw;
+  int32_t wide;          // rows of whole fours, aligned to 16 bytes
+  int32_t rows, vocab, width;
+  int32_t blocks;        // 16-row blocks of the table a workgroup
+  Targets targets;
+  float2* part;          // [workgroups][rows]
+  float* tlogit;
+};
+// four neighbours of a row from column k, zeros behind its `width`: loads without a branch, so that many are in flight
+__device__ __forceinline__ f32x4 load4(const float* row, bool wide, int k, int width) {
+  f32x4 v;
+  if (wide) {
+    v = *(const f32x4*)(row + min(k, width - 4));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = row[min(k + j, width - 1)];
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = k + j < width ? v[j] : 0.0f;
+  return v;
+}
+// `blocks` 16-row blocks of the table and 16 NB positions: the four waves take every fourth 16 columns, and each finishes a
+// block of 16 positions
+template <int NB>
+__global__ __launch_bounds__(256) void k_few(FewArgs a) {
+  __shared__ f32x4 sm[4][NB][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.y * 16 * NB;
+  const float* xrow[NB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) xrow[j] = a.x + min(n0 + 16 * j + r, a.rows - 1) * a.ldx;
+  const bool mine = wave < NB;
+  const int n = n0 + 16 * wave + r;
+  int target = -1;
+  bool counts = false;
+  if (mine && n < a.rows) target = target_of(a.targets, n, counts);
+  float mx = -__builtin_inff(), sum = 0.0f;
+  const int first = blockIdx.x * a.blocks * 16, last = min(first + a.blocks * 16, a.vocab);
+  for (int v0 = first; v0 < last; v0 += 16) {
+    const float* wrow = a.w + min(v0 + r, a.vocab - 1) * a.ldw;
+    f32x4 acc[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) acc[j] = {0, 0, 0, 0};
+    constexpr int U = NB == 1 ? 4 : 2;
+    for (int k0 = wave * 16; k0 < a.width; k0 += 64 * U) {
+      f32x4 wv[U], xv[U][NB];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int k = k0 + 64 * u + 4 * g;
+        wv[u] = load4(wrow, a.wide, k, a.width);
+#pragma unroll
+        for (int j = 0; j < NB; ++j) xv[u][j] = load4(xrow[j], a.wide, k, a.width);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int j = 0; j < NB; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(wv[u][e], xv[u][j][e], acc[j], 0, 0, 0);
+    }
+    __syncthreads();  // the block before has been read
+#pragma unroll
+    for (int j = 0; j < NB; ++j) sm[wave][j][lane] = acc[j];
+    __syncthreads();
+    if (!mine) continue;
+    f32x4 l = {0, 0, 0, 0};
+    for (int w = 0; w < 4; ++w) l += sm[w][wave][lane];
+    const int v = v0 + 4 * g;
+    float m = mx;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (v + q >= a.vocab) l[q] = -__builtin_inff();
+      else if (v + q == target) a.tlogit[n] = l[q];
+      m = fmaxf(m, l[q]);
+    }
+    const float safe = m == -__builtin_inff() ? 0.0f : m;
+    sum *= exp2_fast((mx - safe) * LOG2E);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) sum += exp2_fast((l[q] - safe) * LOG2E);
+    mx = m;
+  }
+  if (!mine) return;
+  const float top = col_max(mx), safe = top == -__builtin_inff() ? 0.0f : top;
+  sum = col_sum(sum * exp2_fast((mx - safe) * LOG2E));
+  if (lane < 16 && n < a.rows) a.part[(int64_t)blockIdx.x * a.rows + n] = make_float2(top, sum);
+}
+
 struct QuantArgs {
   const void* src;
   int64_t ld, ldq;
@@ -1089,6 +1192,7 @@ struct Plan {
   int64_t amax = 0, unscale = 0, x = 0, w = 0;   // offsets
   int64_t part = 0, tlogit = 0;                  // loss
   int64_t gscale = 0, D = 0, dxp = 0, dwp = 0;   // gradient
+  int64_t few = 0;                               // k_few: 16-row blocks a workgroup
   int64_t piece = 0;                             // vocabulary rows of a piece
   int tile = 0, zx = 1, zw = 1;                  // of the two gradients' launch
   int64_t bytes = 0;
@@ -1118,6 +1222,15 @@ Plan plan_common(int type, const void* x, int64_t ldx, const void* w, int64_t ld
 Plan plan_loss(int type, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab, int64_t width) {
   Bump b;
   Plan p = plan_common(type, x, ldx, w, ldw, rows, vocab, width, false, b);
+  // up to 32 positions, or a product of about what its launches take (see k_few); about four workgroups a compute unit
+  if (type == PST_F32 && (rows <= 32 || (rows <= 1024 && rows * vocab * width <= 1 << 27))) {
+    b = Bump();
+    p.few = ceil_div(ceil_div(vocab, 16), 4 * CUS);
+    p.part = b.take(ceil_div(vocab, 16 * p.few) * rows * 8);
+    p.tlogit = b.take(rows * 4);
+    p.bytes = b.n;
+    return p;
+  }
   p.tile = tile_for(vocab, rows, p.width_pad / 64, p.planes, 0);
   p.part = b.take(ceil_div(vocab, TILE_M[p.tile]) * rows * 8);
   p.tlogit = b.take(rows * 4);
@@ -1253,6 +1366,14 @@ int operands(const Plan& p, const void* x, int64_t ldx, const void* w, int64_t l
   return PST_OK;
 }
 
+hipError_t launch_few(const FewArgs& f, hipStream_t st) {
+  const dim3 grid((unsigned)ceil_div(f.vocab, 16ll * f.blocks), (unsigned)ceil_div(f.rows, 64)), block(256);
+  if (f.rows <= 16) hipLaunchKernelGGL(k_few<1>, grid, block, 0, st, f);
+  else if (f.rows <= 32) hipLaunchKernelGGL(k_few<2>, grid, block, 0, st, f);
+  else hipLaunchKernelGGL(k_few<4>, grid, block, 0, st, f);
+  return hipGetLastError();
+}
+
 int token_loss(int device, int type, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab, int64_t width,
                const void* targets, int tbits, int64_t ignore, float* loss, float* lse, void* ws_, int64_t ws_bytes, hipStream_t st) {
   int rc = check_sizes(type, x, ldx, w, ldw, rows, vocab, width);
@@ -1268,6 +1389,15 @@ int token_loss(int device, int type, const void* x, int64_t ldx, const void* w, 
   char* ws = (char*)ws_;
   GemmArgs g{};
   g.targets = {targets, ignore, tbits, (int32_t)vocab};
+  if (p.few) {
+    const bool wide = in_place(x, ldx * 4, width * 4) && in_place(w, ldw * 4, width * 4);
+    const FewArgs f{(const float*)x, (const float*)w, ldx, ldw, wide, (int32_t)rows, (int32_t)vocab, (int32_t)width, (int32_t)p.few, g.targets,
+                    (float2*)(ws + p.part), (float*)(ws + p.tlogit)};
+    HEADCHK(launch_few(f, st));
+    launch_join({f.part, f.tlogit, f.targets, loss, lse, (int32_t)rows, (int32_t)ceil_div(vocab, 16 * p.few)}, st);
+    HEADCHK(hipGetLastError());
+    return PST_OK;
+  }
   rc = operands(p, x, ldx, w, ldw, g.targets, nullptr, ws, st, &g.B, &g.A);
   if (rc != PST_OK) return rc;
   g.M = (int32_t)vocab;
@@ -1281,7 +1411,7 @@ int token_loss(int device, int type, const void* x, int64_t ldx, const void* w, 
   g.tlogit = (float*)(ws + p.tlogit);
   HEADCHK(launch_gemm(LOSS, p.elem, p.tile, g, st));
   JoinArgs j{g.part, g.tlogit, g.targets, loss, lse, (int32_t)rows, (int32_t)ceil_div(vocab, TILE_M[p.tile])};
-  hipLaunchKernelGGL(k_join, dim3((unsigned)ceil_div(rows, 64)), dim3(1024), 0, st, j);
+  launch_join(j, st);
   HEADCHK(hipGetLastError());
   return PST_OK;
 }

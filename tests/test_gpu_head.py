@@ -138,6 +138,16 @@ def test_strides(pad, wpad, dtype):
     check_grad(x, w, t, gl)
 
 
+# few positions of a table that is not read in place otherwise
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("rows,vocab,width,wpad", [(1, 4096, 333, 0), (2, 70001, 68, 1), (16, 1731, 129, 2), (17, 257, 1030, 3), (32, 20000, 37, 0), (64, 500, 250, 5),
+                                                   (100, 17, 20, 1)])
+def test_few_positions(rows, vocab, width, wpad, dtype):
+    x, w, t, gl = make(rows, vocab, width, dtype, seed=11, wpad=wpad)
+    _, lse = check_loss(x, w, t)
+    check_grad(x, w, t, gl, lse)
+
+
 def test_unaligned_storage():
     for dtype in TYPES:
         x, w, t, gl = make(40, 100, 64, dtype)
@@ -225,9 +235,10 @@ def test_infinite_and_not_a_number():
 @pytest.mark.parametrize("scale", [1e-30, 1e-4, 1e4])
 def test_32_bit_ranges(scale):
     # the split halves follow the tensor's largest value: products of very small and very large tensors
-    x, w, t, gl = make(40, 300, 96, torch.float32)
-    check_loss(x * scale, w / scale, t)
-    check_grad(x * scale, w / scale, t, gl)
+    for rows, vocab, width in ((40, 300, 96), (1100, 2100, 160)):
+        x, w, t, gl = make(rows, vocab, width, torch.float32)
+        check_loss(x * scale, w / scale, t)
+        check_grad(x * scale, w / scale, t, gl)
 
 
 def test_large_logits():
