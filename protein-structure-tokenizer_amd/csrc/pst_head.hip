@@ -152,7 +152,8 @@ struct Spread {
 };
 
 // A matrix copied into rows of whole K-steps with zeros behind, 32-bit values split into two planes. Bound by its bytes
-// where they are many: 8192 x 1024 bf16 8.2 us, 1000 + 4096 rows of 512 f32 6.3 us; odd rows, two values a thread, 9 us.
+// where they are many: 8192 x 1024 bf16 8.2 us, 1000 + 4096 rows of 512 f32 6.3 us; 1023 + 4099 odd rows
+// of 333 f32, two values a thread, 8.0 us (9.0 with each piece's loads behind the last one's store).
 struct PackJob {
   const void* src;         // null: nothing to do
   int64_t ld;
@@ -208,25 +209,46 @@ __global__ __launch_bounds__(256) void k_pack(PackArgs a) {
     e = split_exp(block_max(p.part[threadIdx.x], sm));
     if (block == 0 && threadIdx.x == 0) *p.unscale = ldexpf(1.0f, -e);
   }
-  const int by = p.wide ? 8 : 2;  // neighbours a thread takes
-  const Spread at_row(block, a.blocks[which], a.width_pad / by);
+  if (!p.wide) {  // two neighbours a thread; four pieces' loads before the first store
+    const Spread at_row(block, a.blocks[which], a.width_pad / 2);
+    for (int64_t r = at_row.row; r < p.rows_pad; r += at_row.rows) {
+      bool keep = r < p.rows;
+      if (keep && p.zero_rows) (void)target_of(a.targets, r, keep);
+      const int64_t from = min(r, p.rows - 1) * p.ld;
+      char* d = p.dst + r * a.width_pad * 2;
+      for (int c0 = at_row.piece * 2; c0 < a.width_pad; c0 += at_row.pieces * 8) {
+        uint32_t raw[4][2];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int64_t i = from + min(c0 + at_row.pieces * 2 * u + j, a.width - 1);
+            raw[u][j] = !keep ? 0u : f32 ? ((const uint32_t*)p.src)[i] : (uint32_t)((const uint16_t*)p.src)[i];
+          }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int c = c0 + at_row.pieces * 2 * u;
+          if (c >= a.width_pad) break;
+          const uint32_t x = c < a.width ? raw[u][0] : 0, y = c + 1 < a.width ? raw[u][1] : 0;
+          if (f32) {
+            const float fx = ldexpf(__uint_as_float(x), e), fy = ldexpf(__uint_as_float(y), e);
+            *(uint32_t*)(d + c * 2) = pack2(fx, fy, PST_F16);
+            *(uint32_t*)(d + p.plane + c * 2) = pack2(rest16(fx), rest16(fy), PST_F16);
+          } else {
+            *(uint32_t*)(d + c * 2) = x | y << 16;
+          }
+        }
+      }
+    }
+    return;
+  }
+  const Spread at_row(block, a.blocks[which], a.width_pad / 8);
   for (int64_t r = at_row.row; r < p.rows_pad; r += at_row.rows)
-  for (int c = at_row.piece * by; c < a.width_pad; c += at_row.pieces * by) {
+  for (int c = at_row.piece * 8; c < a.width_pad; c += at_row.pieces * 8) {
     bool keep = r < p.rows;
     if (keep && p.zero_rows) (void)target_of(a.targets, r, keep);
     char* d = p.dst + (r * a.width_pad + c) * 2;
-    if (!p.wide) {
-      const int64_t at = r * p.ld + c;
-      const bool k0 = keep && c < a.width, k1 = keep && c + 1 < a.width;
-      if (f32) {
-        const float x = k0 ? ldexpf(((const float*)p.src)[at], e) : 0.0f, y = k1 ? ldexpf(((const float*)p.src)[at + 1], e) : 0.0f;
-        *(uint32_t*)d = pack2(x, y, PST_F16);
-        *(uint32_t*)(d + p.plane) = pack2(rest16(x), rest16(y), PST_F16);
-      } else {
-        const uint32_t x = k0 ? ((const uint16_t*)p.src)[at] : 0, y = k1 ? ((const uint16_t*)p.src)[at + 1] : 0;
-        *(uint32_t*)d = x | y << 16;
-      }
-    } else if (!f32) {
+    if (!f32) {
       uint4 v = make_uint4(0, 0, 0, 0);
       const uint16_t* src = (const uint16_t*)p.src + r * p.ld + c;
       if (keep && c + 8 <= a.width) {
