@@ -258,7 +258,9 @@ int pst_token_loss(int32_t device, int32_t type, const void* d_hidden, int64_t l
  * Gradients of sum_n grad_loss[n] loss[n] for hidden and weight (either may be NULL), of the operands' type, from the
  * lse of pst_token_loss. Ignored positions have zero gradient and add nothing to the weight's, whatever their hidden
  * row holds. A target out of range makes its position's gradient, and the weight's, NaN. rows = 0 writes a zero weight
- * gradient. No atomics: the same inputs give the same bits.
+ * gradient. No atomics: the same inputs give the same bits. PST_F32: hidden (its positions that count), weight and
+ * grad_loss are each scaled as a whole and held to 2^-22 of a value and 2^-38 of the largest one, so that values 10^6
+ * below the largest of their tensor keep about five digits (the loss scales row by row and has no such limit).
  */
 int64_t pst_token_loss_grad_workspace(int32_t type, const void* d_hidden, int64_t ld_hidden, const void* d_weight, int64_t ld_weight,
                                       int64_t rows, int64_t vocab, int64_t width);

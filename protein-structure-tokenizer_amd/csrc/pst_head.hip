@@ -8,8 +8,8 @@
 // row (k_loss) and joins them (k_join); the gradient makes D for a piece of the vocabulary at a time, in 16 bits
 // in a workspace that the last-level cache holds, and multiplies it in both directions from there.
 //
-// 32-bit inputs: each value is split into two 16-bit floats (hi + lo, 22 bits of mantissa) after a scaling of
-// the whole tensor by a power of two, and a product is lo hi + hi lo + hi hi on the 16-bit matrix cores: off by about
+// 32-bit inputs: each value is split into two 16-bit floats (hi + lo, 22 bits of mantissa) after a scaling by
+// a power of two (of each row for the loss, of the whole tensor for the gradient), and a product is lo hi + hi lo + hi hi on the 16-bit matrix cores: off by about
 // 2^-22 of the operands' product, at 0.41 - 0.49 PFLOP/s of such products where the 32-bit instructions reach 0.154.
 //
 // Times in this file: one MI355X, median of 40 - 600 calls in a row.
@@ -114,14 +114,20 @@ struct AmaxArgs {
   int64_t rows[2];
   int32_t width;
   float* part;  // [2][AMAX_BLOCKS]
+  Targets targets;
 };
-// the largest finite magnitude of each of two matrices, in AMAX_BLOCKS parts; a wave a row. A pass of its own, since a
-// split by the largest value of each row would have to put the rows' scales into D. 1023 + 4099 rows of 333: 4.7 us.
+// The gradient's operands: the largest finite magnitude of each of two matrices, in AMAX_BLOCKS parts; a wave a row. Rows of
+// the first whose position does not count are left out (k_pack makes them zeros). A pass of its own, since the products
+// sum over rows: a split by the largest value of each row would have to put the rows' scales into D. 1000 + 4096 rows of
+// 512: 4.0 us.
 __global__ __launch_bounds__(1024) void k_amax(AmaxArgs a) {
   const int t = blockIdx.x / AMAX_BLOCKS, b = blockIdx.x % AMAX_BLOCKS;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   float m = 0.0f;
   for (int64_t r = b * 16 + wave; r < a.rows[t]; r += AMAX_BLOCKS * 16) {
+    bool counts = true;
+    if (t == 0) (void)target_of(a.targets, r, counts);
+    if (!counts) continue;
     const float* row = a.p[t] + r * a.ld[t];
 #pragma unroll 8
     for (int k = lane; k < a.width; k += 64) m = fmaxf(m, finite_abs(row[k]));
@@ -160,8 +166,8 @@ struct PackJob {
   int64_t rows, rows_pad;  // rows beyond `rows` are zeros
   char* dst;               // 16-bit [planes][rows_pad][width_pad]
   int64_t plane;           // bytes
-  const float* part;       // 32-bit: the tensor's AMAX_BLOCKS maxima
-  float* unscale;          // 32-bit: 2^-e
+  const float* part;       // 32-bit: the tensor's AMAX_BLOCKS maxima; null: each row is split by its own maximum
+  float* unscale;          // 32-bit: 2^-e, of the tensor or of each row
   int32_t zero_rows;       // rows whose position does not count are zeros
   int32_t wide;            // the source allows 16-byte loads
 };
@@ -182,6 +188,16 @@ __device__ __forceinline__ float block_max(float m, float* sm) {
   if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
   __syncthreads();
   return fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+}
+// a row's exponent, by the neighbouring threads that have it
+__device__ __forceinline__ int row_exp(const float* row, int width, int64_t r, const Spread& at_row, float* unscale) {
+  float m = 0.0f;
+#pragma unroll 8
+  for (int k = at_row.piece; k < width; k += at_row.pieces) m = fmaxf(m, finite_abs(row[k]));
+  for (int s = at_row.pieces / 2; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
+  const int e = split_exp(m);
+  if (at_row.piece == 0) unscale[r] = ldexpf(1.0f, -e);
+  return e;
 }
 __global__ __launch_bounds__(256) void k_pack(PackArgs a) {
   __shared__ float sm[4];
@@ -205,7 +221,8 @@ __global__ __launch_bounds__(256) void k_pack(PackArgs a) {
   const PackJob& p = a.job[which];
   const bool f32 = a.type == PST_F32;
   int e = 0;
-  if (f32) {
+  const bool by_row = f32 && !p.part;
+  if (f32 && !by_row) {
     e = split_exp(block_max(p.part[threadIdx.x], sm));
     if (block == 0 && threadIdx.x == 0) *p.unscale = ldexpf(1.0f, -e);
   }
@@ -215,6 +232,7 @@ __global__ __launch_bounds__(256) void k_pack(PackArgs a) {
       bool keep = r < p.rows;
       if (keep && p.zero_rows) (void)target_of(a.targets, r, keep);
       const int64_t from = min(r, p.rows - 1) * p.ld;
+      if (by_row && keep) e = row_exp((const float*)p.src + from, a.width, r, at_row, p.unscale);
       char* d = p.dst + r * a.width_pad * 2;
       for (int c0 = at_row.piece * 2; c0 < a.width_pad; c0 += at_row.pieces * 8) {
         uint32_t raw[4][2];
@@ -243,43 +261,45 @@ __global__ __launch_bounds__(256) void k_pack(PackArgs a) {
     return;
   }
   const Spread at_row(block, a.blocks[which], a.width_pad / 8);
-  for (int64_t r = at_row.row; r < p.rows_pad; r += at_row.rows)
-  for (int c = at_row.piece * 8; c < a.width_pad; c += at_row.pieces * 8) {
+  for (int64_t r = at_row.row; r < p.rows_pad; r += at_row.rows) {
     bool keep = r < p.rows;
     if (keep && p.zero_rows) (void)target_of(a.targets, r, keep);
-    char* d = p.dst + (r * a.width_pad + c) * 2;
-    if (!f32) {
-      uint4 v = make_uint4(0, 0, 0, 0);
-      const uint16_t* src = (const uint16_t*)p.src + r * p.ld + c;
-      if (keep && c + 8 <= a.width) {
-        v = *(const uint4*)src;
-      } else if (keep) {
-        uint32_t h[8];
+    if (by_row && keep) e = row_exp((const float*)p.src + r * p.ld, a.width, r, at_row, p.unscale);
+    for (int c = at_row.piece * 8; c < a.width_pad; c += at_row.pieces * 8) {
+      char* d = p.dst + (r * a.width_pad + c) * 2;
+      if (!f32) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        const uint16_t* src = (const uint16_t*)p.src + r * p.ld + c;
+        if (keep && c + 8 <= a.width) {
+          v = *(const uint4*)src;
+        } else if (keep) {
+          uint32_t h[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) h[j] = c + j < a.width ? src[j] : 0;
-        v = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+          for (int j = 0; j < 8; ++j) h[j] = c + j < a.width ? src[j] : 0;
+          v = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+        }
+        *(uint4*)d = v;
+      } else {
+        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        const float* src = (const float*)p.src + r * p.ld + c;
+        if (keep && c + 8 <= a.width) {
+          const f32x4 lo = *(const f32x4*)src, hi = *(const f32x4*)(src + 4);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = lo[j], v[4 + j] = hi[j];
+        } else if (keep) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = c + j < a.width ? src[j] : 0.0f;
+        }
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float x = ldexpf(v[2 * j], e), y = ldexpf(v[2 * j + 1], e);
+          hi[j] = pack2(x, y, PST_F16);
+          lo[j] = pack2(rest16(x), rest16(y), PST_F16);  // an infinity or NaN stands in hi alone
+        }
+        *(uint4*)d = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *(uint4*)(d + p.plane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
-      *(uint4*)d = v;
-    } else {
-      float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-      const float* src = (const float*)p.src + r * p.ld + c;
-      if (keep && c + 8 <= a.width) {
-        const f32x4 lo = *(const f32x4*)src, hi = *(const f32x4*)(src + 4);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = lo[j], v[4 + j] = hi[j];
-      } else if (keep) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = c + j < a.width ? src[j] : 0.0f;
-      }
-      uint32_t hi[4], lo[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float x = ldexpf(v[2 * j], e), y = ldexpf(v[2 * j + 1], e);
-        hi[j] = pack2(x, y, PST_F16);
-        lo[j] = pack2(rest16(x), rest16(y), PST_F16);  // an infinity or NaN stands in hi alone
-      }
-      *(uint4*)d = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      *(uint4*)(d + p.plane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
   }
 }
@@ -293,7 +313,7 @@ struct GemmArgs {
   int32_t thins;
   int32_t steps;       // K-steps of the whole range
   int32_t gm;
-  // unscaling of 32-bit operands (device; null: 1)
+  // unscaling of 32-bit operands (device; null: 1): of each row for the loss, else of the tensor
   const float *ua, *ub;
   // loss and logit gradient: n = position, m = vocabulary row (from v0)
   Targets targets;
@@ -412,23 +432,49 @@ __device__ __forceinline__ void tiles(const GemmArgs& g, int tile, int stride, i
 // go to memory. One exponential a logit (16 clocks of a SIMD for 64 of them) is 1/8 of the matrix work at d = 1024;
 // persistent workgroups load the next tile meanwhile.
 // 8192 x 64003 x 1024 bf16: 829 us, 1.30 PFLOP/s (the library's product of that shape alone, logits to memory: 961 us).
+template <int PLANES>
 struct LossEpilogue {
   struct Inputs {
     int target;
+    float ua, ub;  // of this thread's row and column, 32-bit operands
   };
   template <class P>
   __device__ __forceinline__ Inputs load(const GemmArgs& g, const P& p) const {
     bool counts;
     const int n = p.n0 + (int)threadIdx.x;
-    return {(int)threadIdx.x < P::BN && n < g.N ? target_of(g.targets, n, counts) : -1};
+    Inputs in{(int)threadIdx.x < P::BN && n < g.N ? target_of(g.targets, n, counts) : -1, 0.0f, 0.0f};
+    if (PLANES == 2) {
+      in.ua = g.ua[min(p.m0 + (int)threadIdx.x, g.M - 1)];
+      in.ub = g.ub[min(n, g.N - 1)];
+    }
+    return in;
   }
   __device__ __forceinline__ void share(const Inputs& in, float* lds) const {
     asm volatile("" ::"v"(in.target));
     if (threadIdx.x < 256) ((int*)lds)[threadIdx.x] = in.target;
+    if (PLANES == 2) {
+      asm volatile("" ::"v"(in.ua), "v"(in.ub));
+      if (threadIdx.x < 128) {
+        lds[768 + threadIdx.x] = in.ua;
+        lds[896 + threadIdx.x] = in.ub;
+      }
+    }
   }
   template <class T>
   __device__ __forceinline__ void store(const GemmArgs& g, const Place<T>& p, f32x4 (&acc)[T::MI][T::NI], float* lds) const {
-    if (T::PLANES == 2) unscale<T>(acc, *g.ua * *g.ub);
+    if (PLANES == 2) {  // (a product of two scales stays finite, so that a logit of zero does)
+      static_assert(T::PLANES == PLANES && (PLANES == 1 || (T::BM <= 128 && T::BN <= 128)), "the scales' LDS");
+#pragma unroll
+      for (int i = 0; i < T::MI; ++i) {
+        const f32x4 ua = *(const f32x4*)(lds + 768 + p.mw - p.m0 + 16 * i);
+#pragma unroll
+        for (int j = 0; j < T::NI; ++j) {
+          const float ub = lds[896 + p.nw - p.n0 + 16 * j + p.col];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[i][j][r] *= fminf(ua[r] * ub, 3.4028234663852886e38f);
+        }
+      }
+    }
     if (p.mwave + T::MI * 16 > g.M) {  // rows behind the vocabulary's last
 #pragma unroll
       for (int i = 0; i < T::MI; ++i)
@@ -496,9 +542,9 @@ template <int E, class T>
 __global__ __launch_bounds__(T::THREADS, T::WAVES) void k_loss(GemmArgs g) {
   extern __shared__ char smem[];
   if ((int)blockIdx.x < g.blocks) {
-    tiles<E, T, true>(g, blockIdx.x, g.blocks, g.nm, g.nn, 0, smem, LossEpilogue{});
+    tiles<E, T, true>(g, blockIdx.x, g.blocks, g.nm, g.nn, 0, smem, LossEpilogue<T::PLANES>{});
   } else if constexpr (T::HAS_THIN) {
-    tiles<E, typename T::Thin, false>(g, blockIdx.x - g.blocks, 1 << 30, 1, g.thins, g.nm * T::BM, smem, LossEpilogue{});
+    tiles<E, typename T::Thin, false>(g, blockIdx.x - g.blocks, 1 << 30, 1, g.thins, g.nm * T::BM, smem, LossEpilogue<T::PLANES>{});
   }
 }
 
@@ -579,7 +625,7 @@ struct DlogitEpilogue {
   }
   template <class T>
   __device__ __forceinline__ void store(const GemmArgs& g, const Place<T>& p, f32x4 (&acc)[T::MI][T::NI], float* lds) const {
-    if (T::PLANES == 2) unscale<T>(acc, *g.ua * *g.ub);
+    if (T::PLANES == 2) unscale<T>(acc, fminf(*g.ua * *g.ub, 3.4028234663852886e38f));
     const bool edge = p.mwave + T::MI * 16 > g.M;
 #pragma unroll
     for (int j = 0; j < T::NI; ++j) {
@@ -1234,8 +1280,8 @@ Plan plan_common(int type, const void* x, int64_t ldx, const void* w, int64_t ld
   // x is the operand with zeros behind the last column; the gradient needs zeros behind the last row too
   p.pack_x = type == PST_F32 || grad || p.width_pad != width || !in_place(x, ldx * e, width * e);
   if (type == PST_F32) {
-    p.amax = b.take(2 * AMAX_BLOCKS * 4);
-    p.unscale = b.take(8);
+    if (grad) p.amax = b.take(2 * AMAX_BLOCKS * 4);
+    p.unscale = b.take((grad ? 2 : rows + vocab) * 4);
   }
   if (p.pack_x) p.x = b.take(p.rows_pad * p.width_pad * 2 * p.planes);
   if (p.pack_w) p.w = b.take(vocab * p.width_pad * 2 * p.planes);
@@ -1351,7 +1397,7 @@ int32_t row_grid(int64_t rows, int64_t per_row) {
 }
 
 // the operands in a form that the products read: in place, or packed (and split) into the workspace; for the gradient
-// (gloss) also the scale of D. One launch, two for 32-bit operands, none where there is nothing to do.
+// (gloss) also the scale of D. One launch, two for its 32-bit operands, none where there is nothing to do.
 int operands(const Plan& p, const void* x, int64_t ldx, const void* w, int64_t ldw, const Targets& t, const float* gloss, char* ws,
              hipStream_t st, Operand* X, Operand* W) {
   PackArgs a{};
@@ -1359,15 +1405,17 @@ int operands(const Plan& p, const void* x, int64_t ldx, const void* w, int64_t l
   a.width_pad = (int32_t)p.width_pad;
   a.type = p.type;
   a.targets = t;
-  if (p.type == PST_F32) {
-    AmaxArgs m{{(const float*)x, (const float*)w}, {ldx, ldw}, {p.rows, p.vocab}, (int32_t)p.width, (float*)(ws + p.amax)};
+  const bool by_row = !gloss;
+  if (p.type == PST_F32 && !by_row) {
+    AmaxArgs m{{(const float*)x, (const float*)w}, {ldx, ldw}, {p.rows, p.vocab}, (int32_t)p.width, (float*)(ws + p.amax), t};
     hipLaunchKernelGGL(k_amax, dim3(2 * AMAX_BLOCKS), dim3(1024), 0, st, m);
     HEADCHK(hipGetLastError());
   }
   const int e = size_of(p.type);
   auto job = [&](int which, const void* src, int64_t ld, int64_t rows, int64_t rows_pad, int64_t at) {
     PackJob& j = a.job[which];
-    j = {src, ld, rows, rows_pad, ws + at, rows_pad * p.width_pad * 2, (float*)(ws + p.amax) + which * AMAX_BLOCKS, (float*)(ws + p.unscale) + which,
+    j = {src, ld, rows, rows_pad, ws + at, rows_pad * p.width_pad * 2, by_row ? nullptr : (float*)(ws + p.amax) + which * AMAX_BLOCKS,
+         (float*)(ws + p.unscale) + (by_row ? which * p.rows : which),
          which == 0 && gloss, ((uintptr_t)src & 15) == 0 && ld * e % 16 == 0};
     a.blocks[which] = row_grid(rows_pad, p.width_pad / (j.wide ? 8 : 2));
     return Operand{ws + at, j.plane, p.width_pad * 2, (int32_t)rows_pad, (int32_t)p.width_pad * 2};
@@ -1426,7 +1474,7 @@ int token_loss(int device, int type, const void* x, int64_t ldx, const void* w, 
   g.N = (int32_t)rows;
   g.steps = (int32_t)(p.width_pad / 64);
   if (p.planes == 2) {
-    g.ua = (float*)(ws + p.unscale) + 1;
+    g.ua = (float*)(ws + p.unscale) + rows;
     g.ub = (float*)(ws + p.unscale);
   }
   g.part = (float2*)(ws + p.part);

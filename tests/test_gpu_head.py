@@ -499,3 +499,18 @@ def test_under_autograd():
     # 60 and 432 terms, split products of 2^-21, exponents off by a few of 2^-24: far below 1e-5 of the norm
     assert (x.grad.double() - a.grad).norm() <= 1e-5 * a.grad.norm()
     assert (w.grad.double() - b.grad).norm() <= 1e-5 * b.grad.norm()
+
+
+@pytest.mark.parametrize("rows,vocab,width", [(90, 400, 72), (300, 4099, 333), (1100, 2100, 160)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+def test_padding_may_hold_large_numbers(rows, vocab, width, dtype):
+    x, w, t, gl = make(rows, vocab, width, dtype)
+    keep = t != -100
+    loss, lse = head.token_loss(x, w, t)
+    dx, dw = head.token_loss_grad(x, w, t, lse, gl)
+    x2 = x.clone()
+    x2[~keep] = 1e30
+    loss2, lse2 = head.token_loss(x2, w, t)
+    assert torch.equal(loss2, loss) and torch.equal(lse2[keep], lse[keep])
+    dx2, dw2 = head.token_loss_grad(x2, w, t, lse2, gl)
+    assert torch.equal(dx2, dx) and torch.equal(dw2, dw)
