@@ -497,12 +497,12 @@ struct LossEpilogue {
 #pragma unroll
         for (int r = 0; r < 4; ++r) mx = fmaxf(mx, acc[i][j][r]);
       mx = col_max(mx);
-      const float base = mx == -__builtin_inff() ? 0.0f : mx * LOG2E;
+      const float base = mx == -__builtin_inff() ? 0.0f : mx;
       float sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < T::MI; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) sum += exp2_fast(__builtin_fmaf(acc[i][j][r], LOG2E, -base));
+#pragma unroll  // (the difference first: a rounded mx log2 e is off by more than an exponential's range from 2^31 on)
+        for (int r = 0; r < 4; ++r) sum += exp2_fast((acc[i][j][r] - base) * LOG2E);
       sum = col_sum(sum);
       mxs[j] = mx;
       sums[j] = sum;

@@ -514,3 +514,18 @@ def test_padding_may_hold_large_numbers(rows, vocab, width, dtype):
     assert torch.equal(loss2, loss) and torch.equal(lse2[keep], lse[keep])
     dx2, dw2 = head.token_loss_grad(x2, w, t, lse2, gl)
     assert torch.equal(dx2, dx) and torch.equal(dw2, dw)
+
+
+@pytest.mark.parametrize("rows,vocab,width", [(300, 4099, 333), (1100, 2100, 160)])
+def test_32_bit_positions_of_very_different_sizes(rows, vocab, width):
+    # each position's loss and lse within the bound of its own values (ignored ones' lse too), whatever the others hold
+    x, w, t, _ = make(rows, vocab, width, torch.float32)
+    scale = 10.0 ** torch.linspace(-2, 16, rows, device=DEV)
+    check_loss(x * scale[:, None], w, t)
+
+
+@pytest.mark.parametrize("dtype,scale", [(torch.bfloat16, 1e15), (torch.bfloat16, 1e30), (torch.float16, 1e4), (torch.float32, 1e30)])
+def test_logits_of_any_finite_size(dtype, scale):
+    for rows, vocab, width in ((40, 300, 96), (300, 4099, 333)):
+        x, w, t, _ = make(rows, vocab, width, torch.float32)
+        check_loss((x * scale / 8).to(dtype), w.to(dtype), t)
