@@ -159,7 +159,8 @@ struct Spread {
 
 // A matrix copied into rows of whole K-steps with zeros behind, 32-bit values split into two planes. Bound by its bytes
 // where they are many: 8192 x 1024 bf16 8.2 us, 1000 + 4096 rows of 512 f32 6.3 us; 1023 + 4099 odd rows
-// of 333 f32, two values a thread, 8.0 us (9.0 with each piece's loads behind the last one's store).
+// of 333 f32, two values a thread, 8.0 us (9.0 with each piece's loads behind the last one's store), by the rows' own
+// maxima, read once more for it, 10.2 (a maximum of the whole first: 4.6 + 8.0).
 struct PackJob {
   const void* src;         // null: nothing to do
   int64_t ld;
@@ -1290,9 +1291,13 @@ Plan plan_common(int type, const void* x, int64_t ldx, const void* w, int64_t ld
 Plan plan_loss(int type, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab, int64_t width) {
   Bump b;
   Plan p = plan_common(type, x, ldx, w, ldw, rows, vocab, width, false, b);
-  // up to 32 positions, or a product of about what its launches take (see k_few); about four workgroups a compute unit
-  if (type == PST_F32 && (rows <= 32 || (rows <= 1024 && rows * vocab * width <= 1 << 27))) {
+  // Up to 32 positions of aligned rows, or a product of about what its launches take (see k_few). A call, this kernel and
+  // the split, us: 32 x 64000 x 512 55 and 72, 1 x 64000 x 1024 51 and 166, 64 x 4096 x 1024 23 and 33; of 333 columns, whose
+  // loads are of one value, 1 x 64000 60 and 76, 16 x 64000 90 and 74; 64 x 64000 x 512 89 and 72.
+  const bool aligned = in_place(x, ldx * 4, width * 4) && in_place(w, ldw * 4, width * 4);
+  if (type == PST_F32 && ((rows <= 32 && aligned) || (rows <= 1024 && rows * vocab * width <= 1 << 28))) {
     b = Bump();
+    // about four workgroups a compute unit
     p.few = ceil_div(ceil_div(vocab, 16), 4 * CUS);
     p.part = b.take(ceil_div(vocab, 16 * p.few) * rows * 8);
     p.tlogit = b.take(rows * 4);
