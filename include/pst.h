@@ -258,7 +258,8 @@ int pst_token_loss(int32_t device, int32_t type, const void* d_hidden, int64_t l
  * Gradients of sum_n grad_loss[n] loss[n] for hidden and weight (either may be NULL), of the operands' type, from the
  * lse of pst_token_loss. Ignored positions have zero gradient and add nothing to the weight's, whatever their hidden
  * row holds. A target out of range makes its position's gradient, and the weight's, NaN. rows = 0 writes a zero weight
- * gradient. No atomics: the same inputs give the same bits. PST_F32: hidden (its positions that count), weight and
+ * gradient. No atomics: the same inputs give the same bits. The logits' gradient g_n (softmax - indicator) is held to
+ * 2^-16 of each entry for 16-bit types, whose products with it are summed in 32 bits. PST_F32: hidden (its positions that count), weight and
  * grad_loss are each scaled as a whole and held to 2^-22 of a value and 2^-38 of the largest one, so that values 10^6
  * below the largest of their tensor keep about five digits (the loss scales row by row and has no such limit).
  */

@@ -5,8 +5,8 @@
 //   8-bit scores      s_n s_v sum_k q_nk q_vk, q_nk = rint(x_nk / s_n), s_n = max_k |x_nk| * (1/127)
 //
 // The logits never reach memory: the loss keeps per tile of the vocabulary a running maximum and sum for each
-// row (k_loss) and joins them (k_join); the gradient makes D for a piece of the vocabulary at a time, in 16 bits
-// in a workspace that the last-level cache holds, and multiplies it in both directions from there.
+// row (k_loss) and joins them (k_join); the gradient makes D for a piece of the vocabulary at a time, as sums of two
+// 16-bit floats in a workspace that the last-level cache holds, and multiplies it in both directions from there.
 //
 // 32-bit inputs: each value is split into two 16-bit floats (hi + lo, 22 bits of mantissa) after a scaling by
 // a power of two (of each row for the loss, of the whole tensor for the gradient), and a product is lo hi + hi lo + hi hi on the 16-bit matrix cores: off by about
@@ -63,8 +63,11 @@ __device__ __forceinline__ uint32_t bits16(float v, int type) {  // (type: a con
   return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v);
 }
 __device__ __forceinline__ uint32_t pack2(float a, float b, int type) { return bits16(a, type) | bits16(b, type) << 16; }
-// what a 16-bit float leaves of v
-__device__ __forceinline__ float rest16(float v) { return fabsf(v) <= 65504.0f ? v - (float)(_Float16)v : 0.0f; }
+// what a 16-bit float leaves of v (of an infinity or NaN, and of what rounds to one, nothing)
+__device__ __forceinline__ float rest(float v, int type) {
+  if (type == PST_BF16) return fabsf(v) <= 3.3895313892515355e38f ? v - (float)(__bf16)v : 0.0f;
+  return fabsf(v) <= 65504.0f ? v - (float)(_Float16)v : 0.0f;
+}
 // four neighbours of an output row, `n` of them valid
 __device__ __forceinline__ void store4(void* p, int type, int64_t i, const float* v, int n, bool wide) {
   if (type == PST_F32) {
@@ -165,7 +168,8 @@ struct PackJob {
   const void* src;         // null: nothing to do
   int64_t ld;
   int64_t rows, rows_pad;  // rows beyond `rows` are zeros
-  char* dst;               // 16-bit [planes][rows_pad][width_pad]
+  char* dst;               // 16-bit [planes][rows_pad][width_pad]; null (wide sources): only `halves` are made
+  char* halves;            // f16: two bf16 planes, hi and lo, whose sum is the value (8 + 3 bits); null: not needed
   int64_t plane;           // bytes
   const float* part;       // 32-bit: the tensor's AMAX_BLOCKS maxima; null: each row is split by its own maximum
   float* unscale;          // 32-bit: 2^-e, of the tensor or of each row
@@ -177,7 +181,7 @@ struct PackArgs {
   int32_t blocks[2];  // workgroups of each job; one more makes the scale of the logits' gradient if gloss is set
   int32_t width, width_pad, type;
   Targets targets;
-  // D of 16-bit floats with a short exponent (and of the halves of a split one) is scaled by the power of two that
+  // 32-bit operands: D's halves have a short exponent, and are scaled by the power of two that
   // brings the largest |g_n| to 2^13 ... 2^14; gscale[0] = that power, gscale[1] = its inverse
   const float* gloss;
   int64_t n;
@@ -199,6 +203,16 @@ __device__ __forceinline__ int row_exp(const float* row, int width, int64_t r, c
   const int e = split_exp(m);
   if (at_row.piece == 0) unscale[r] = ldexpf(1.0f, -e);
   return e;
+}
+// pairs of f16 values as pairs of bf16 ones, hi and lo
+template <int N>
+__device__ __forceinline__ void halves_of(const uint32_t (&h)[N], uint32_t (&hi)[N], uint32_t (&lo)[N]) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const float x = (float)__builtin_bit_cast(_Float16, (uint16_t)h[j]), y = (float)__builtin_bit_cast(_Float16, (uint16_t)(h[j] >> 16));
+    hi[j] = pack2(x, y, PST_BF16);
+    lo[j] = pack2(rest(x, PST_BF16), rest(y, PST_BF16), PST_BF16);
+  }
 }
 __global__ __launch_bounds__(256) void k_pack(PackArgs a) {
   __shared__ float sm[4];
@@ -249,10 +263,17 @@ __global__ __launch_bounds__(256) void k_pack(PackArgs a) {
           const int c = c0 + at_row.pieces * 2 * u;
           if (c >= a.width_pad) break;
           const uint32_t x = c < a.width ? raw[u][0] : 0, y = c + 1 < a.width ? raw[u][1] : 0;
+          if (p.halves) {
+            const uint32_t h[1] = {x | y << 16};
+            uint32_t hi[1], lo[1];
+            halves_of(h, hi, lo);
+            *(uint32_t*)(p.halves + (r * a.width_pad + c) * 2) = hi[0];
+            *(uint32_t*)(p.halves + p.plane + (r * a.width_pad + c) * 2) = lo[0];
+          }
           if (f32) {
             const float fx = ldexpf(__uint_as_float(x), e), fy = ldexpf(__uint_as_float(y), e);
             *(uint32_t*)(d + c * 2) = pack2(fx, fy, PST_F16);
-            *(uint32_t*)(d + p.plane + c * 2) = pack2(rest16(fx), rest16(fy), PST_F16);
+            *(uint32_t*)(d + p.plane + c * 2) = pack2(rest(fx, PST_F16), rest(fy, PST_F16), PST_F16);
           } else {
             *(uint32_t*)(d + c * 2) = x | y << 16;
           }
@@ -279,7 +300,15 @@ __global__ __launch_bounds__(256) void k_pack(PackArgs a) {
           for (int j = 0; j < 8; ++j) h[j] = c + j < a.width ? src[j] : 0;
           v = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
         }
-        *(uint4*)d = v;
+        if (p.dst) *(uint4*)d = v;
+        if (p.halves) {
+          const uint32_t h[4] = {v.x, v.y, v.z, v.w};
+          uint32_t hi[4], lo[4];
+          halves_of(h, hi, lo);
+          char* to = p.halves + (r * a.width_pad + c) * 2;
+          *(uint4*)to = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *(uint4*)(to + p.plane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
       } else {
         float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
         const float* src = (const float*)p.src + r * p.ld + c;
@@ -296,7 +325,7 @@ __global__ __launch_bounds__(256) void k_pack(PackArgs a) {
         for (int j = 0; j < 4; ++j) {
           const float x = ldexpf(v[2 * j], e), y = ldexpf(v[2 * j + 1], e);
           hi[j] = pack2(x, y, PST_F16);
-          lo[j] = pack2(rest16(x), rest16(y), PST_F16);  // an infinity or NaN stands in hi alone
+          lo[j] = pack2(rest(x, PST_F16), rest(y, PST_F16), PST_F16);  // an infinity or NaN stands in hi alone
         }
         *(uint4*)d = make_uint4(hi[0], hi[1], hi[2], hi[3]);
         *(uint4*)(d + p.plane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
@@ -313,6 +342,7 @@ struct GemmArgs {
   int32_t blocks;      // workgroups that share the nm nn tiles; those behind them take the `thins` thin tiles of the last rows
   int32_t thins;
   int32_t steps;       // K-steps of the whole range
+  int32_t range, products;  // gradients: K-steps of one product, and how many (see Loop); steps is of all of them
   int32_t gm;
   // unscaling of 32-bit operands (device; null: 1): of each row for the loss, else of the tensor
   const float *ua, *ub;
@@ -322,7 +352,7 @@ struct GemmArgs {
   float* tlogit;       // loss: [N]
   const float *lse, *gloss;
   const float* gscale; // power of two on D (device; null: 1)
-  char* D;             // [planes][rows][ldd] 16-bit
+  char* D;             // [2][rows][ldd] 16-bit: hi and lo
   int64_t dplane, ldd; // bytes, elements
   int32_t v0;
   // matrix outputs
@@ -592,13 +622,16 @@ void launch_join(const JoinArgs& j, hipStream_t st) {
   else hipLaunchKernelGGL(k_join<64>, dim3((unsigned)((j.n + 63) / 64)), dim3(1024), 0, st, j);
 }
 
-// D of one piece of the vocabulary (columns v0 ...; zeros behind the last row and for positions that do not count), in
-// 16 bits: the type the matrix cores take, and the 2^-8 (2^-11) it costs, relative, is what the operands' own rounding did. exp(l - lse) as
-// 2^((l - lse) log2 e): the difference first, so that large logits lose nothing in the product.
-// Stores of 16 bytes a lane. 8192 x 16384 x 1024 bf16: 240 us, 1.14 PFLOP/s.
-template <int E>
+// D of one piece of the vocabulary (columns v0 ...; zeros behind the last row and for positions that do not count), each entry
+// as a sum of two bf16 values, hi + lo: off by 2^-16 of the entry whatever its size, since a bf16 has a float's exponents.
+// One alone would be off by 2^-8, which the sums over thousands of entries of either sign do not lose; f16 ones, scaled to
+// the largest |g|, would drop probabilities and weights far below it. (32-bit operands: two f16, so scaled.) The second
+// half is a second run of the products (see Loop): 8192 x 64003 x 1024 bf16 4.46 ms, with hi alone 2.71.
+// exp(l - lse) as 2^((l - lse) log2 e): the difference first, so that large logits lose nothing in the product. Stores of
+// 16 bytes a lane.
+template <int PLANES>
 struct DlogitEpilogue {
-  static constexpr int TYPE = E == BF16 ? PST_BF16 : PST_F16;
+  static constexpr int TYPE = PLANES == 2 ? PST_F16 : PST_BF16;  // (32-bit operands: scaled)
   struct Inputs {
     int target;  // less v0; a position that does not count has a factor of 0
     float lse, c;
@@ -671,13 +704,11 @@ struct DlogitEpilogue {
 #pragma unroll
           for (int q = 0; q < 2; ++q) w[u][q] = pack2(acc[i + u][j][2 * q], acc[i + u][j][2 * q + 1], TYPE);
         store_pair(to + i * 32, w, p.lane);
-        if (T::PLANES == 2) {
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int q = 0; q < 2; ++q) w[u][q] = pack2(rest16(acc[i + u][j][2 * q]), rest16(acc[i + u][j][2 * q + 1]), PST_F16);
-          store_pair(to + g.dplane + i * 32, w, p.lane);
-        }
+          for (int q = 0; q < 2; ++q) w[u][q] = pack2(rest(acc[i + u][j][2 * q], TYPE), rest(acc[i + u][j][2 * q + 1], TYPE), TYPE);
+        store_pair(to + g.dplane + i * 32, w, p.lane);
       }
     }
   }
@@ -687,9 +718,9 @@ template <int E, class T>
 __global__ __launch_bounds__(T::THREADS, T::WAVES) void k_dlogit(GemmArgs g) {
   extern __shared__ char smem[];
   if ((int)blockIdx.x < g.blocks) {
-    tiles<E, T, true>(g, blockIdx.x, g.blocks, g.nm, g.nn, 0, smem, DlogitEpilogue<E>{});
+    tiles<E, T, true>(g, blockIdx.x, g.blocks, g.nm, g.nn, 0, smem, DlogitEpilogue<T::PLANES>{});
   } else if constexpr (T::HAS_THIN) {
-    tiles<E, typename T::Thin, false>(g, blockIdx.x - g.blocks, 1 << 30, 1, g.thins, g.nm * T::BM, smem, DlogitEpilogue<E>{});
+    tiles<E, typename T::Thin, false>(g, blockIdx.x - g.blocks, 1 << 30, 1, g.thins, g.nm * T::BM, smem, DlogitEpilogue<T::PLANES>{});
   }
 }
 
@@ -817,8 +848,8 @@ __device__ __forceinline__ void grad_tile(const GemmArgs& g, int tile, int nm, i
   const Place<T> p(g, tile, nm, nn, 0, n_base);
   const int s0 = (int)((int64_t)g.steps * p.z / g.nz), s1 = (int)((int64_t)g.steps * (p.z + 1) / g.nz);
   f32x4 acc[T::MI][T::NI];
-  Loop<E, T, true, !DX> loop(smem);
-  loop.begin(g.A, g.B, p.m0, p.n0, s0, s1);
+  Loop<E, T, true, !DX, T::PLANES == 1> loop(smem);
+  loop.begin(g.A, g.B, p.m0, p.n0, s0, s1, g.range, g.products);
   loop.run(acc);
   if (DX || g.part_out) {
     store_part<T>(acc, g, p);
@@ -1226,17 +1257,7 @@ hipError_t launch_gemm(int kind, int elem, int tile, GemmArgs g, hipStream_t st)
          : elem == BF16 ? launch_elem<BF16>(kind, tile, g, grid, st)
                         : launch_elem<F16>(kind, tile, g, grid, st);
 }
-template <int E>
-hipError_t launch_grads_elem(int tile, const GradArgs& g, int64_t grid, hipStream_t st) {
-  if constexpr (E == F16) {
-    if (tile == SPLIT128) return launch(k_grads<E, S128>, grid, S128::THREADS, S128::LDS, st, g);
-    if (tile == SPLIT64) return launch(k_grads<E, S64>, grid, S64::THREADS, S64::LDS, st, g);
-  }
-  return tile == TILE256   ? launch(k_grads<E, T256>, grid, T256::THREADS, T256::LDS, st, g)
-         : tile == TILE128 ? launch(k_grads<E, T128>, grid, T128::THREADS, T128::LDS, st, g)
-                           : launch(k_grads<E, T64>, grid, T64::THREADS, T64::LDS, st, g);
-}
-hipError_t launch_grads(int elem, int tile, GradArgs g, bool dx, bool dw, hipStream_t st) {
+hipError_t launch_grads(int tile, GradArgs g, bool dx, bool dw, hipStream_t st) {
   int64_t grid = 0;
   for (int i = 0; i < 2; ++i) {
     GemmArgs& q = i ? g.dw : g.dx;
@@ -1250,17 +1271,22 @@ hipError_t launch_grads(int elem, int tile, GradArgs g, bool dx, bool dw, hipStr
     g.blocks[i] = (int32_t)blocks;
     g.blocks[2 + i] = (int32_t)thins;
   }
-  return elem == BF16 ? launch_grads_elem<BF16>(tile, g, grid, st) : launch_grads_elem<F16>(tile, g, grid, st);
+  return tile == SPLIT128  ? launch(k_grads<F16, S128>, grid, S128::THREADS, S128::LDS, st, g)
+         : tile == SPLIT64 ? launch(k_grads<F16, S64>, grid, S64::THREADS, S64::LDS, st, g)
+         : tile == TILE256 ? launch(k_grads<BF16, T256>, grid, T256::THREADS, T256::LDS, st, g)
+         : tile == TILE128 ? launch(k_grads<BF16, T128>, grid, T128::THREADS, T128::LDS, st, g)
+                           : launch(k_grads<BF16, T64>, grid, T64::THREADS, T64::LDS, st, g);
 }
 
 // What a call on [rows, width] x [vocab, width] needs of its workspace; the same for the query and for the call.
 struct Plan {
   int type, elem, planes;
+  int products;                                  // of each gradient (see Loop)
   int64_t rows, vocab, width, width_pad, rows_pad;
   bool pack_x, pack_w;
   int64_t amax = 0, unscale = 0, x = 0, w = 0;   // offsets
   int64_t part = 0, tlogit = 0;                  // loss
-  int64_t gscale = 0, D = 0, dxp = 0, dwp = 0;   // gradient
+  int64_t gscale = 0, xh = 0, wh = 0, D = 0, dxp = 0, dwp = 0;  // gradient
   int64_t few = 0;                               // k_few: 16-row blocks a workgroup
   int64_t piece = 0;                             // vocabulary rows of a piece
   int tile = 0, zx = 1, zw = 1;                  // of the two gradients' launch
@@ -1271,6 +1297,7 @@ Plan plan_common(int type, const void* x, int64_t ldx, const void* w, int64_t ld
   p.type = type;
   p.elem = type == PST_BF16 ? BF16 : F16;
   p.planes = type == PST_F32 ? 2 : 1;
+  p.products = type == PST_BF16 ? 2 : type == PST_F16 ? 3 : 1;
   p.rows = rows;
   p.vocab = vocab;
   p.width = width;
@@ -1315,13 +1342,13 @@ Plan plan_loss(int type, const void* x, int64_t ldx, const void* w, int64_t ldw,
 void split_grads(Plan& p, int64_t nv, bool pieces) {
   struct Last {
     int64_t rows = -1, nv, width;
-    int planes, tile, zx, zw;
+    int products, tile, zx, zw;
     bool pieces;
   };
   thread_local Last last;
-  if (last.rows != p.rows || last.nv != nv || last.width != p.width || last.planes != p.planes || last.pieces != pieces) {
+  if (last.rows != p.rows || last.nv != nv || last.width != p.width || last.products != p.products || last.pieces != pieces) {
     constexpr int Z[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
-    const int64_t sx = ceil_div(nv, 64), sw = ceil_div(p.rows, 64), least = p.planes == 2 ? 2 : 4;
+    const int64_t sx = p.products * ceil_div(nv, 64), sw = p.products * ceil_div(p.rows, 64), least = p.planes == 2 ? 2 : 4;
     double best = 1e30;
     for (int t = p.planes == 2 ? SPLIT128 : TILE256; t >= (p.planes == 2 ? SPLIT64 : TILE64); --t) {
       const int64_t thin_x = thin_rows(p.rows, t), thin_w = thin_rows(nv, t);
@@ -1344,7 +1371,7 @@ void split_grads(Plan& p, int64_t nv, bool pieces) {
     last.rows = p.rows;
     last.nv = nv;
     last.width = p.width;
-    last.planes = p.planes;
+    last.products = p.products;
     last.pieces = pieces;
   }
   p.tile = last.tile;
@@ -1357,14 +1384,20 @@ constexpr int64_t PIECE_BYTES = 288ll << 20, PIECE_LEAST = 4096;
 Plan plan_grad(int type, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab, int64_t width) {
   Bump b;
   Plan p = plan_common(type, x, ldx, w, ldw, rows, vocab, width, true, b);
-  p.gscale = b.take(8);
+  if (type == PST_F32) p.gscale = b.take(8);
+  if (type == PST_F16) {
+    p.xh = b.take(p.rows_pad * p.width_pad * 4);
+    p.wh = b.take(vocab * p.width_pad * 4);
+  }
   const int64_t drows = up(rows, 256);
-  int64_t most = std::max<int64_t>(PIECE_LEAST, PIECE_BYTES / (drows * 2 * p.planes) / 256 * 256);
-  // several pieces: of a size that gives dW's largest tiles in whole rounds, where that is not much smaller
-  const int64_t round = CUS / std::max<int64_t>(1, ceil_div(p.width_pad, 256)) * 256;
-  if (vocab > most && round > 0 && most >= round) most = most / round * round;
+  int64_t most = std::max<int64_t>(PIECE_LEAST, PIECE_BYTES / (drows * 4) / 256 * 256);
+  // several pieces: of a size that gives both gradients' largest tiles in whole rounds, where that is not much smaller
+  const int64_t across = ceil_div(p.width_pad, 256), round = CUS / across * 256;
+  const int64_t first = (CUS - across * (drows / 256) % CUS) / across * 256;
+  if (vocab > most && round > 0 && first > 0 && most >= first && first + (most - first) / round * round >= most / 2)
+    most = first + (most - first) / round * round;
   p.piece = vocab > most ? most : up(vocab, 256);
-  p.D = b.take(drows * p.piece * 2 * p.planes);
+  p.D = b.take(drows * p.piece * 4);
   split_grads(p, std::min(p.piece, vocab), vocab > p.piece);
   p.dxp = b.take(p.zx * rows * p.width_pad * 4);
   if (p.zw > 1) p.dwp = b.take(p.zw * vocab * p.width_pad * 4);
@@ -1417,18 +1450,21 @@ int operands(const Plan& p, const void* x, int64_t ldx, const void* w, int64_t l
     HEADCHK(hipGetLastError());
   }
   const int e = size_of(p.type);
-  auto job = [&](int which, const void* src, int64_t ld, int64_t rows, int64_t rows_pad, int64_t at) {
+  const bool halves = gloss && p.type == PST_F16;
+  auto job = [&](int which, const void* src, int64_t ld, int64_t rows, int64_t rows_pad, int64_t at, int64_t half) {
     PackJob& j = a.job[which];
-    j = {src, ld, rows, rows_pad, ws + at, rows_pad * p.width_pad * 2, by_row ? nullptr : (float*)(ws + p.amax) + which * AMAX_BLOCKS,
+    j = {src, ld, rows, rows_pad, at < 0 ? nullptr : ws + at, half < 0 ? nullptr : ws + half, rows_pad * p.width_pad * 2, by_row ? nullptr : (float*)(ws + p.amax) + which * AMAX_BLOCKS,
          (float*)(ws + p.unscale) + (by_row ? which * p.rows : which),
          which == 0 && gloss, ((uintptr_t)src & 15) == 0 && ld * e % 16 == 0};
     a.blocks[which] = row_grid(rows_pad, p.width_pad / (j.wide ? 8 : 2));
     return Operand{ws + at, j.plane, p.width_pad * 2, (int32_t)rows_pad, (int32_t)p.width_pad * 2};
   };
-  *X = p.pack_x ? job(0, x, ldx, p.rows, p.rows_pad, p.x) : Operand{(const char*)x, 0, ldx * e, (int32_t)p.rows, (int32_t)p.width * e};
-  *W = p.pack_w ? job(1, w, ldw, p.vocab, p.vocab, p.w) : Operand{(const char*)w, 0, ldw * e, (int32_t)p.vocab, (int32_t)p.width * e};
+  *X = p.pack_x ? job(0, x, ldx, p.rows, p.rows_pad, p.x, halves ? p.xh : -1)
+                : Operand{(const char*)x, 0, ldx * e, (int32_t)p.rows, (int32_t)p.width * e};
+  if (p.pack_w || halves) *W = job(1, w, ldw, p.vocab, p.vocab, p.pack_w ? p.w : -1, halves ? p.wh : -1);
+  if (!p.pack_w) *W = Operand{(const char*)w, 0, ldw * e, (int32_t)p.vocab, (int32_t)p.width * e};
   int blocks = a.blocks[0] + a.blocks[1];
-  if (gloss && p.type != PST_BF16) {
+  if (gloss && p.type == PST_F32) {
     a.gloss = gloss;
     a.n = p.rows;
     a.gscale = (float*)(ws + p.gscale);
@@ -1518,13 +1554,16 @@ int token_loss_grad(int device, int type, const void* x, int64_t ldx, const void
   static const float none = 0.0f;  // (never read: there are no rows)
   rc = operands(q, x, ldx, w, ldw, t, rows ? gloss : &none, ws, st, &X, &W);
   if (rc != PST_OK) return rc;
-  const float* gs = p.type == PST_BF16 ? nullptr : (float*)(ws + p.gscale);
+  const float* gs = p.type == PST_F32 ? (float*)(ws + p.gscale) : nullptr;
   const float* ungs = gs ? gs + 1 : nullptr;
   const float* ux = p.planes == 2 ? (float*)(ws + p.unscale) : nullptr;
   const float* uw = p.planes == 2 ? ux + 1 : nullptr;
   char* D = ws + p.D;
   const int64_t drows = up(std::max<int64_t>(rows, 1), 256);
   const bool need_dx = dx && rows;
+  // what the gradients' products read
+  const Operand Xh = p.type == PST_F16 ? Operand{ws + p.xh, X.rows * X.ld, X.ld, X.rows, X.bytes} : X;
+  const Operand Wh = p.type == PST_F16 ? Operand{ws + p.wh, vocab * X.ld, X.ld, (int32_t)vocab, X.bytes} : W;
   for (int64_t v0 = 0; v0 < vocab; v0 += p.piece) {
     const int64_t nv = std::min(p.piece, vocab - v0), ldd = up(nv, 256);
     const Operand dop{D, drows * ldd * 2, ldd * 2, (int32_t)drows, (int32_t)ldd * 2};
@@ -1532,7 +1571,7 @@ int token_loss_grad(int device, int type, const void* x, int64_t ldx, const void
     Wv.p += v0 * W.ld;
     Wv.rows = (int32_t)nv;
     GemmArgs g{};
-      g.A = Wv;
+    g.A = Wv;
     g.B = X;
     g.M = (int32_t)nv;
     g.N = (int32_t)rows;
@@ -1547,21 +1586,26 @@ int token_loss_grad(int device, int type, const void* x, int64_t ldx, const void
     g.dplane = dop.plane;
     g.ldd = ldd;
     g.v0 = (int32_t)v0;
-    if (rows) HEADCHK(launch_gemm(DLOGIT, p.elem, tile_for(nv, rows, g.steps, p.planes, p.planes), g, st));
+    if (rows) HEADCHK(launch_gemm(DLOGIT, p.elem, tile_for(nv, rows, g.steps, p.planes, 4), g, st));
     GradArgs b{};
-    b.dx.A = Wv;
+    b.dx.A = Wh;
+    b.dx.A.p += v0 * Wh.ld;
+    b.dx.A.rows = (int32_t)nv;
     b.dx.B = b.dw.B = dop;
     b.dx.M = b.dw.M = (int32_t)width;
     b.dx.N = (int32_t)rows;
-    b.dx.steps = (int32_t)ceil_div(nv, 64);
+    b.dx.range = (int32_t)ceil_div(nv, 64);
+    b.dw.range = (int32_t)ceil_div(rows, 64);
+    b.dx.products = b.dw.products = p.products;
+    b.dx.steps = b.dx.range * p.products;
+    b.dw.steps = b.dw.range * p.products;
     b.dx.nz = p.zx;
     b.dx.part_out = (float*)(ws + p.dxp);
     b.dx.ldp = b.dw.ldp = p.width_pad;
     b.dx.zstride = rows * p.width_pad;
     b.dx.add = v0 > 0;
-    b.dw.A = X;
+    b.dw.A = Xh;
     b.dw.N = (int32_t)nv;
-    b.dw.steps = (int32_t)ceil_div(rows, 64);
     b.dw.nz = p.zw;
     b.dw.ua = ungs;
     b.dw.ub = ux;
@@ -1574,7 +1618,7 @@ int token_loss_grad(int device, int type, const void* x, int64_t ldx, const void
       b.dw.part_out = (float*)(ws + p.dwp);
       b.dw.zstride = vocab * p.width_pad;
     }
-    HEADCHK(launch_grads(p.elem, p.tile, b, need_dx, dw != nullptr, st));
+    HEADCHK(launch_grads(p.tile, b, need_dx, dw != nullptr, st));
   }
   FinishArgs f{};
   f.width = (int32_t)width;

@@ -137,21 +137,26 @@ struct Stager {
       }
     }
   }
-  // K-step `step` goes to the LDS tile at `lds` (its lo plane to the tile behind), by one(0) ... one(NI - 1) a plane
-  __device__ __forceinline__ void aim(int step, uint32_t lds, int lane, int wave) {
+  // K-step `step` goes to the LDS tile at `lds` (its lo plane to the tile behind), by one(0) ... one(NI - 1) a plane.
+  // AGAIN: the K range comes more than once, from plane `q`
+  template <bool AGAIN>
+  __device__ __forceinline__ void aim(int step, int q, uint32_t lds, int lane, int wave) {
     constexpr int WHOLE = COLS ? 64 : STEP;
+    if (AGAIN && left < WHOLE) shift<-1>(left, lane, wave);  // back from the last step of the range
     src = base + (COLS ? (int64_t)min(step * 64, k_bytes - 1) * ld : (int64_t)step * STEP);
+    if (AGAIN) src += q * plane;
     left = COLS ? k_bytes - step * 64 : k_bytes - step * STEP;
-    if (left < WHOLE) shift(left, lane, wave);  // the last step of all
+    if (left < WHOLE) shift<1>(left, lane, wave);  // the last step of the range
     to = __builtin_amdgcn_readfirstlane(lds + (uint32_t)wave * (NI * 1024));
   }
-  // a K-step of which `valid` (k-rows or bytes) exist: what lies behind reads the last of them
+  // a K-step of which `valid` (k-rows or bytes) exist: what lies behind reads the last of them (SIGN -1: no more)
+  template <int SIGN>
   __device__ __forceinline__ void shift(int valid, int lane, int wave) {
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
       const int r = (wave * NI + j) * PER + lane / (RT / 16);
       const int c = lane % (RT / 16);
-      off[j] -= COLS ? (uint32_t)((int64_t)max(0, r - max(0, valid - 1)) * ld) : (uint32_t)max(0, ((c ^ (r >> 1 & 7)) << 4) - (valid - 16));
+      off[j] -= SIGN * (COLS ? (uint32_t)((int64_t)max(0, r - max(0, valid - 1)) * ld) : (uint32_t)max(0, ((c ^ (r >> 1 & 7)) << 4) - (valid - 16)));
     }
   }
   __device__ __forceinline__ void one(int j) const {
@@ -205,7 +210,10 @@ struct Tile {
 // Measured at 8192 x 16128 x 1024 bf16 (dW, 210 - 216 us as it is): K-steps of 64 bytes in rings of 3, 4 and 5 stages
 // 226 - 228 (twice the barriers; deeper prefetch gains nothing), two 256 x 128 workgroups a unit 252 (half as much again
 // through LDS), four waves of 128 x 128 224, blocks of 32 x 32 227, loads in one burst 222.
-template <int E, class T, bool ACOLS, bool BCOLS>
+// HALVES: operands that are sums of two planes, hi and lo, come in `products` runs through the same `range` of K-steps: of B alone
+// lo, hi (2 products); of both hi lo, lo hi, hi hi (3; lo lo, 2^-16 of the whole, is left out). The small ones first. More
+// of the K loop, where both planes in LDS would take as much room as a tile twice as large.
+template <int E, class T, bool ACOLS, bool BCOLS, bool HALVES = false>
 struct Loop {
   typedef typename Mma<E>::Acc Acc;
   static constexpr int HI = T::MI / 2;
@@ -222,6 +230,7 @@ struct Loop {
   uint32_t lds0;
   int lane, wave;
   int step, total;  // step: what is loaded next
+  int range, products;
 
   __device__ __forceinline__ explicit Loop(const char* smem_) : smem(smem_), lds0(lds_addr(smem_)) {
     lane = threadIdx.x & 63;
@@ -231,8 +240,11 @@ struct Loop {
   }
   __device__ __forceinline__ void aim(int stage) {
     const uint32_t to = lds0 + stage * T::STAGE;
-    sa.aim(step, to, lane, wave);
-    sb.aim(step, to + T::BM * STEP * PL, lane, wave);
+    int c = 0;
+    if (HALVES) c = step >= 2 * range ? 2 : step >= range ? 1 : 0;
+    const int s = HALVES ? step - c * range : step;
+    sa.template aim<HALVES>(s, products == 3 && c == 1, to, lane, wave);
+    sb.template aim<HALVES>(s, products > 1 && c == 0, to + T::BM * STEP * PL, lane, wave);
     ++step;
   }
   __device__ __forceinline__ void load(int i) const {
@@ -244,12 +256,14 @@ struct Loop {
 #pragma unroll
     for (int i = 0; i < L; ++i) load(i);
   }
-  // K-steps [from, to); all waves have left the stages
-  __device__ __forceinline__ void begin(const Operand& A, const Operand& B, int m0, int n0, int from, int to) {
+  // K-steps [from, to) of all products'; all waves have left the stages
+  __device__ __forceinline__ void begin(const Operand& A, const Operand& B, int m0, int n0, int from, int to, int range_ = 0, int products_ = 1) {
     sa.init(A, m0, lane, wave);
     sb.init(B, n0, lane, wave);
     step = from;
     total = to - from;
+    range = range_;
+    products = products_;
     for (int t = 0; t < min(S, total); ++t) issue(t);
   }
 

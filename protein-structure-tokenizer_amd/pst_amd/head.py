@@ -148,7 +148,7 @@ def token_loss_grad(hidden, weight, targets, lse, grad_loss, *, ignore_index=-10
     """Gradients of sum_n grad_loss[n] loss[n]: (for hidden, for weight), of their type; None where not needed.
 
     `lse` [N] float32 from `token_loss`, `grad_loss` [N] float32. Positions whose target is `ignore_index` have zero
-    gradient and add nothing to the weight's, whatever their hidden row holds; a target out of range gives NaN.
+    gradient and add nothing to the weight's, whatever their hidden row holds; a target out of range gives NaN. The logits' gradient is held to 2^-16 of each entry for 16-bit types.
     float16: scale the loss, since gradients below 6e-8 vanish in the type."""
     torch = _torch()
     device, code, x, ldx, w, ldw = _head(torch, hidden, weight)
