@@ -242,7 +242,8 @@ const char* pst_head_error(void);
 /*
  * Softmax cross entropy of each position over the vocabulary, without the logits in memory:
  *   lse[n] = log sum_v exp(<hidden[n], weight[v]>),  loss[n] = lse[n] - <hidden[n], weight[targets[n]]>
- *   hidden [rows, width], weight [vocab, width]  of `type` (products of 16-bit types are exact, sums 32-bit)
+ *   hidden [rows, width], weight [vocab, width]  of `type` (products of 16-bit types are exact, those of
+ *                   32-bit ones rounded to 32 bits, and so are all sums)
  *   targets [rows]  int32 or int64 (target_bits; uint32 token ids below 2^31 are int32 ids). Positions whose target is
  *                   `ignore` have loss 0; a target outside [0, vocab) that is not `ignore` gives loss NaN.
  *   loss, lse [rows] f32 (lse of ignored positions too)
@@ -259,9 +260,8 @@ int pst_token_loss(int32_t device, int32_t type, const void* d_hidden, int64_t l
  * lse of pst_token_loss. Ignored positions have zero gradient and add nothing to the weight's, whatever their hidden
  * row holds. A target out of range makes its position's gradient, and the weight's, NaN. rows = 0 writes a zero weight
  * gradient. No atomics: the same inputs give the same bits. The logits' gradient g_n (softmax - indicator) is held to
- * 2^-16 of each entry for 16-bit types, whose products with it are summed in 32 bits. PST_F32: hidden (its positions that count), weight and
- * grad_loss are each scaled as a whole and held to 2^-22 of a value and 2^-38 of the largest one, so that values 10^6
- * below the largest of their tensor keep about five digits (the loss scales row by row and has no such limit).
+ * 2^-16 of each entry for 16-bit types, whose products with it are summed in 32 bits. PST_F32: 32-bit
+ * products throughout.
  */
 int64_t pst_token_loss_grad_workspace(int32_t type, const void* d_hidden, int64_t ld_hidden, const void* d_weight, int64_t ld_weight,
                                       int64_t rows, int64_t vocab, int64_t width);

@@ -8,9 +8,10 @@
 // row (k_loss) and joins them (k_join); the gradient makes D for a piece of the vocabulary at a time, as sums of two
 // 16-bit floats in a workspace that the last-level cache holds, and multiplies it in both directions from there.
 //
-// 32-bit inputs: each value is split into two 16-bit floats (hi + lo, 22 bits of mantissa) after a scaling by
-// a power of two (of each row for the loss, of the whole tensor for the gradient), and a product is lo hi + hi lo + hi hi on the 16-bit matrix cores: off by about
-// 2^-22 of the operands' product, at 0.41 - 0.49 PFLOP/s of such products where the 32-bit instructions reach 0.154.
+// 32-bit inputs are multiplied by the 32-bit matrix instructions (0.157 PFLOP/s at most): every value keeps its 24 bits and
+// its exponent, whatever else its row or tensor holds, and an infinity in one place stays there. Splits into 16-bit
+// floats are two to three times as fast and have neither: their halves share a scale, and infinity times a half that is
+// zero is NaN.
 //
 // Times in this file: one MI355X, median of 40 - 600 calls in a row.
 #include <hip/hip_runtime.h>
@@ -39,17 +40,7 @@ struct T256 : Tile<256, 256, 2, 4, 2> {
   static constexpr bool HAS_THIN = true;
   struct Thin : Tile<64, 64, 2, 4, 4> {};
 };
-// of split 32-bit values: a K-step brings both planes of both operands, and three products are made of them
-struct S64 : Tile<64, 64, 2, 2, 2, 2> {
-  static constexpr bool HAS_THIN = false;
-};
-struct S128 : Tile<128, 128, 2, 4, 2, 2> {
-  static constexpr bool HAS_THIN = true;
-  struct Thin : Tile<64, 64, 2, 4, 2, 2> {};
-};
-
 constexpr float LOG2E = 1.44269504088896340736f;
-constexpr int AMAX_BLOCKS = 256;
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -63,11 +54,8 @@ __device__ __forceinline__ uint32_t bits16(float v, int type) {  // (type: a con
   return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v);
 }
 __device__ __forceinline__ uint32_t pack2(float a, float b, int type) { return bits16(a, type) | bits16(b, type) << 16; }
-// what a 16-bit float leaves of v (of an infinity or NaN, and of what rounds to one, nothing)
-__device__ __forceinline__ float rest(float v, int type) {
-  if (type == PST_BF16) return fabsf(v) <= 3.3895313892515355e38f ? v - (float)(__bf16)v : 0.0f;
-  return fabsf(v) <= 65504.0f ? v - (float)(_Float16)v : 0.0f;
-}
+// what a bf16 leaves of v (of an infinity or NaN, and of what rounds to one, nothing)
+__device__ __forceinline__ float rest(float v) { return fabsf(v) <= 3.3895313892515355e38f ? v - (float)(__bf16)v : 0.0f; }
 // four neighbours of an output row, `n` of them valid
 __device__ __forceinline__ void store4(void* p, int type, int64_t i, const float* v, int n, bool wide) {
   if (type == PST_F32) {
@@ -103,49 +91,6 @@ __device__ __forceinline__ int target_of(const Targets& t, int64_t n, bool& coun
   return counts && v >= 0 && v < t.vocab ? (int)v : -1;
 }
 
-// ------------------------------------------------------------------ 32-bit operands: scaling and splitting
-__device__ __forceinline__ float finite_abs(float v) {
-  v = fabsf(v);
-  return v <= 3.4028234663852886e38f ? v : 0.0f;
-}
-// 2^e with max |x| 2^e in [2^13, 2^14): both halves of a product stay inside the 16-bit range
-__device__ __forceinline__ int split_exp(float amax) { return amax > 0.0f ? 13 - ilogbf(amax) : 0; }
-
-struct AmaxArgs {
-  const float* p[2];
-  int64_t ld[2];
-  int64_t rows[2];
-  int32_t width;
-  float* part;  // [2][AMAX_BLOCKS]
-  Targets targets;
-};
-// The gradient's operands: the largest finite magnitude of each of two matrices, in AMAX_BLOCKS parts; a wave a row. Rows of
-// the first whose position does not count are left out (k_pack makes them zeros). A pass of its own, since the products
-// sum over rows: a split by the largest value of each row would have to put the rows' scales into D. 1000 + 4096 rows of
-// 512: 4.0 us.
-__global__ __launch_bounds__(1024) void k_amax(AmaxArgs a) {
-  const int t = blockIdx.x / AMAX_BLOCKS, b = blockIdx.x % AMAX_BLOCKS;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  float m = 0.0f;
-  for (int64_t r = b * 16 + wave; r < a.rows[t]; r += AMAX_BLOCKS * 16) {
-    bool counts = true;
-    if (t == 0) (void)target_of(a.targets, r, counts);
-    if (!counts) continue;
-    const float* row = a.p[t] + r * a.ld[t];
-#pragma unroll 8
-    for (int k = lane; k < a.width; k += 64) m = fmaxf(m, finite_abs(row[k]));
-  }
-#pragma unroll
-  for (int s = 32; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
-  __shared__ float sm[16];
-  if (lane == 0) sm[wave] = m;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < 16; ++w) m = fmaxf(m, sm[w]);
-    a.part[t * AMAX_BLOCKS + b] = m;
-  }
-}
-
 // The pieces of a matrix's rows over workgroups of 256 threads, without a division: a power of two of threads, at most 64,
 // takes a row.
 struct Spread {
@@ -160,50 +105,22 @@ struct Spread {
   }
 };
 
-// A matrix copied into rows of whole K-steps with zeros behind, 32-bit values split into two planes. Bound by its bytes
-// where they are many: 8192 x 1024 bf16 8.2 us, 1000 + 4096 rows of 512 f32 6.3 us; 1023 + 4099 odd rows
-// of 333 f32, two values a thread, 8.0 us (9.0 with each piece's loads behind the last one's store), by the rows' own
-// maxima, read once more for it, 10.2 (a maximum of the whole first: 4.6 + 8.0).
+// A matrix copied into rows of whole K-steps with zeros behind. Bound by its bytes where they are many.
 struct PackJob {
-  const void* src;         // null: nothing to do
-  int64_t ld;
+  const char* src;
+  int64_t ld;              // bytes
   int64_t rows, rows_pad;  // rows beyond `rows` are zeros
-  char* dst;               // 16-bit [planes][rows_pad][width_pad]; null (wide sources): only `halves` are made
+  char* dst;               // [rows_pad][width_pad]; null (wide sources): only `halves` are made
   char* halves;            // f16: two bf16 planes, hi and lo, whose sum is the value (8 + 3 bits); null: not needed
-  int64_t plane;           // bytes
-  const float* part;       // 32-bit: the tensor's AMAX_BLOCKS maxima; null: each row is split by its own maximum
-  float* unscale;          // 32-bit: 2^-e, of the tensor or of each row
   int32_t zero_rows;       // rows whose position does not count are zeros
   int32_t wide;            // the source allows 16-byte loads
 };
 struct PackArgs {
   PackJob job[2];
-  int32_t blocks[2];  // workgroups of each job; one more makes the scale of the logits' gradient if gloss is set
-  int32_t width, width_pad, type;
+  int32_t blocks[2];       // workgroups of each job
+  int32_t bytes, bytes_pad, type;  // of a row
   Targets targets;
-  // 32-bit operands: D's halves have a short exponent, and are scaled by the power of two that
-  // brings the largest |g_n| to 2^13 ... 2^14; gscale[0] = that power, gscale[1] = its inverse
-  const float* gloss;
-  int64_t n;
-  float* gscale;
 };
-__device__ __forceinline__ float block_max(float m, float* sm) {
-#pragma unroll
-  for (int s = 32; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
-  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
-  __syncthreads();
-  return fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-}
-// a row's exponent, by the neighbouring threads that have it
-__device__ __forceinline__ int row_exp(const float* row, int width, int64_t r, const Spread& at_row, float* unscale) {
-  float m = 0.0f;
-#pragma unroll 8
-  for (int k = at_row.piece; k < width; k += at_row.pieces) m = fmaxf(m, finite_abs(row[k]));
-  for (int s = at_row.pieces / 2; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
-  const int e = split_exp(m);
-  if (at_row.piece == 0) unscale[r] = ldexpf(1.0f, -e);
-  return e;
-}
 // pairs of f16 values as pairs of bf16 ones, hi and lo
 template <int N>
 __device__ __forceinline__ void halves_of(const uint32_t (&h)[N], uint32_t (&hi)[N], uint32_t (&lo)[N]) {
@@ -211,124 +128,72 @@ __device__ __forceinline__ void halves_of(const uint32_t (&h)[N], uint32_t (&hi)
   for (int j = 0; j < N; ++j) {
     const float x = (float)__builtin_bit_cast(_Float16, (uint16_t)h[j]), y = (float)__builtin_bit_cast(_Float16, (uint16_t)(h[j] >> 16));
     hi[j] = pack2(x, y, PST_BF16);
-    lo[j] = pack2(rest(x, PST_BF16), rest(y, PST_BF16), PST_BF16);
+    lo[j] = pack2(rest(x), rest(y), PST_BF16);
   }
 }
+// four bytes of a row from byte c, zeros behind the last: a 32-bit value or two 16-bit ones, without a branch
+__device__ __forceinline__ uint32_t load_word(const char* row, int c, int bytes, bool f32) {
+  if (f32) {
+    const uint32_t v = *(const uint32_t*)(row + min(c, bytes - 4));
+    return c < bytes ? v : 0;
+  }
+  const uint32_t x = *(const uint16_t*)(row + min(c, bytes - 2)), y = *(const uint16_t*)(row + min(c + 2, bytes - 2));
+  return (c < bytes ? x : 0) | (c + 2 < bytes ? y : 0) << 16;
+}
 __global__ __launch_bounds__(256) void k_pack(PackArgs a) {
-  __shared__ float sm[4];
   const int which = (int)blockIdx.x < a.blocks[0] ? 0 : 1;
   const int block = (int)blockIdx.x - (which ? a.blocks[0] : 0);
-  if (which && block >= a.blocks[1]) {
-    float m = 0.0f;
-    for (int64_t i = threadIdx.x; i < a.n; i += 256) {
-      bool counts;
-      (void)target_of(a.targets, i, counts);
-      if (counts) m = fmaxf(m, finite_abs(a.gloss[i]));
-    }
-    m = block_max(m, sm);
-    if (threadIdx.x == 0) {
-      const int e = max(-100, min(100, split_exp(m)));
-      a.gscale[0] = ldexpf(1.0f, e);
-      a.gscale[1] = ldexpf(1.0f, -e);
-    }
-    return;
-  }
   const PackJob& p = a.job[which];
   const bool f32 = a.type == PST_F32;
-  int e = 0;
-  const bool by_row = f32 && !p.part;
-  if (f32 && !by_row) {
-    e = split_exp(block_max(p.part[threadIdx.x], sm));
-    if (block == 0 && threadIdx.x == 0) *p.unscale = ldexpf(1.0f, -e);
-  }
-  if (!p.wide) {  // two neighbours a thread; four pieces' loads before the first store
-    const Spread at_row(block, a.blocks[which], a.width_pad / 2);
+  if (!p.wide) {  // four bytes a thread; four pieces' loads before the first store
+    const Spread at_row(block, a.blocks[which], a.bytes_pad / 4);
     for (int64_t r = at_row.row; r < p.rows_pad; r += at_row.rows) {
       bool keep = r < p.rows;
       if (keep && p.zero_rows) (void)target_of(a.targets, r, keep);
-      const int64_t from = min(r, p.rows - 1) * p.ld;
-      if (by_row && keep) e = row_exp((const float*)p.src + from, a.width, r, at_row, p.unscale);
-      char* d = p.dst + r * a.width_pad * 2;
-      for (int c0 = at_row.piece * 2; c0 < a.width_pad; c0 += at_row.pieces * 8) {
-        uint32_t raw[4][2];
+      const char* row = p.src + r * p.ld;
+      const int64_t to = r * a.bytes_pad;
+      for (int c0 = at_row.piece * 4; c0 < a.bytes_pad; c0 += at_row.pieces * 16) {
+        uint32_t v[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int64_t i = from + min(c0 + at_row.pieces * 2 * u + j, a.width - 1);
-            raw[u][j] = !keep ? 0u : f32 ? ((const uint32_t*)p.src)[i] : (uint32_t)((const uint16_t*)p.src)[i];
-          }
+        for (int u = 0; u < 4; ++u) v[u] = keep ? load_word(row, c0 + at_row.pieces * 4 * u, a.bytes, f32) : 0;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          const int c = c0 + at_row.pieces * 2 * u;
-          if (c >= a.width_pad) break;
-          const uint32_t x = c < a.width ? raw[u][0] : 0, y = c + 1 < a.width ? raw[u][1] : 0;
+          const int c = c0 + at_row.pieces * 4 * u;
+          if (c >= a.bytes_pad) break;
+          *(uint32_t*)(p.dst + to + c) = v[u];
           if (p.halves) {
-            const uint32_t h[1] = {x | y << 16};
+            const uint32_t h[1] = {v[u]};
             uint32_t hi[1], lo[1];
             halves_of(h, hi, lo);
-            *(uint32_t*)(p.halves + (r * a.width_pad + c) * 2) = hi[0];
-            *(uint32_t*)(p.halves + p.plane + (r * a.width_pad + c) * 2) = lo[0];
-          }
-          if (f32) {
-            const float fx = ldexpf(__uint_as_float(x), e), fy = ldexpf(__uint_as_float(y), e);
-            *(uint32_t*)(d + c * 2) = pack2(fx, fy, PST_F16);
-            *(uint32_t*)(d + p.plane + c * 2) = pack2(rest(fx, PST_F16), rest(fy, PST_F16), PST_F16);
-          } else {
-            *(uint32_t*)(d + c * 2) = x | y << 16;
+            *(uint32_t*)(p.halves + to + c) = hi[0];
+            *(uint32_t*)(p.halves + p.rows_pad * a.bytes_pad + to + c) = lo[0];
           }
         }
       }
     }
     return;
   }
-  const Spread at_row(block, a.blocks[which], a.width_pad / 8);
+  const Spread at_row(block, a.blocks[which], a.bytes_pad / 16);
   for (int64_t r = at_row.row; r < p.rows_pad; r += at_row.rows) {
     bool keep = r < p.rows;
     if (keep && p.zero_rows) (void)target_of(a.targets, r, keep);
-    if (by_row && keep) e = row_exp((const float*)p.src + r * p.ld, a.width, r, at_row, p.unscale);
-    for (int c = at_row.piece * 8; c < a.width_pad; c += at_row.pieces * 8) {
-      char* d = p.dst + (r * a.width_pad + c) * 2;
-      if (!f32) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        const uint16_t* src = (const uint16_t*)p.src + r * p.ld + c;
-        if (keep && c + 8 <= a.width) {
-          v = *(const uint4*)src;
-        } else if (keep) {
-          uint32_t h[8];
+    const char* row = p.src + r * p.ld;
+    for (int c = at_row.piece * 16; c < a.bytes_pad; c += at_row.pieces * 16) {
+      const int64_t to = r * a.bytes_pad + c;
+      uint32_t h[4] = {0, 0, 0, 0};
+      if (keep && c + 16 <= a.bytes) {
+        const uint4 v = *(const uint4*)(row + c);
+        h[0] = v.x, h[1] = v.y, h[2] = v.z, h[3] = v.w;
+      } else if (keep) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) h[j] = c + j < a.width ? src[j] : 0;
-          v = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
-        }
-        if (p.dst) *(uint4*)d = v;
-        if (p.halves) {
-          const uint32_t h[4] = {v.x, v.y, v.z, v.w};
-          uint32_t hi[4], lo[4];
-          halves_of(h, hi, lo);
-          char* to = p.halves + (r * a.width_pad + c) * 2;
-          *(uint4*)to = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          *(uint4*)(to + p.plane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        }
-      } else {
-        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        const float* src = (const float*)p.src + r * p.ld + c;
-        if (keep && c + 8 <= a.width) {
-          const f32x4 lo = *(const f32x4*)src, hi = *(const f32x4*)(src + 4);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) v[j] = lo[j], v[4 + j] = hi[j];
-        } else if (keep) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = c + j < a.width ? src[j] : 0.0f;
-        }
+        for (int j = 0; j < 4; ++j) h[j] = load_word(row, c + 4 * j, a.bytes, f32);
+      }
+      if (p.dst) *(uint4*)(p.dst + to) = make_uint4(h[0], h[1], h[2], h[3]);
+      if (p.halves) {
         uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float x = ldexpf(v[2 * j], e), y = ldexpf(v[2 * j + 1], e);
-          hi[j] = pack2(x, y, PST_F16);
-          lo[j] = pack2(rest(x, PST_F16), rest(y, PST_F16), PST_F16);  // an infinity or NaN stands in hi alone
-        }
-        *(uint4*)d = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *(uint4*)(d + p.plane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        halves_of(h, hi, lo);
+        *(uint4*)(p.halves + to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *(uint4*)(p.halves + p.rows_pad * a.bytes_pad + to) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
     }
   }
@@ -344,15 +209,12 @@ struct GemmArgs {
   int32_t steps;       // K-steps of the whole range
   int32_t range, products;  // gradients: K-steps of one product, and how many (see Loop); steps is of all of them
   int32_t gm;
-  // unscaling of 32-bit operands (device; null: 1): of each row for the loss, else of the tensor
-  const float *ua, *ub;
   // loss and logit gradient: n = position, m = vocabulary row (from v0)
   Targets targets;
   float2* part;        // loss: [nm][N] (maximum, sum)
   float* tlogit;       // loss: [N]
   const float *lse, *gloss;
-  const float* gscale; // power of two on D (device; null: 1)
-  char* D;             // [2][rows][ldd] 16-bit: hi and lo
+  char* D;             // [2][rows][ldd] 16-bit: hi and lo; 32-bit operands: [rows][ldd] 32-bit
   int64_t dplane, ldd; // bytes, elements
   int32_t v0;
   // matrix outputs
@@ -393,16 +255,6 @@ struct Place {
     nw = n0 + (wave % T::WN) * T::NI * 16;
   }
 };
-
-template <class T>
-__device__ __forceinline__ void unscale(f32x4 (&acc)[T::MI][T::NI], float mul) {
-#pragma unroll
-  for (int i = 0; i < T::MI; ++i)
-#pragma unroll
-    for (int j = 0; j < T::NI; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) acc[i][j][r] *= mul;
-}
 
 // Two blocks' packed 16-bit values (w[u][q]: block u, the lane's values 2q and 2q + 1) to 32 consecutive columns of the
 // lane's row, whose first is at `to`: the exchange of odd and even 16-lane groups leaves 16 consecutive bytes in a lane.
@@ -463,49 +315,22 @@ __device__ __forceinline__ void tiles(const GemmArgs& g, int tile, int stride, i
 // go to memory. One exponential a logit (16 clocks of a SIMD for 64 of them) is 1/8 of the matrix work at d = 1024;
 // persistent workgroups load the next tile meanwhile.
 // 8192 x 64003 x 1024 bf16: 829 us, 1.30 PFLOP/s (the library's product of that shape alone, logits to memory: 961 us).
-template <int PLANES>
 struct LossEpilogue {
   struct Inputs {
     int target;
-    float ua, ub;  // of this thread's row and column, 32-bit operands
   };
   template <class P>
   __device__ __forceinline__ Inputs load(const GemmArgs& g, const P& p) const {
     bool counts;
     const int n = p.n0 + (int)threadIdx.x;
-    Inputs in{(int)threadIdx.x < P::BN && n < g.N ? target_of(g.targets, n, counts) : -1, 0.0f, 0.0f};
-    if (PLANES == 2) {
-      in.ua = g.ua[min(p.m0 + (int)threadIdx.x, g.M - 1)];
-      in.ub = g.ub[min(n, g.N - 1)];
-    }
-    return in;
+    return {(int)threadIdx.x < P::BN && n < g.N ? target_of(g.targets, n, counts) : -1};
   }
   __device__ __forceinline__ void share(const Inputs& in, float* lds) const {
     asm volatile("" ::"v"(in.target));
     if (threadIdx.x < 256) ((int*)lds)[threadIdx.x] = in.target;
-    if (PLANES == 2) {
-      asm volatile("" ::"v"(in.ua), "v"(in.ub));
-      if (threadIdx.x < 128) {
-        lds[768 + threadIdx.x] = in.ua;
-        lds[896 + threadIdx.x] = in.ub;
-      }
-    }
   }
   template <class T>
   __device__ __forceinline__ void store(const GemmArgs& g, const Place<T>& p, f32x4 (&acc)[T::MI][T::NI], float* lds) const {
-    if (PLANES == 2) {  // (a product of two scales stays finite, so that a logit of zero does)
-      static_assert(T::PLANES == PLANES && (PLANES == 1 || (T::BM <= 128 && T::BN <= 128)), "the scales' LDS");
-#pragma unroll
-      for (int i = 0; i < T::MI; ++i) {
-        const f32x4 ua = *(const f32x4*)(lds + 768 + p.mw - p.m0 + 16 * i);
-#pragma unroll
-        for (int j = 0; j < T::NI; ++j) {
-          const float ub = lds[896 + p.nw - p.n0 + 16 * j + p.col];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) acc[i][j][r] *= fminf(ua[r] * ub, 3.4028234663852886e38f);
-        }
-      }
-    }
     if (p.mwave + T::MI * 16 > g.M) {  // rows behind the vocabulary's last
 #pragma unroll
       for (int i = 0; i < T::MI; ++i)
@@ -573,9 +398,9 @@ template <int E, class T>
 __global__ __launch_bounds__(T::THREADS, T::WAVES) void k_loss(GemmArgs g) {
   extern __shared__ char smem[];
   if ((int)blockIdx.x < g.blocks) {
-    tiles<E, T, true>(g, blockIdx.x, g.blocks, g.nm, g.nn, 0, smem, LossEpilogue<T::PLANES>{});
+    tiles<E, T, true>(g, blockIdx.x, g.blocks, g.nm, g.nn, 0, smem, LossEpilogue{});
   } else if constexpr (T::HAS_THIN) {
-    tiles<E, typename T::Thin, false>(g, blockIdx.x - g.blocks, 1 << 30, 1, g.thins, g.nm * T::BM, smem, LossEpilogue<T::PLANES>{});
+    tiles<E, typename T::Thin, false>(g, blockIdx.x - g.blocks, 1 << 30, 1, g.thins, g.nm * T::BM, smem, LossEpilogue{});
   }
 }
 
@@ -625,13 +450,12 @@ void launch_join(const JoinArgs& j, hipStream_t st) {
 // D of one piece of the vocabulary (columns v0 ...; zeros behind the last row and for positions that do not count), each entry
 // as a sum of two bf16 values, hi + lo: off by 2^-16 of the entry whatever its size, since a bf16 has a float's exponents.
 // One alone would be off by 2^-8, which the sums over thousands of entries of either sign do not lose; f16 ones, scaled to
-// the largest |g|, would drop probabilities and weights far below it. (32-bit operands: two f16, so scaled.) The second
+// the largest |g|, would drop probabilities and weights far below it. (32-bit operands: D in 32 bits.) The second
 // half is a second run of the products (see Loop): 8192 x 64003 x 1024 bf16 4.46 ms, with hi alone 2.71.
 // exp(l - lse) as 2^((l - lse) log2 e): the difference first, so that large logits lose nothing in the product. Stores of
 // 16 bytes a lane.
-template <int PLANES>
+template <int E>
 struct DlogitEpilogue {
-  static constexpr int TYPE = PLANES == 2 ? PST_F16 : PST_BF16;  // (32-bit operands: scaled)
   struct Inputs {
     int target;  // less v0; a position that does not count has a factor of 0
     float lse, c;
@@ -645,7 +469,7 @@ struct DlogitEpilogue {
       const int t = target_of(g.targets, n, counts);
       in.target = t < 0 ? -1 : t - g.v0;
       in.lse = counts ? g.lse[n] : 0.0f;
-      in.c = !counts ? 0.0f : t < 0 ? __builtin_nanf("") : g.gloss[n] * (g.gscale ? *g.gscale : 1.0f);
+      in.c = !counts ? 0.0f : t < 0 ? __builtin_nanf("") : g.gloss[n];
     }
     return in;
   }
@@ -659,7 +483,6 @@ struct DlogitEpilogue {
   }
   template <class T>
   __device__ __forceinline__ void store(const GemmArgs& g, const Place<T>& p, f32x4 (&acc)[T::MI][T::NI], float* lds) const {
-    if (T::PLANES == 2) unscale<T>(acc, fminf(*g.ua * *g.ub, 3.4028234663852886e38f));
     const bool edge = p.mwave + T::MI * 16 > g.M;
 #pragma unroll
     for (int j = 0; j < T::NI; ++j) {
@@ -695,6 +518,12 @@ struct DlogitEpilogue {
 #pragma unroll
           for (int r = 0; r < 4; ++r) acc[i][j][r] = p.mw + 16 * i + r < g.M ? acc[i][j][r] : 0.0f;
       }
+      if constexpr (E == F32) {
+        float* to = (float*)g.D + (int64_t)n * g.ldd + p.mw;
+#pragma unroll
+        for (int i = 0; i < T::MI; ++i) *(f32x4*)(to + 16 * i) = acc[i][j];
+        continue;
+      }
       char* to = g.D + ((int64_t)n * g.ldd + p.mwave) * 2;
 #pragma unroll
       for (int i = 0; i < T::MI; i += 2) {
@@ -702,12 +531,12 @@ struct DlogitEpilogue {
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int q = 0; q < 2; ++q) w[u][q] = pack2(acc[i + u][j][2 * q], acc[i + u][j][2 * q + 1], TYPE);
+          for (int q = 0; q < 2; ++q) w[u][q] = pack2(acc[i + u][j][2 * q], acc[i + u][j][2 * q + 1], PST_BF16);
         store_pair(to + i * 32, w, p.lane);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int q = 0; q < 2; ++q) w[u][q] = pack2(rest(acc[i + u][j][2 * q], TYPE), rest(acc[i + u][j][2 * q + 1], TYPE), TYPE);
+          for (int q = 0; q < 2; ++q) w[u][q] = pack2(rest(acc[i + u][j][2 * q]), rest(acc[i + u][j][2 * q + 1]), PST_BF16);
         store_pair(to + g.dplane + i * 32, w, p.lane);
       }
     }
@@ -718,9 +547,9 @@ template <int E, class T>
 __global__ __launch_bounds__(T::THREADS, T::WAVES) void k_dlogit(GemmArgs g) {
   extern __shared__ char smem[];
   if ((int)blockIdx.x < g.blocks) {
-    tiles<E, T, true>(g, blockIdx.x, g.blocks, g.nm, g.nn, 0, smem, DlogitEpilogue<T::PLANES>{});
+    tiles<E, T, true>(g, blockIdx.x, g.blocks, g.nm, g.nn, 0, smem, DlogitEpilogue<E>{});
   } else if constexpr (T::HAS_THIN) {
-    tiles<E, typename T::Thin, false>(g, blockIdx.x - g.blocks, 1 << 30, 1, g.thins, g.nm * T::BM, smem, DlogitEpilogue<T::PLANES>{});
+    tiles<E, typename T::Thin, false>(g, blockIdx.x - g.blocks, 1 << 30, 1, g.thins, g.nm * T::BM, smem, DlogitEpilogue<E>{});
   }
 }
 
@@ -759,7 +588,6 @@ struct FinishJob {
   int32_t rows_count;  // rows are positions: those that do not count become zeros
   void* out;
   int64_t ldo;
-  const float *u0, *u1;
   int32_t wide;
 };
 struct FinishArgs {
@@ -773,7 +601,6 @@ __global__ __launch_bounds__(256) void k_finish(FinishArgs a) {
   const int block = (int)blockIdx.x - (which ? a.blocks[0] : 0);
   const FinishJob& f = a.job[which];
   const Spread at_row(block, a.blocks[which], (a.width + 3) / 4);
-  const float mul = (f.u0 ? *f.u0 : 1.0f) * (f.u1 ? *f.u1 : 1.0f);
   for (int64_t n = at_row.row; n < f.rows; n += at_row.rows)
   for (int c = at_row.piece * 4; c < a.width; c += at_row.pieces * 4) {
     f32x4 s = {0, 0, 0, 0};
@@ -787,7 +614,7 @@ __global__ __launch_bounds__(256) void k_finish(FinishArgs a) {
     }
     bool counts = true;
     if (f.rows_count) (void)target_of(a.targets, n, counts);
-    const float v[4] = {counts ? s.x * mul : 0.0f, counts ? s.y * mul : 0.0f, counts ? s.z * mul : 0.0f, counts ? s.w * mul : 0.0f};
+    const float v[4] = {counts ? s.x : 0.0f, counts ? s.y : 0.0f, counts ? s.z : 0.0f, counts ? s.w : 0.0f};
     store4(f.out, a.otype, n * f.ldo + c, v, a.width - c, f.wide);
   }
 }
@@ -848,13 +675,12 @@ __device__ __forceinline__ void grad_tile(const GemmArgs& g, int tile, int nm, i
   const Place<T> p(g, tile, nm, nn, 0, n_base);
   const int s0 = (int)((int64_t)g.steps * p.z / g.nz), s1 = (int)((int64_t)g.steps * (p.z + 1) / g.nz);
   f32x4 acc[T::MI][T::NI];
-  Loop<E, T, true, !DX, T::PLANES == 1> loop(smem);
+  Loop<E, T, true, !DX, E != F32> loop(smem);
   loop.begin(g.A, g.B, p.m0, p.n0, s0, s1, g.range, g.products);
   loop.run(acc);
   if (DX || g.part_out) {
     store_part<T>(acc, g, p);
   } else {
-    unscale<T>(acc, (g.ua ? *g.ua : 1.0f) * (g.ub ? *g.ub : 1.0f));
     store_rows<T>(acc, g, p, g.v0);
   }
 }
@@ -919,11 +745,11 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES) void k_scores(GemmArgs g) {
 }
 
 // ------------------------------------------------------------------ the loss of few positions, 32 bits
-// With few positions the way of a 32-bit table through memory is all that counts, and the products above would split it
-// first: read it twice, write as much and read that. This kernel reads it once for 16 NB positions, at any alignment, and
-// multiplies in 32 bits (v_mfma_f32_16x16x4: 32 clocks of a SIMD for 256 bytes of the table, 17 TB/s of them all). us with
-// the split, and so: 1 x 64000 x 1024 205, 51 (5.1 TB/s); 32 x 64000 x 1024 206, 99; 16 x 4096 x 2048 50, 19; 64 x 432 x 64
-// 25, 19; but 64 x 64000 x 333 92, 160 and 256 x 4096 x 1024 35, 46: many positions read the table again and again.
+// With few positions the way of a 32-bit table through memory is all that counts, and the products above are launches of
+// many K-steps for tiles that are mostly empty, after a copy of the table where its rows are not aligned. This kernel
+// reads it once for 16 NB positions, at any alignment (v_mfma_f32_16x16x4: 32 clocks of a SIMD for 256 bytes of the table,
+// 17 TB/s of them all). A call, us: 1 x 64000 x 1024 48 (5.4 TB/s), 16 x 64000 x 1024 67, 16 x 4096 x 2048 16. More
+// positions read the table again and again, and each block of the table all their hidden states.
 struct FewArgs {
   const float *x, *w;
   int64_t ldx, ldw;
@@ -1173,18 +999,18 @@ bool in_place(const void* p, int64_t ld_bytes, int64_t row_bytes) {
   return ((uintptr_t)p & 15) == 0 && ld_bytes % 16 == 0 && row_bytes % 16 == 0;
 }
 
-enum TileId { TILE64 = 0, TILE128 = 1, TILE256 = 2, SPLIT64 = 3, SPLIT128 = 4 };
+enum TileId { TILE64 = 0, TILE128 = 1, TILE256 = 2, FLOAT64 = 3, FLOAT128 = 4 };
 constexpr int TILE_M[5] = {64, 128, 256, 64, 128};
 
 // ---- the choice of tiles
 // Times of a workgroup in us, fitted to single launches on the card (d = 128 ... 1024, 16 ... 8192 positions): BASE and, for
 // each K-step of 64, STEP + MORE for each workgroup that shares the compute unit, up to `slots` of them. The largest
 // tiles reach 1.3 PFLOP/s, those of 128 about 0.95, those of 64 about 0.65; the smaller ones fill the card sooner. The two
-// of split values make three products a step.
+// of 32-bit values, whose K-steps are of 32, are bound by their instructions alone (0.145 PFLOP/s of tiles of 128, 0.135 of 64).
 constexpr int CUS = 256;  // the card's compute units, whatever device is asked: a workspace's size needs none
-constexpr double TILE_BASE[5] = {2.0, 3.0, 4.0, 2.5, 4.0}, TILE_STEP[5] = {0.45, 0.55, 1.5, 0.3, 1.1}, TILE_MORE[5] = {0.1, 0.27, 0.0, 0.28, 0.0};
-constexpr int TILE_SLOTS[5] = {4, 2, 1, 2, 1};
-constexpr double THIN[5] = {0.0, 0.6, 0.35, 0.0, 0.5};  // a thin tile's time, of a whole one's
+constexpr double TILE_BASE[5] = {2.0, 3.0, 4.0, 2.0, 3.0}, TILE_STEP[5] = {0.45, 0.55, 1.5, 0.1, 0.0}, TILE_MORE[5] = {0.1, 0.27, 0.0, 0.45, 1.75};
+constexpr int TILE_SLOTS[5] = {4, 2, 1, 4, 2};
+constexpr double THIN[5] = {0.0, 0.6, 0.35, 0.0, 0.15};  // a thin tile's time, of a whole one's
 double tile_us(int tile, double tiles, int64_t steps) {
   const double share = std::min<double>(TILE_SLOTS[tile], std::max(1.0, tiles / CUS));
   return TILE_BASE[tile] + (TILE_STEP[tile] + TILE_MORE[tile] * share) * steps;
@@ -1196,10 +1022,10 @@ int64_t thin_rows(int64_t m, int tile) {
   return THIN[tile] > 0 && m > rest && rest <= 64 ? rest : 0;
 }
 // m x n of the loss, the logits' gradient and the scores; a compute unit stores about 20 KB in a us (5 TB/s of all)
-int tile_for(int64_t m, int64_t n, int64_t steps, int planes, int out_bytes) {
+int tile_for(int64_t m, int64_t n, int64_t steps, bool f32, int out_bytes) {
   int best = TILE64;
   double us = 1e30;
-  for (int t = planes == 2 ? SPLIT128 : TILE256; t >= (planes == 2 ? SPLIT64 : TILE64); --t) {
+  for (int t = f32 ? FLOAT128 : TILE256; t >= (f32 ? FLOAT64 : TILE64); --t) {
     const int64_t thin = thin_rows(m, t), slots = (int64_t)CUS * TILE_SLOTS[t], full = tiles_of(m - thin, n, t);
     const double share = std::min<double>(TILE_SLOTS[t], std::max(1.0, (double)full / CUS));
     const double one = tile_us(t, full, steps) + (double)TILE_M[t] * TILE_M[t] * out_bytes * share / 20e3;
@@ -1237,13 +1063,13 @@ void set_tiles(GemmArgs& g, int64_t m, int64_t n, int tile) {
 }
 template <int E>
 hipError_t launch_elem(int kind, int tile, const GemmArgs& g, int64_t grid, hipStream_t st) {
-  if constexpr (E == F16) {
-    if (tile == SPLIT128) return launch_kind<E, S128>(kind, g, grid, st);
-    if (tile == SPLIT64) return launch_kind<E, S64>(kind, g, grid, st);
+  if constexpr (E == F32) {
+    return tile == FLOAT128 ? launch_kind<E, T128>(kind, g, grid, st) : launch_kind<E, T64>(kind, g, grid, st);
+  } else {
+    return tile == TILE256   ? launch_kind<E, T256>(kind, g, grid, st)
+           : tile == TILE128 ? launch_kind<E, T128>(kind, g, grid, st)
+                             : launch_kind<E, T64>(kind, g, grid, st);
   }
-  return tile == TILE256   ? launch_kind<E, T256>(kind, g, grid, st)
-         : tile == TILE128 ? launch_kind<E, T128>(kind, g, grid, st)
-                           : launch_kind<E, T64>(kind, g, grid, st);
 }
 hipError_t launch_gemm(int kind, int elem, int tile, GemmArgs g, hipStream_t st) {
   const int64_t thin = thin_rows(g.M, tile);
@@ -1255,6 +1081,7 @@ hipError_t launch_gemm(int kind, int elem, int tile, GemmArgs g, hipStream_t st)
   const int64_t grid = g.blocks + (thin ? g.thins : 0);
   return elem == I8     ? launch_elem<I8>(kind, tile, g, grid, st)
          : elem == BF16 ? launch_elem<BF16>(kind, tile, g, grid, st)
+         : elem == F32  ? launch_elem<F32>(kind, tile, g, grid, st)
                         : launch_elem<F16>(kind, tile, g, grid, st);
 }
 hipError_t launch_grads(int tile, GradArgs g, bool dx, bool dw, hipStream_t st) {
@@ -1271,8 +1098,7 @@ hipError_t launch_grads(int tile, GradArgs g, bool dx, bool dw, hipStream_t st) 
     g.blocks[i] = (int32_t)blocks;
     g.blocks[2 + i] = (int32_t)thins;
   }
-  return tile == SPLIT128  ? launch(k_grads<F16, S128>, grid, S128::THREADS, S128::LDS, st, g)
-         : tile == SPLIT64 ? launch(k_grads<F16, S64>, grid, S64::THREADS, S64::LDS, st, g)
+  return tile == FLOAT64   ? launch(k_grads<F32, T64>, grid, T64::THREADS, T64::LDS, st, g)
          : tile == TILE256 ? launch(k_grads<BF16, T256>, grid, T256::THREADS, T256::LDS, st, g)
          : tile == TILE128 ? launch(k_grads<BF16, T128>, grid, T128::THREADS, T128::LDS, st, g)
                            : launch(k_grads<BF16, T64>, grid, T64::THREADS, T64::LDS, st, g);
@@ -1280,13 +1106,13 @@ hipError_t launch_grads(int tile, GradArgs g, bool dx, bool dw, hipStream_t st) 
 
 // What a call on [rows, width] x [vocab, width] needs of its workspace; the same for the query and for the call.
 struct Plan {
-  int type, elem, planes;
+  int type, elem;
   int products;                                  // of each gradient (see Loop)
   int64_t rows, vocab, width, width_pad, rows_pad;
   bool pack_x, pack_w;
-  int64_t amax = 0, unscale = 0, x = 0, w = 0;   // offsets
+  int64_t x = 0, w = 0;                          // offsets
   int64_t part = 0, tlogit = 0;                  // loss
-  int64_t gscale = 0, xh = 0, wh = 0, D = 0, dxp = 0, dwp = 0;  // gradient
+  int64_t xh = 0, wh = 0, D = 0, dxp = 0, dwp = 0;  // gradient
   int64_t few = 0;                               // k_few: 16-row blocks a workgroup
   int64_t piece = 0;                             // vocabulary rows of a piece
   int tile = 0, zx = 1, zw = 1;                  // of the two gradients' launch
@@ -1295,34 +1121,29 @@ struct Plan {
 Plan plan_common(int type, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab, int64_t width, bool grad, Bump& b) {
   Plan p;
   p.type = type;
-  p.elem = type == PST_BF16 ? BF16 : F16;
-  p.planes = type == PST_F32 ? 2 : 1;
+  p.elem = type == PST_F32 ? F32 : type == PST_BF16 ? BF16 : F16;
   p.products = type == PST_BF16 ? 2 : type == PST_F16 ? 3 : 1;
   p.rows = rows;
   p.vocab = vocab;
   p.width = width;
-  p.width_pad = up(width, 64);
-  p.rows_pad = grad ? up(rows, 64) : rows;
   const int e = size_of(type);
-  p.pack_w = type == PST_F32 || !in_place(w, ldw * e, width * e);
+  p.width_pad = up(width, STEP / e);
+  p.rows_pad = grad ? up(rows, 64) : rows;
+  p.pack_w = !in_place(w, ldw * e, width * e);
   // x is the operand with zeros behind the last column; the gradient needs zeros behind the last row too
-  p.pack_x = type == PST_F32 || grad || p.width_pad != width || !in_place(x, ldx * e, width * e);
-  if (type == PST_F32) {
-    if (grad) p.amax = b.take(2 * AMAX_BLOCKS * 4);
-    p.unscale = b.take((grad ? 2 : rows + vocab) * 4);
-  }
-  if (p.pack_x) p.x = b.take(p.rows_pad * p.width_pad * 2 * p.planes);
-  if (p.pack_w) p.w = b.take(vocab * p.width_pad * 2 * p.planes);
+  p.pack_x = grad || p.width_pad != width || !in_place(x, ldx * e, width * e);
+  if (p.pack_x) p.x = b.take(p.rows_pad * p.width_pad * e);
+  if (p.pack_w) p.w = b.take(vocab * p.width_pad * e);
   return p;
 }
 Plan plan_loss(int type, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab, int64_t width) {
   Bump b;
   Plan p = plan_common(type, x, ldx, w, ldw, rows, vocab, width, false, b);
-  // Up to 32 positions of aligned rows, or a product of about what its launches take (see k_few). A call, this kernel and
-  // the split, us: 32 x 64000 x 512 55 and 72, 1 x 64000 x 1024 51 and 166, 64 x 4096 x 1024 23 and 33; of 333 columns, whose
-  // loads are of one value, 1 x 64000 60 and 76, 16 x 64000 90 and 74; 64 x 64000 x 512 89 and 72.
+  // Up to 16 positions of aligned rows, or a product of about what its launches take (see k_few). A call, this kernel and
+  // the tiles, us: 1, 16, 32 x 64000 x 1024 48, 67, 96 and 74; 16 x 4096 x 2048 16 and 45; 64 x 4096 x 1024 20 and 26;
+  // 256 x 4096 x 256 16 and 15; of 333 columns, whose rows are not aligned, 1, 16 x 64000 57, 87 and 74.
   const bool aligned = in_place(x, ldx * 4, width * 4) && in_place(w, ldw * 4, width * 4);
-  if (type == PST_F32 && ((rows <= 32 && aligned) || (rows <= 1024 && rows * vocab * width <= 1 << 28))) {
+  if (type == PST_F32 && ((rows <= 16 && aligned) || (rows <= 1024 && rows * vocab * width <= 1 << 28))) {
     b = Bump();
     // about four workgroups a compute unit
     p.few = ceil_div(ceil_div(vocab, 16), 4 * CUS);
@@ -1331,14 +1152,16 @@ Plan plan_loss(int type, const void* x, int64_t ldx, const void* w, int64_t ldw,
     p.bytes = b.n;
     return p;
   }
-  p.tile = tile_for(vocab, rows, p.width_pad / 64, p.planes, 0);
+  p.tile = tile_for(vocab, rows, p.width_pad * size_of(type) / STEP, type == PST_F32, 0);
   p.part = b.take(ceil_div(vocab, TILE_M[p.tile]) * rows * 8);
   p.tlogit = b.take(rows * 4);
   p.bytes = b.n;
   return p;
 }
 // The tiles of the two gradients' launch and the parts zx, zw of their K loops: the least of the estimated launch and of
-// the parts' way back through memory (4.5 TB/s). The last choice is kept, by the sizes alone.
+// the parts' way back through memory (4.5 TB/s). 32-bit operands: tiles of 64 alone, which fill the card sooner and lose nothing
+// to those of 128 (both gradients, us: 300 x 432 x 512 29 and 36, 4096 x 4099 x 512 427 and 455, 2048 x 8192 x 2048 1493
+// and 1481). The last choice is kept, by the sizes alone.
 void split_grads(Plan& p, int64_t nv, bool pieces) {
   struct Last {
     int64_t rows = -1, nv, width;
@@ -1348,9 +1171,10 @@ void split_grads(Plan& p, int64_t nv, bool pieces) {
   thread_local Last last;
   if (last.rows != p.rows || last.nv != nv || last.width != p.width || last.products != p.products || last.pieces != pieces) {
     constexpr int Z[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
-    const int64_t sx = p.products * ceil_div(nv, 64), sw = p.products * ceil_div(p.rows, 64), least = p.planes == 2 ? 2 : 4;
+    const bool f32 = p.type == PST_F32;
+    const int64_t ks = STEP / (f32 ? 4 : 2), sx = p.products * ceil_div(nv, ks), sw = p.products * ceil_div(p.rows, ks), least = 4;
     double best = 1e30;
-    for (int t = p.planes == 2 ? SPLIT128 : TILE256; t >= (p.planes == 2 ? SPLIT64 : TILE64); --t) {
+    for (int t = f32 ? FLOAT64 : TILE256; t >= (f32 ? FLOAT64 : TILE64); --t) {
       const int64_t thin_x = thin_rows(p.rows, t), thin_w = thin_rows(nv, t);
       const double slots = (double)CUS * TILE_SLOTS[t];
       const double one_x = tiles_of(p.width_pad, p.rows - thin_x, t), one_w = tiles_of(p.width, nv - thin_w, t);
@@ -1384,7 +1208,6 @@ constexpr int64_t PIECE_BYTES = 288ll << 20, PIECE_LEAST = 4096;
 Plan plan_grad(int type, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab, int64_t width) {
   Bump b;
   Plan p = plan_common(type, x, ldx, w, ldw, rows, vocab, width, true, b);
-  if (type == PST_F32) p.gscale = b.take(8);
   if (type == PST_F16) {
     p.xh = b.take(p.rows_pad * p.width_pad * 4);
     p.wh = b.take(vocab * p.width_pad * 4);
@@ -1434,44 +1257,29 @@ int32_t row_grid(int64_t rows, int64_t per_row) {
   return (int32_t)std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows << shift, 256), CUS * 16ll));
 }
 
-// the operands in a form that the products read: in place, or packed (and split) into the workspace; for the gradient
-// (gloss) also the scale of D. One launch, two for its 32-bit operands, none where there is nothing to do.
-int operands(const Plan& p, const void* x, int64_t ldx, const void* w, int64_t ldw, const Targets& t, const float* gloss, char* ws,
-             hipStream_t st, Operand* X, Operand* W) {
+// the operands in a form that the products read: in place, or packed into the workspace; for the gradient (`grad`) of f16
+// also their bf16 halves. One launch, none where there is nothing to do.
+int operands(const Plan& p, const void* x, int64_t ldx, const void* w, int64_t ldw, const Targets& t, bool grad, char* ws, hipStream_t st,
+             Operand* X, Operand* W) {
+  const int e = size_of(p.type);
   PackArgs a{};
-  a.width = (int32_t)p.width;
-  a.width_pad = (int32_t)p.width_pad;
+  a.bytes = (int32_t)(p.width * e);
+  a.bytes_pad = (int32_t)(p.width_pad * e);
   a.type = p.type;
   a.targets = t;
-  const bool by_row = !gloss;
-  if (p.type == PST_F32 && !by_row) {
-    AmaxArgs m{{(const float*)x, (const float*)w}, {ldx, ldw}, {p.rows, p.vocab}, (int32_t)p.width, (float*)(ws + p.amax), t};
-    hipLaunchKernelGGL(k_amax, dim3(2 * AMAX_BLOCKS), dim3(1024), 0, st, m);
-    HEADCHK(hipGetLastError());
-  }
-  const int e = size_of(p.type);
-  const bool halves = gloss && p.type == PST_F16;
-  auto job = [&](int which, const void* src, int64_t ld, int64_t rows, int64_t rows_pad, int64_t at, int64_t half) {
+  const bool halves = grad && p.type == PST_F16;
+  auto job = [&](int which, const void* src, int64_t ld, int64_t rows, int64_t rows_pad, bool copy, int64_t at, int64_t half) {
     PackJob& j = a.job[which];
-    j = {src, ld, rows, rows_pad, at < 0 ? nullptr : ws + at, half < 0 ? nullptr : ws + half, rows_pad * p.width_pad * 2, by_row ? nullptr : (float*)(ws + p.amax) + which * AMAX_BLOCKS,
-         (float*)(ws + p.unscale) + (by_row ? which * p.rows : which),
-         which == 0 && gloss, ((uintptr_t)src & 15) == 0 && ld * e % 16 == 0};
-    a.blocks[which] = row_grid(rows_pad, p.width_pad / (j.wide ? 8 : 2));
-    return Operand{ws + at, j.plane, p.width_pad * 2, (int32_t)rows_pad, (int32_t)p.width_pad * 2};
+    j = {(const char*)src, ld * e, rows, rows_pad, copy ? ws + at : nullptr, halves ? ws + half : nullptr, which == 0 && grad,
+         ((uintptr_t)src & 15) == 0 && ld * e % 16 == 0};
+    a.blocks[which] = row_grid(rows_pad, a.bytes_pad / (j.wide ? 16 : 4));
   };
-  *X = p.pack_x ? job(0, x, ldx, p.rows, p.rows_pad, p.x, halves ? p.xh : -1)
-                : Operand{(const char*)x, 0, ldx * e, (int32_t)p.rows, (int32_t)p.width * e};
-  if (p.pack_w || halves) *W = job(1, w, ldw, p.vocab, p.vocab, p.pack_w ? p.w : -1, halves ? p.wh : -1);
-  if (!p.pack_w) *W = Operand{(const char*)w, 0, ldw * e, (int32_t)p.vocab, (int32_t)p.width * e};
-  int blocks = a.blocks[0] + a.blocks[1];
-  if (gloss && p.type == PST_F32) {
-    a.gloss = gloss;
-    a.n = p.rows;
-    a.gscale = (float*)(ws + p.gscale);
-    ++blocks;
-  }
-  if (blocks) {
-    hipLaunchKernelGGL(k_pack, dim3((unsigned)blocks), dim3(256), 0, st, a);
+  *X = p.pack_x ? Operand{ws + p.x, 0, a.bytes_pad, (int32_t)p.rows_pad, a.bytes_pad} : Operand{(const char*)x, 0, ldx * e, (int32_t)p.rows, a.bytes};
+  *W = p.pack_w ? Operand{ws + p.w, 0, a.bytes_pad, (int32_t)p.vocab, a.bytes_pad} : Operand{(const char*)w, 0, ldw * e, (int32_t)p.vocab, a.bytes};
+  if (p.pack_x) job(0, x, ldx, p.rows, p.rows_pad, true, p.x, p.xh);
+  if (p.pack_w || halves) job(1, w, ldw, p.vocab, p.vocab, p.pack_w, p.w, p.wh);
+  if (a.blocks[0] + a.blocks[1]) {
+    hipLaunchKernelGGL(k_pack, dim3((unsigned)(a.blocks[0] + a.blocks[1])), dim3(256), 0, st, a);
     HEADCHK(hipGetLastError());
   }
   return PST_OK;
@@ -1509,15 +1317,11 @@ int token_loss(int device, int type, const void* x, int64_t ldx, const void* w, 
     HEADCHK(hipGetLastError());
     return PST_OK;
   }
-  rc = operands(p, x, ldx, w, ldw, g.targets, nullptr, ws, st, &g.B, &g.A);
+  rc = operands(p, x, ldx, w, ldw, g.targets, false, ws, st, &g.B, &g.A);
   if (rc != PST_OK) return rc;
   g.M = (int32_t)vocab;
   g.N = (int32_t)rows;
-  g.steps = (int32_t)(p.width_pad / 64);
-  if (p.planes == 2) {
-    g.ua = (float*)(ws + p.unscale) + rows;
-    g.ub = (float*)(ws + p.unscale);
-  }
+  g.steps = (int32_t)(p.width_pad * size_of(type) / STEP);
   g.part = (float2*)(ws + p.part);
   g.tlogit = (float*)(ws + p.tlogit);
   HEADCHK(launch_gemm(LOSS, p.elem, p.tile, g, st));
@@ -1551,13 +1355,9 @@ int token_loss_grad(int device, int type, const void* x, int64_t ldx, const void
   Plan q = p;
   q.rows = rows;
   Operand X, W;
-  static const float none = 0.0f;  // (never read: there are no rows)
-  rc = operands(q, x, ldx, w, ldw, t, rows ? gloss : &none, ws, st, &X, &W);
+  rc = operands(q, x, ldx, w, ldw, t, true, ws, st, &X, &W);
   if (rc != PST_OK) return rc;
-  const float* gs = p.type == PST_F32 ? (float*)(ws + p.gscale) : nullptr;
-  const float* ungs = gs ? gs + 1 : nullptr;
-  const float* ux = p.planes == 2 ? (float*)(ws + p.unscale) : nullptr;
-  const float* uw = p.planes == 2 ? ux + 1 : nullptr;
+  const int de = p.type == PST_F32 ? 4 : 2, ks = STEP / de;  // bytes of D's values, K-steps' values
   char* D = ws + p.D;
   const int64_t drows = up(std::max<int64_t>(rows, 1), 256);
   const bool need_dx = dx && rows;
@@ -1566,7 +1366,7 @@ int token_loss_grad(int device, int type, const void* x, int64_t ldx, const void
   const Operand Wh = p.type == PST_F16 ? Operand{ws + p.wh, vocab * X.ld, X.ld, (int32_t)vocab, X.bytes} : W;
   for (int64_t v0 = 0; v0 < vocab; v0 += p.piece) {
     const int64_t nv = std::min(p.piece, vocab - v0), ldd = up(nv, 256);
-    const Operand dop{D, drows * ldd * 2, ldd * 2, (int32_t)drows, (int32_t)ldd * 2};
+    const Operand dop{D, drows * ldd * de, ldd * de, (int32_t)drows, (int32_t)ldd * de};
     Operand Wv = W;
     Wv.p += v0 * W.ld;
     Wv.rows = (int32_t)nv;
@@ -1575,18 +1375,15 @@ int token_loss_grad(int device, int type, const void* x, int64_t ldx, const void
     g.B = X;
     g.M = (int32_t)nv;
     g.N = (int32_t)rows;
-    g.steps = (int32_t)(p.width_pad / 64);
-    g.ua = uw;
-    g.ub = ux;
+    g.steps = (int32_t)(p.width_pad * e / STEP);
     g.targets = t;
     g.lse = lse;
     g.gloss = gloss;
-    g.gscale = gs;
     g.D = D;
     g.dplane = dop.plane;
     g.ldd = ldd;
     g.v0 = (int32_t)v0;
-    if (rows) HEADCHK(launch_gemm(DLOGIT, p.elem, tile_for(nv, rows, g.steps, p.planes, 4), g, st));
+    if (rows) HEADCHK(launch_gemm(DLOGIT, p.elem, tile_for(nv, rows, g.steps, p.type == PST_F32, 4), g, st));
     GradArgs b{};
     b.dx.A = Wh;
     b.dx.A.p += v0 * Wh.ld;
@@ -1594,8 +1391,8 @@ int token_loss_grad(int device, int type, const void* x, int64_t ldx, const void
     b.dx.B = b.dw.B = dop;
     b.dx.M = b.dw.M = (int32_t)width;
     b.dx.N = (int32_t)rows;
-    b.dx.range = (int32_t)ceil_div(nv, 64);
-    b.dw.range = (int32_t)ceil_div(rows, 64);
+    b.dx.range = (int32_t)ceil_div(nv, ks);
+    b.dw.range = (int32_t)ceil_div(rows, ks);
     b.dx.products = b.dw.products = p.products;
     b.dx.steps = b.dx.range * p.products;
     b.dw.steps = b.dw.range * p.products;
@@ -1607,8 +1404,6 @@ int token_loss_grad(int device, int type, const void* x, int64_t ldx, const void
     b.dw.A = Xh;
     b.dw.N = (int32_t)nv;
     b.dw.nz = p.zw;
-    b.dw.ua = ungs;
-    b.dw.ub = ux;
     b.dw.v0 = (int32_t)v0;
     b.dw.out = dw;
     b.dw.ldo = lddw;
@@ -1624,13 +1419,13 @@ int token_loss_grad(int device, int type, const void* x, int64_t ldx, const void
   f.width = (int32_t)width;
   f.otype = type;
   f.targets = t;
-  auto job = [&](int which, int64_t part, int64_t n, int nz, void* out, int64_t ldo, const float* u) {
-    f.job[which] = {(const float*)(ws + part), p.width_pad, n * p.width_pad, n, nz, which == 0, out, ldo, ungs, u,
+  auto job = [&](int which, int64_t part, int64_t n, int nz, void* out, int64_t ldo) {
+    f.job[which] = {(const float*)(ws + part), p.width_pad, n * p.width_pad, n, nz, which == 0, out, ldo,
                     ldo % 4 == 0 && ((uintptr_t)out & (type == PST_F32 ? 15 : 7)) == 0};
     f.blocks[which] = row_grid(n, ceil_div(width, 4));
   };
-  if (need_dx) job(0, p.dxp, rows, p.zx, dx, lddx, uw);
-  if (dw && p.zw > 1) job(1, p.dwp, vocab, p.zw, dw, lddw, ux);
+  if (need_dx) job(0, p.dxp, rows, p.zx, dx, lddx);
+  if (dw && p.zw > 1) job(1, p.dwp, vocab, p.zw, dw, lddw);
   if (f.blocks[0] + f.blocks[1]) {
     hipLaunchKernelGGL(k_finish, dim3((unsigned)(f.blocks[0] + f.blocks[1])), dim3(256), 0, st, f);
     HEADCHK(hipGetLastError());
@@ -1727,7 +1522,7 @@ int token_scores_i8(int device, int type, const void* x, int64_t ldx, const int8
   g.wide = ldo % (16 / size_of(otype)) == 0 && ((uintptr_t)out & 15) == 0;
   g.sn = (const float*)(ws + p.scale);
   g.sm = wscale;
-  HEADCHK(launch_gemm(SCORES, I8, tile_for(vocab, rows, g.steps, 1, size_of(otype)), g, st));
+  HEADCHK(launch_gemm(SCORES, I8, tile_for(vocab, rows, g.steps, false, size_of(otype)), g, st));
   return PST_OK;
 }
 

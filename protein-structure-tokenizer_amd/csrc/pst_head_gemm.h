@@ -1,7 +1,7 @@
 // pst_head_gemm.h — the matrix product under the token head's operators (gfx950 / CDNA4).
 //
-// D[m][n] = sum_k A[m][k] B[n][k] on a BM x BN tile, 16-bit floats (f32 sums) or 8-bit integers (i32 sums), by
-// v_mfma_*_16x16x32 / 16x16x64. Lane l of a wave holds, of each 16x16 block, column n = l & 15 and rows
+// D[m][n] = sum_k A[m][k] B[n][k] on a BM x BN tile, 16-bit or 32-bit floats (f32 sums) or 8-bit integers (i32 sums), by
+// v_mfma_*_16x16x32 / 16x16x4 / 16x16x64. Lane l of a wave holds, of each 16x16 block, column n = l & 15 and rows
 // m = 4 (l >> 4) + r, r = 0..3: the operand whose index runs along the outputs' contiguous axis is A (four
 // neighbours in one lane), and a reduction over that axis is 32 values in a lane and two lane exchanges.
 //
@@ -12,7 +12,7 @@
 // instructions take 155 us instead of 216, without the LDS reads 195: what remains is moving operands. 80 % of the loads
 // hit L2, whose share of the rest is what the tile order leaves: each matrix once from behind it.
 //
-// A K-step is 128 bytes of k (64 16-bit values, 128 8-bit ones) of every tile row. Operands are staged by
+// A K-step is 128 bytes of k (64 16-bit values, 32 32-bit ones, 128 8-bit ones) of every tile row. Operands are staged by
 // global_load_lds_dwordx4 (global memory to LDS without registers: lane i of the instruction fills 16 bytes
 // at base + 16 i, so what is permuted is the global address each lane reads) in two forms:
 //   ROWS  memory holds k contiguous in each row. LDS: [row][8 chunks of 16 bytes], chunk c of row r at place
@@ -35,35 +35,48 @@ typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-enum Elem { BF16 = 0, F16 = 1, I8 = 2 };
+enum Elem { BF16 = 0, F16 = 1, I8 = 2, F32 = 3 };
+constexpr int bytes_of(int elem) { return elem == I8 ? 1 : elem == F32 ? 4 : 2; }
 
 template <int E>
 struct Mma;
 template <>
 struct Mma<BF16> {
   typedef f32x4 Acc;
-  static __device__ __forceinline__ Acc mma(i32x4 a, i32x4 b, Acc c) {
+  static constexpr int PARTS = 1;  // instructions for the 16 bytes of k a lane holds
+  static __device__ __forceinline__ Acc mma(i32x4 a, i32x4 b, Acc c, int) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
 };
 template <>
 struct Mma<F16> {
   typedef f32x4 Acc;
-  static __device__ __forceinline__ Acc mma(i32x4 a, i32x4 b, Acc c) {
+  static constexpr int PARTS = 1;
+  static __device__ __forceinline__ Acc mma(i32x4 a, i32x4 b, Acc c, int) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
 };
 template <>
 struct Mma<I8> {
   typedef i32x4 Acc;
-  static __device__ __forceinline__ Acc mma(i32x4 a, i32x4 b, Acc c) {
+  static constexpr int PARTS = 1;
+  static __device__ __forceinline__ Acc mma(i32x4 a, i32x4 b, Acc c, int) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+  }
+};
+// 32-bit floats: of the four k a lane holds, each instruction takes one of each 16-lane group
+template <>
+struct Mma<F32> {
+  typedef f32x4 Acc;
+  static constexpr int PARTS = 4;
+  static __device__ __forceinline__ Acc mma(i32x4 a, i32x4 b, Acc c, int part) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, a)[part], __builtin_bit_cast(f32x4, b)[part], c, 0, 0, 0);
   }
 };
 
 // One operand in memory. ROWS: `rows` rows of `bytes` valid bytes (a multiple of 16). COLS: `rows` k-rows of
-// `bytes` valid bytes. ld in bytes, a multiple of 16 (and p 16-byte aligned). Split 32-bit floats have two planes of
-// 16-bit ones, hi at p and lo at p + plane.
+// `bytes` valid bytes. ld in bytes, a multiple of 16 (and p 16-byte aligned). Sums of two 16-bit floats have two planes,
+// hi at p and lo at p + plane.
 struct Operand {
   const char* p;
   int64_t plane;
@@ -94,18 +107,21 @@ __device__ __forceinline__ void landed_but() {
 // All waves meet, with what they wrote to LDS and whatever loads in flight.
 __device__ __forceinline__ void met() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// COLS: what the number of a 32-byte piece of LDS row k is xored with, rows of RT bytes. A read takes k-rows
-// 8 g + i (g, i = 0..3) and one piece of each: eight places of the 256-byte bank row, each twice.
-template <int RT>
+// COLS: LDS row k is made of pieces of 16 values (a block's rows), and this is what a piece's number is xored with, of B-byte
+// values in rows of RT bytes. 16 bits: a read takes k-rows 8 g + i (g, i = 0..3) and one piece of each: eight places
+// of the 256-byte bank row, each twice. 32 bits: k-rows 4 g + e, each e a read of its own: four places, each once.
+template <int RT, int B>
 __device__ __forceinline__ int swizzle(int k) {
+  if (B == 4) return k >> 2 & 3;
   return RT == 128 ? (k >> 1 & 1) | (k >> 2 & 2) : (k & 3) | (k >> 1 & 4);
 }
 
-// R: tile rows (m or n); NW: waves that share the loading
-template <int R, bool COLS, int NW>
+// R: tile rows (m or n); NW: waves that share the loading; B: bytes of a value
+template <int R, bool COLS, int NW, int B>
 struct Stager {
   static constexpr int NI = R * STEP / 1024 / NW;  // instructions a wave and K-step
-  static constexpr int RT = COLS ? R * 2 : STEP;   // bytes of an LDS row
+  static constexpr int RT = COLS ? R * B : STEP;   // bytes of an LDS row
+  static constexpr int KS = STEP / B;              // k-rows of a K-step
   static constexpr int PER = 1024 / RT;            // LDS rows an instruction fills
   static_assert(NI >= 1 && NI * NW * 1024 == R * STEP, "tile and waves do not fit");
   uint32_t off[NI];
@@ -122,7 +138,7 @@ struct Stager {
     plane = o.plane;
     left = 1 << 30;
     // a tile behind the last row (a column of zeros in the output) reads the last one
-    const int first = COLS ? min(row0 * 2, o.bytes - 16) : min(row0, o.rows - 1);
+    const int first = COLS ? min(row0 * B, o.bytes - 16) : min(row0, o.rows - 1);
     base = o.p + (COLS ? (int64_t)first : (int64_t)first * o.ld);
     k_bytes = COLS ? o.rows : o.bytes;
 #pragma unroll
@@ -130,22 +146,22 @@ struct Stager {
       const int r = (wave * NI + j) * PER + lane / (RT / 16);  // LDS row
       const int c = lane % (RT / 16);                          // 16-byte place in it
       if (COLS) {
-        const int col = (((c >> 1) ^ swizzle<RT>(r)) << 5) | ((c & 1) << 4);
+        const int col = ((c / B) ^ swizzle<RT, B>(r)) * (16 * B) + c % B * 16;
         off[j] = (uint32_t)(r * (int64_t)o.ld) + (uint32_t)min(col, o.bytes - 16 - first);
       } else {
         off[j] = (uint32_t)(min(r, o.rows - 1 - first) * o.ld) + (uint32_t)((c ^ (r >> 1 & 7)) << 4);
       }
     }
   }
-  // K-step `step` goes to the LDS tile at `lds` (its lo plane to the tile behind), by one(0) ... one(NI - 1) a plane.
+  // K-step `step` goes to the LDS tile at `lds`, by one(0) ... one(NI - 1).
   // AGAIN: the K range comes more than once, from plane `q`
   template <bool AGAIN>
   __device__ __forceinline__ void aim(int step, int q, uint32_t lds, int lane, int wave) {
-    constexpr int WHOLE = COLS ? 64 : STEP;
+    constexpr int WHOLE = COLS ? KS : STEP;
     if (AGAIN && left < WHOLE) shift<-1>(left, lane, wave);  // back from the last step of the range
-    src = base + (COLS ? (int64_t)min(step * 64, k_bytes - 1) * ld : (int64_t)step * STEP);
+    src = base + (COLS ? (int64_t)min(step * KS, k_bytes - 1) * ld : (int64_t)step * STEP);
     if (AGAIN) src += q * plane;
-    left = COLS ? k_bytes - step * 64 : k_bytes - step * STEP;
+    left = COLS ? k_bytes - step * KS : k_bytes - step * STEP;
     if (left < WHOLE) shift<1>(left, lane, wave);  // the last step of the range
     to = __builtin_amdgcn_readfirstlane(lds + (uint32_t)wave * (NI * 1024));
   }
@@ -160,27 +176,34 @@ struct Stager {
     }
   }
   __device__ __forceinline__ void one(int j) const {
-    const int q = j / NI, i = j % NI;
-    load_lds(q ? src + plane : src, off[i], to + q * (R * STEP) + i * 1024);
+    load_lds(src, off[j], to + j * 1024);
   }
 };
 
 // Fragments of one wave, 16 rows x 64 bytes of k each: block b (from block blk0 of the tile), half s of the K-step
-template <int R, bool COLS>
+template <int R, bool COLS, int B>
 struct Reader {
   uint32_t at[2];
   __device__ __forceinline__ void init(int blk0, int lane) {
     const int g = lane >> 4, i = lane & 15;
     if (COLS) {
-      constexpr int RT = R * 2;
-      const int k = 8 * g + (i >> 2);
-      at[0] = k * RT + ((blk0 ^ swizzle<RT>(k)) << 5) + ((i & 3) << 3);
+      constexpr int RT = R * B;
+      const int k = B == 4 ? 4 * g : 8 * g + (i >> 2);
+      at[0] = k * RT + (blk0 ^ swizzle<RT, B>(k)) * (16 * B) + (B == 4 ? i << 2 : (i & 3) << 3);
     } else {
 #pragma unroll
       for (int s = 0; s < 2; ++s) at[s] = (blk0 * 16 + i) * STEP + (((4 * s + g) ^ (i >> 1)) << 4);
     }
   }
   __device__ __forceinline__ i32x4 get(const char* tile, int b, int s) const {
+    if (COLS && B == 4) {
+      constexpr int RT = R * B;
+      const char* q = tile + (at[0] ^ (uint32_t)(b << 6)) + s * 16 * RT;
+      i32x4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = *(const int*)(q + e * RT);
+      return v;
+    }
     if (COLS) {
       constexpr int RT = R * 2;
       typedef __attribute__((address_space(3))) s16x4* P;
@@ -193,13 +216,13 @@ struct Reader {
   }
 };
 
-template <int BM_, int BN_, int WM_, int WN_, int STAGES_, int PLANES_ = 1>
+template <int BM_, int BN_, int WM_, int WN_, int STAGES_>
 struct Tile {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NW = WM_ * WN_, THREADS = NW * 64;
   static constexpr int MI = BM_ / WM_ / 16, NI = BN_ / WN_ / 16;  // a wave's 16x16 blocks
   static constexpr int WAVES = 2;  // on each SIMD at least: what a workgroup's registers leave room for
-  static constexpr int STAGES = STAGES_, PLANES = PLANES_;
-  static constexpr int STAGE = (BM_ + BN_) * STEP * PLANES_, LDS = STAGES * STAGE;  // (an epilogue's own LDS lies behind)
+  static constexpr int STAGES = STAGES_;
+  static constexpr int STAGE = (BM_ + BN_) * STEP, LDS = STAGES * STAGE;  // (an epilogue's own LDS lies behind)
 };
 
 // The K loop of one tile after another: begin() starts the loads of a tile's first K-steps, run() leaves the tile's sums in
@@ -219,13 +242,13 @@ struct Loop {
   static constexpr int HI = T::MI / 2;
   // blocks of a wave start at a multiple of their number, so that a COLS read can xor the block into its address
   static_assert((T::MI & (T::MI - 1)) == 0 && (T::NI & (T::NI - 1)) == 0 && T::MI >= 2, "wave tile");
-  static constexpr int S = T::STAGES, PL = T::PLANES;
-  static constexpr int LA = Stager<T::BM, ACOLS, T::NW>::NI * PL, LB = Stager<T::BN, BCOLS, T::NW>::NI * PL, L = LA + LB;
+  static constexpr int S = T::STAGES, B = bytes_of(E);
+  static constexpr int LA = Stager<T::BM, ACOLS, T::NW, B>::NI, LB = Stager<T::BN, BCOLS, T::NW, B>::NI, L = LA + LB;
   static_assert((S & (S - 1)) == 0 && S >= 2, "ring of stages");
-  Stager<T::BM, ACOLS, T::NW> sa;
-  Stager<T::BN, BCOLS, T::NW> sb;
-  Reader<T::BM, ACOLS> ra;
-  Reader<T::BN, BCOLS> rb;
+  Stager<T::BM, ACOLS, T::NW, B> sa;
+  Stager<T::BN, BCOLS, T::NW, B> sb;
+  Reader<T::BM, ACOLS, B> ra;
+  Reader<T::BN, BCOLS, B> rb;
   const char* smem;
   uint32_t lds0;
   int lane, wave;
@@ -244,7 +267,7 @@ struct Loop {
     if (HALVES) c = step >= 2 * range ? 2 : step >= range ? 1 : 0;
     const int s = HALVES ? step - c * range : step;
     sa.template aim<HALVES>(s, products == 3 && c == 1, to, lane, wave);
-    sb.template aim<HALVES>(s, products > 1 && c == 0, to + T::BM * STEP * PL, lane, wave);
+    sb.template aim<HALVES>(s, products > 1 && c == 0, to + T::BM * STEP, lane, wave);
     ++step;
   }
   __device__ __forceinline__ void load(int i) const {
@@ -293,32 +316,27 @@ struct Loop {
     __builtin_amdgcn_sched_barrier(0);
   }
 
-  i32x4 a[2][PL][HI], b[2][PL][T::NI];
+  i32x4 a[2][HI], b[2][T::NI];
   // fragments of part p of the K-step in `stage`
   __device__ __forceinline__ void fetch(int stage, int p) {
     const char* ta = smem + stage * T::STAGE;
-    const char* tb = ta + T::BM * STEP * PL;
+    const char* tb = ta + T::BM * STEP;
 #pragma unroll
-    for (int q = 0; q < PL; ++q) {
+    for (int i = 0; i < HI; ++i) a[p & 1][i] = ra.get(ta, (p & 1) * HI + i, p >> 1);
+    if ((p & 1) == 0) {
 #pragma unroll
-      for (int i = 0; i < HI; ++i) a[p & 1][q][i] = ra.get(ta + q * (T::BM * STEP), (p & 1) * HI + i, p >> 1);
-      if ((p & 1) == 0) {
-#pragma unroll
-        for (int j = 0; j < T::NI; ++j) b[p >> 1][q][j] = rb.get(tb + q * (T::BN * STEP), j, p >> 1);
-      }
+      for (int j = 0; j < T::NI; ++j) b[p >> 1][j] = rb.get(tb, j, p >> 1);
     }
     __builtin_amdgcn_sched_barrier(0);
   }
-  // multiplies part p; MORE: with the loads of a K-step. Of split values the three products that count, the small ones
-  // first: lo hi + hi lo + hi hi.
+  // multiplies part p; MORE: with the loads of a K-step
   template <bool MORE>
   __device__ __forceinline__ void mult(Acc (&acc)[T::MI][T::NI], int p) {
-    constexpr int ONE = HI * T::NI, COUNT = ONE * (PL == 2 ? 3 : 1);
+    constexpr int ONE = HI * T::NI, COUNT = ONE * Mma<E>::PARTS;
 #pragma unroll
     for (int q = 0; q < COUNT; ++q) {
-      const int i = q % ONE / T::NI, j = q % T::NI, c = q / ONE;
-      const int qa = PL == 2 && c == 0, qb = PL == 2 && c == 1;
-      acc[(p & 1) * HI + i][j] = Mma<E>::mma(a[p & 1][qa][i], b[p >> 1][qb][j], acc[(p & 1) * HI + i][j]);
+      const int i = q % ONE / T::NI, j = q % T::NI;
+      acc[(p & 1) * HI + i][j] = Mma<E>::mma(a[p & 1][i], b[p >> 1][j], acc[(p & 1) * HI + i][j], q / ONE);
       if constexpr (MORE) load_behind<COUNT>(q);
     }
     __builtin_amdgcn_sched_barrier(0);

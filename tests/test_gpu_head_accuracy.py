@@ -78,7 +78,8 @@ def check_grad(x, w, t, gl, lse=None, columns=slice(None)):
     err = c.abs() * p * (torch.expm1(off.clamp(max=700)).where(p > 0, 0.0) + 4 * U32 * (z.abs() + 2)) + slope.abs() * 4 * U32
     # 16-bit types: the slope as a sum of two bf16 halves (2^-16); f16: without the product of two low halves (2^-16)
     halves = 0.0 if dt == torch.float32 else 2.0 ** -16
-    err = err + slope.abs() * halves + 2.0 ** -149
+    # (the hardware's exponential of less than the smallest normal number, 2^-126, is 0: never more than that off)
+    err = err + slope.abs() * halves + c.abs() * 2.0 ** -126
     left = 2.0 ** -16 if dt == torch.float16 else 0.0
     passes = {torch.float32: 1, torch.bfloat16: 2, torch.float16: 3}[dt]
     for got, s, e, other, terms in ((dx, slope, err, w, v), (dw, slope.T, err.T, x, n)):
@@ -124,3 +125,70 @@ def test_improbable_ids(rows, vocab, width, dtype, bias, weight):
     _, dw = check_grad(x, w, t, gl * weight / 1.5)
     # float16: e^-24 / 500 ids, times 4e4 and a sum of 48 of either sign, is 2e-8, less than the smallest step of 6e-8
     assert dtype == torch.float16 or (dw[5] != 0).all()
+
+
+# in 32 bits too: each value keeps its digits whatever else its row, its tensor or the weights of positions hold
+@pytest.mark.parametrize("rows,vocab,width", [(40, 300, 64), (600, 700, 136), (2049, 4099, 72), (1100, 2100, 333), (900, 130, 8)])
+def test_32_bits(rows, vocab, width):
+    x, w, t, gl = make(rows, vocab, width, torch.float32, seed=1)
+    check_loss(x, w, t)
+    check_grad(x, w, t, gl)
+
+
+@pytest.mark.parametrize("rows,vocab,width", [(200, 64003, 64), (1100, 4099, 96)])
+def test_32_bit_weights_and_rows_of_very_different_sizes(rows, vocab, width):
+    x, w, t, _ = make(rows, vocab, width, torch.float32, seed=2)
+    w += 0.1
+    gl = 10.0 ** torch.linspace(-9, 6, rows, device=DEV)
+    check_grad(x, w, t, gl)
+    check_grad(x, w, t, gl.flip(0))
+    sizes = 10.0 ** torch.linspace(-6, 1, rows, device=DEV)[:, None]
+    check_grad(x * sizes, w, t, gl)
+    # one column of hidden a million million times the others', with nothing in the table beside it
+    x[:, 0], w[:, 0] = 1e12, 0
+    check_loss(x, w, t)
+    check_grad(x, w, t, gl, columns=slice(1, None))
+
+
+@pytest.mark.parametrize("bias", [-40, -80])
+@pytest.mark.parametrize("rows,vocab,width", [(60, 500, 64), (1200, 2100, 80)])
+def test_32_bit_improbable_ids(rows, vocab, width, bias):
+    x, w, t, gl = make(rows, vocab, width, torch.float32, seed=3)
+    x, w = with_bias(x, w)
+    w[5, -1] = bias
+    t[t == 5] = 6
+    _, dw = check_grad(x, w, t, gl)
+    assert (dw[5] != 0).all()
+
+
+MASKED = [(40, 300, 96), (600, 700, 128), (2049, 4099, 160), (1200, 2100, 333), (3, 70, 64)]
+
+
+# ids that are not allowed: their bias is a large negative number, as large as the type has
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("mask", ["least", -1e30, -1e9, -1e4])
+@pytest.mark.parametrize("rows,vocab,width", MASKED)
+def test_masks_of_large_numbers(rows, vocab, width, mask, dtype):
+    least = torch.finfo(dtype).min
+    x, w, t, gl = make(rows, vocab, width, dtype, seed=4)
+    x, w = with_bias(x, w)
+    w[[5, vocab - 1], -1] = least if mask == "least" else max(mask, least)
+    t[(t == 5) | (t == vocab - 1)] = 6
+    x[::3, -1] = 0  # (positions that allow them)
+    _, lse = check_loss(x, w, t)
+    check_grad(x, w, t, gl, lse)
+
+
+# the same with -inf: probability 0, and nothing else of the position's
+@pytest.mark.parametrize("dtype", [torch.float32], ids=str)
+@pytest.mark.parametrize("rows,vocab,width", MASKED)
+def test_masks_of_infinity(rows, vocab, width, dtype):
+    x, w, t, gl = make(rows, vocab, width, dtype, seed=5)
+    x, w = with_bias(x, w)
+    w[[5, vocab - 1], -1] = -torch.inf
+    t[(t == 5) | (t == vocab - 1)] = 6
+    _, lse = check_loss(x, w, t)
+    assert lse.isfinite().all()
+    # (the bias column of hidden's gradient is a sum over 0 (-inf))
+    dx, _ = check_grad(x, w, t, gl, lse, columns=slice(0, -1))
+    assert not dx[t != -100, -1].isfinite().any()
