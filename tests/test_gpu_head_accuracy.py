@@ -180,8 +180,9 @@ def test_masks_of_large_numbers(rows, vocab, width, mask, dtype):
 
 
 # the same with -inf: probability 0, and nothing else of the position's
-@pytest.mark.parametrize("dtype", [torch.float32], ids=str)
-@pytest.mark.parametrize("rows,vocab,width", MASKED)
+# (widths of 72 and 100: rows read in place that end inside a K-step, with the infinity in their last 16 bytes)
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("rows,vocab,width", MASKED + [(600, 700, 72), (600, 700, 100), (2100, 4160, 8), (70, 20000, 20)])
 def test_masks_of_infinity(rows, vocab, width, dtype):
     x, w, t, gl = make(rows, vocab, width, dtype, seed=5)
     x, w = with_bias(x, w)
