@@ -41,9 +41,9 @@ def _torch():
         _native.lib()
         if not _native.shares_torch_runtime:
             raise _native.PstError("import torch before pst_amd loads libpst: the two hold different HIP runtimes")
-        _torch_module = torch
         for bits in (32, 64):
             _target_bits[getattr(torch, f"int{bits}")] = bits
+        _torch_module = torch  # last: another thread that sees it goes on with what is above
     return _torch_module
 
 

@@ -114,3 +114,18 @@ def test_strides_are_checked():
         head._matrix(m[0], "m")
     with pytest.raises(ValueError, match="vector"):
         head._vector(m[:, 0], "v", 6, m.device)
+
+
+def test_another_thread_s_first_call_sees_all_of_the_set_up(monkeypatch):
+    order = []
+
+    class Watched(dict):
+        def __setitem__(self, key, value):
+            order.append(head._torch_module)
+            super().__setitem__(key, value)
+
+    monkeypatch.setattr(head, "_torch_module", None)
+    monkeypatch.setattr(head, "_target_bits", Watched())
+    assert head._torch() is torch
+    # while the table of target types is filled nobody is told that it is there
+    assert order and all(m is None for m in order) and set(head._target_bits) == {torch.int32, torch.int64}
