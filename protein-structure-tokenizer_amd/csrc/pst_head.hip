@@ -1547,11 +1547,8 @@ const char* pst_head_error(void) { return pst_head::g_error.c_str(); }
 int64_t pst_token_loss_workspace(int32_t type, const void* d_hidden, int64_t ld_hidden, const void* d_weight, int64_t ld_weight, int64_t rows,
                                  int64_t vocab, int64_t width) {
   using namespace pst_head;
-  return guarded([&]() -> int {
-           return check_sizes(type, d_hidden, ld_hidden, d_weight, ld_weight, rows, vocab, width);
-         }) == PST_OK
-             ? plan_loss(type, d_hidden, ld_hidden, d_weight, ld_weight, rows, vocab, width).bytes
-             : (int64_t)PST_E_INVALID;
+  const int rc = guarded([&]() -> int { return check_sizes(type, d_hidden, ld_hidden, d_weight, ld_weight, rows, vocab, width); });
+  return rc == PST_OK ? plan_loss(type, d_hidden, ld_hidden, d_weight, ld_weight, rows, vocab, width).bytes : rc;
 }
 
 int pst_token_loss(int32_t device, int32_t type, const void* d_hidden, int64_t ld_hidden, const void* d_weight, int64_t ld_weight, int64_t rows,
@@ -1566,11 +1563,8 @@ int pst_token_loss(int32_t device, int32_t type, const void* d_hidden, int64_t l
 int64_t pst_token_loss_grad_workspace(int32_t type, const void* d_hidden, int64_t ld_hidden, const void* d_weight, int64_t ld_weight, int64_t rows,
                                       int64_t vocab, int64_t width) {
   using namespace pst_head;
-  return guarded([&]() -> int {
-           return check_sizes(type, d_hidden, ld_hidden, d_weight, ld_weight, rows, vocab, width);
-         }) == PST_OK
-             ? plan_grad(type, d_hidden, ld_hidden, d_weight, ld_weight, std::max<int64_t>(rows, 1), vocab, width).bytes
-             : (int64_t)PST_E_INVALID;
+  const int rc = guarded([&]() -> int { return check_sizes(type, d_hidden, ld_hidden, d_weight, ld_weight, rows, vocab, width); });
+  return rc == PST_OK ? plan_grad(type, d_hidden, ld_hidden, d_weight, ld_weight, std::max<int64_t>(rows, 1), vocab, width).bytes : rc;
 }
 
 int pst_token_loss_grad(int32_t device, int32_t type, const void* d_hidden, int64_t ld_hidden, const void* d_weight, int64_t ld_weight, int64_t rows,
@@ -1593,11 +1587,8 @@ int pst_quantize_rows(int32_t device, int32_t type, const void* d_x, int64_t ld_
 int64_t pst_token_scores_i8_workspace(int32_t type, const void* d_hidden, int64_t ld_hidden, const int8_t* d_weight, int64_t ld_weight, int64_t rows,
                                       int64_t vocab, int64_t width) {
   using namespace pst_head;
-  return guarded([&]() -> int {
-           return check_scores(type, d_hidden, ld_hidden, d_weight, ld_weight, rows, vocab, width);
-         }) == PST_OK
-             ? plan_scores(d_weight, ld_weight, rows, vocab, width).bytes
-             : (int64_t)PST_E_INVALID;
+  const int rc = guarded([&]() -> int { return check_scores(type, d_hidden, ld_hidden, d_weight, ld_weight, rows, vocab, width); });
+  return rc == PST_OK ? plan_scores(d_weight, ld_weight, rows, vocab, width).bytes : rc;
 }
 
 int pst_token_scores_i8(int32_t device, int32_t type, const void* d_hidden, int64_t ld_hidden, const int8_t* d_weight, int64_t ld_weight,

@@ -10,7 +10,8 @@ scores over the implicit codebook).
 Arguments are torch tensors on one GPU: matrices with unit column stride and any row stride. Calls launch on torch's
 current stream of that GPU and do not synchronise; workspaces come from torch's allocator, so calls on several streams
 and captured graphs each have their own. Types: float32, bfloat16, float16 (hidden and weight of the same type).
-`ValueError` names an argument that does not fit, `PstError` what the runtime reported. torch has to be imported before
+`ValueError` names an argument that does not fit, `NotImplementedError` a size past the limits (2^30 rows or ids,
+2^20 columns, 131072 of 8-bit scores), `PstError` what the runtime reported. torch has to be imported before
 pst_amd loads libpst, so that both use one HIP runtime.
 """
 import functools

@@ -129,3 +129,14 @@ def test_another_thread_s_first_call_sees_all_of_the_set_up(monkeypatch):
     assert head._torch() is torch
     # while the table of target types is filled nobody is told that it is there
     assert order and all(m is None for m in order) and set(head._target_bits) == {torch.int32, torch.int64}
+
+
+def test_workspaces_of_sizes_that_are_too_large():
+    L = _native.lib()
+    for fn in ("pst_token_loss_workspace", "pst_token_loss_grad_workspace", "pst_token_scores_i8_workspace"):
+        for rows, vocab, width in ((1 << 31, 8, 64), (4, 1 << 31, 64), (4, 8, 1 << 21)):
+            args = (BF16, P, max(width, 64), P, max(width, 64), rows, vocab, width)
+            assert getattr(L, fn)(*args) == _native.PST_E_TOO_LARGE
+            assert b"over 2^30" in L.pst_head_error()
+            with pytest.raises(NotImplementedError, match="2\\^30"):
+                head._workspace_bytes(fn, *args)
