@@ -3,6 +3,7 @@ ids that the tokenizer makes (`include/pst.h`, section "Token head"; `Tokenizer.
 scores over the implicit codebook).
 
     loss, lse = token_loss(hidden, weight, targets)              # softmax cross entropy per position, no logits kept
+    loss.sum().backward()                                        # where hidden or weight requires grad, or by hand:
     dhidden, dweight = token_loss_grad(hidden, weight, targets, lse, grad_loss)
     qweight, scale = quantize_rows(weight)                       # once
     scores = token_scores_int8(hidden, qweight, scale)           # 8-bit products, a scale for each row and each id
@@ -125,13 +126,54 @@ def _targets(targets, rows, device):
     return _vector(targets, "targets", rows, device), bits
 
 
+_function = None
+
+
+def _differentiable(torch):
+    """token_loss as an autograd function, made on first use."""
+    global _function
+    if _function is None:
+        class TokenLoss(torch.autograd.Function):
+            @staticmethod
+            def forward(ctx, hidden, weight, targets, ignore_index):
+                loss, lse = _loss(torch, hidden, weight, targets, ignore_index)
+                ctx.save_for_backward(hidden, weight, targets, lse)
+                ctx.ignore_index = ignore_index
+                ctx.set_materialize_grads(False)
+                return loss, lse
+
+            @staticmethod
+            @torch.autograd.function.once_differentiable
+            def backward(ctx, grad_loss, grad_lse):
+                if grad_lse is not None:
+                    raise NotImplementedError("lse of token_loss has no gradient: use loss, or lse.detach()")
+                if grad_loss is None:
+                    return None, None, None, None
+                hidden, weight, targets, lse = ctx.saved_tensors
+                need_hidden, need_weight = ctx.needs_input_grad[:2]
+                return (*token_loss_grad(hidden, weight, targets, lse, grad_loss.contiguous(), ignore_index=ctx.ignore_index,
+                                         need_hidden=need_hidden, need_weight=need_weight), None, None)
+
+        _function = TokenLoss
+    return _function
+
+
 def token_loss(hidden, weight, targets, *, ignore_index=-100):
     """Softmax cross entropy of each position over the vocabulary: (loss [N], lse [N]) in float32,
     lse[n] = log sum_v exp(<hidden[n], weight[v]>), loss[n] = lse[n] - <hidden[n], weight[targets[n]]>.
 
     `hidden` [N, d], `weight` [V, d], `targets` [N] int64 or int32. Positions whose target is `ignore_index` have loss
-    0; a target outside [0, V) that is not `ignore_index` gives loss NaN. `lse` is what `token_loss_grad` takes."""
+    0; a target outside [0, V) that is not `ignore_index` gives loss NaN. `lse` is what `token_loss_grad` takes.
+
+    Where grad mode is on and `hidden` or `weight` requires grad, `loss` is differentiable (once) by `token_loss_grad`; a
+    gradient that arrives at `lse` raises `NotImplementedError`."""
     torch = _torch()
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        return _differentiable(torch).apply(hidden, weight, targets, ignore_index)
+    return _loss(torch, hidden, weight, targets, ignore_index)
+
+
+def _loss(torch, hidden, weight, targets, ignore_index):
     device, code, x, ldx, w, ldw = _head(torch, hidden, weight)
     rows, width = hidden.shape
     vocab = weight.shape[0]
@@ -146,7 +188,8 @@ def token_loss(hidden, weight, targets, *, ignore_index=-100):
 
 
 def token_loss_grad(hidden, weight, targets, lse, grad_loss, *, ignore_index=-100, need_hidden=True, need_weight=True):
-    """Gradients of sum_n grad_loss[n] loss[n]: (for hidden, for weight), of their type; None where not needed.
+    """Gradients of sum_n grad_loss[n] loss[n]: (for hidden, for weight), of their type; None where not needed. They are
+    detached: what autograd has for `token_loss`, called by hand.
 
     `lse` [N] float32 from `token_loss`, `grad_loss` [N] float32. Positions whose target is `ignore_index` have zero
     gradient and add nothing to the weight's, whatever their hidden row holds; a target out of range gives NaN. The logits' gradient is held to 2^-16 of each entry for 16-bit types.
@@ -191,7 +234,7 @@ def token_scores_int8(hidden, qweight, scale, *, out_dtype=None):
     """Scores [N, V] of all token ids in 8-bit products: hidden's rows are rounded to 8 bits with a scale each
     (`quantize_rows`' rule) within the call, `qweight` int8 [V, d] and `scale` float32 [V] are `quantize_rows` of the
     table. Sums are exact. `out_dtype`: float32, bfloat16 or float16, hidden's by default. The result's rows are
-    aligned: its row stride is V rounded up to a multiple of 64."""
+    aligned: its row stride is V rounded up to a multiple of 64. They are detached: rounding has no gradient."""
     torch = _torch()
     device = _device(hidden, "hidden")
     code = _code(hidden, "hidden")
