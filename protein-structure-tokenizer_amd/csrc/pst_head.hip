@@ -1114,7 +1114,7 @@ struct Plan {
   int64_t part = 0, tlogit = 0;                  // loss
   int64_t xh = 0, wh = 0, D = 0, dxp = 0, dwp = 0;  // gradient
   int64_t few = 0;                               // k_few: 16-row blocks a workgroup
-  int64_t piece = 0;                             // vocabulary rows of a piece
+  int64_t span = 0, piece = 0;                   // positions and vocabulary rows of a piece of D
   int tile = 0, zx = 1, zw = 1;                  // of the two gradients' launch
   int64_t bytes = 0;
 };
@@ -1202,18 +1202,22 @@ void split_grads(Plan& p, int64_t nv, bool pieces) {
   p.zx = last.zx;
   p.zw = last.zw;
 }
-// Vocabulary rows of a piece: D takes about what the last-level cache (256 MB) holds, but a piece has 4096 rows at least,
-// since each adds to all of dx's sums in memory.
-constexpr int64_t PIECE_BYTES = 288ll << 20, PIECE_LEAST = 4096;
+// D is made in pieces of about what the last-level cache (256 MB) holds: of all positions by as many vocabulary rows, or of
+// SPAN positions at least, since each piece of the vocabulary adds to the sums of its positions' dx in memory, and each
+// span of positions to those of all of dW.
+constexpr int64_t PIECE_BYTES = 288ll << 20, SPAN = 8192;
 Plan plan_grad(int type, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab, int64_t width) {
+  const int64_t longest = std::max(SPAN, PIECE_BYTES / (4 * up(vocab, 256)) / 256 * 256);
+  const int64_t span = rows <= longest ? rows : up(ceil_div(rows, ceil_div(rows, longest)), 256);
   Bump b;
-  Plan p = plan_common(type, x, ldx, w, ldw, rows, vocab, width, true, b);
+  Plan p = plan_common(type, x, ldx, w, ldw, span, vocab, width, true, b);
+  p.span = span;
   if (type == PST_F16) {
     p.xh = b.take(p.rows_pad * p.width_pad * 4);
     p.wh = b.take(vocab * p.width_pad * 4);
   }
-  const int64_t drows = up(rows, 256);
-  int64_t most = std::max<int64_t>(PIECE_LEAST, PIECE_BYTES / (drows * 4) / 256 * 256);
+  const int64_t drows = up(span, 256);
+  int64_t most = PIECE_BYTES / (drows * 4) / 256 * 256;
   // several pieces: of a size that gives both gradients' largest tiles in whole rounds, where that is not much smaller
   const int64_t across = ceil_div(p.width_pad, 256), round = CUS / across * 256;
   const int64_t first = (CUS - across * (drows / 256) % CUS) / across * 256;
@@ -1222,8 +1226,8 @@ Plan plan_grad(int type, const void* x, int64_t ldx, const void* w, int64_t ldw,
   p.piece = vocab > most ? most : up(vocab, 256);
   p.D = b.take(drows * p.piece * 4);
   split_grads(p, std::min(p.piece, vocab), vocab > p.piece);
-  p.dxp = b.take(p.zx * rows * p.width_pad * 4);
-  if (p.zw > 1) p.dwp = b.take(p.zw * vocab * p.width_pad * 4);
+  p.dxp = b.take(p.zx * span * p.width_pad * 4);
+  if (p.zw > 1 || rows > span) p.dwp = b.take(p.zw * vocab * p.width_pad * 4);
   p.bytes = b.n;
   return p;
 }
@@ -1258,9 +1262,9 @@ int32_t row_grid(int64_t rows, int64_t per_row) {
 }
 
 // the operands in a form that the products read: in place, or packed into the workspace; for the gradient (`grad`) of f16
-// also their bf16 halves. One launch, none where there is nothing to do.
-int operands(const Plan& p, const void* x, int64_t ldx, const void* w, int64_t ldw, const Targets& t, bool grad, char* ws, hipStream_t st,
-             Operand* X, Operand* W) {
+// also their bf16 halves; `table`: the table's too, or they are there. One launch, none where there is nothing to do.
+int operands(const Plan& p, const void* x, int64_t ldx, int64_t rows, const void* w, int64_t ldw, bool table, const Targets& t, bool grad, char* ws,
+             hipStream_t st, Operand* X, Operand* W) {
   const int e = size_of(p.type);
   PackArgs a{};
   a.bytes = (int32_t)(p.width * e);
@@ -1274,10 +1278,11 @@ int operands(const Plan& p, const void* x, int64_t ldx, const void* w, int64_t l
          ((uintptr_t)src & 15) == 0 && ld * e % 16 == 0};
     a.blocks[which] = row_grid(rows_pad, a.bytes_pad / (j.wide ? 16 : 4));
   };
-  *X = p.pack_x ? Operand{ws + p.x, 0, a.bytes_pad, (int32_t)p.rows_pad, a.bytes_pad} : Operand{(const char*)x, 0, ldx * e, (int32_t)p.rows, a.bytes};
+  const int64_t rows_pad = grad ? up(std::max<int64_t>(rows, 1), 64) : rows;
+  *X = p.pack_x ? Operand{ws + p.x, 0, a.bytes_pad, (int32_t)rows_pad, a.bytes_pad} : Operand{(const char*)x, 0, ldx * e, (int32_t)rows, a.bytes};
   *W = p.pack_w ? Operand{ws + p.w, 0, a.bytes_pad, (int32_t)p.vocab, a.bytes_pad} : Operand{(const char*)w, 0, ldw * e, (int32_t)p.vocab, a.bytes};
-  if (p.pack_x) job(0, x, ldx, p.rows, p.rows_pad, true, p.x, p.xh);
-  if (p.pack_w || halves) job(1, w, ldw, p.vocab, p.vocab, p.pack_w, p.w, p.wh);
+  if (p.pack_x) job(0, x, ldx, rows, rows_pad, true, p.x, p.xh);
+  if (table && (p.pack_w || halves)) job(1, w, ldw, p.vocab, p.vocab, p.pack_w, p.w, p.wh);
   if (a.blocks[0] + a.blocks[1]) {
     hipLaunchKernelGGL(k_pack, dim3((unsigned)(a.blocks[0] + a.blocks[1])), dim3(256), 0, st, a);
     HEADCHK(hipGetLastError());
@@ -1317,7 +1322,7 @@ int token_loss(int device, int type, const void* x, int64_t ldx, const void* w, 
     HEADCHK(hipGetLastError());
     return PST_OK;
   }
-  rc = operands(p, x, ldx, w, ldw, g.targets, false, ws, st, &g.B, &g.A);
+  rc = operands(p, x, ldx, rows, w, ldw, true, g.targets, false, ws, st, &g.B, &g.A);
   if (rc != PST_OK) return rc;
   g.M = (int32_t)vocab;
   g.N = (int32_t)rows;
@@ -1350,85 +1355,86 @@ int token_loss_grad(int device, int type, const void* x, int64_t ldx, const void
   OnDevice on(device);
   if (on.e != hipSuccess) return hip_fail("device " + std::to_string(device), on.e);
   char* ws = (char*)ws_;
-  const Targets t{targets, ignore, tbits, (int32_t)vocab};
-  // no positions: 64 of zeros stand for them, so that dW is written as the zeros that it is
-  Plan q = p;
-  q.rows = rows;
-  Operand X, W;
-  rc = operands(q, x, ldx, w, ldw, t, true, ws, st, &X, &W);
-  if (rc != PST_OK) return rc;
-  const int de = p.type == PST_F32 ? 4 : 2, ks = STEP / de;  // bytes of D's values, K-steps' values
+  const int de = type == PST_F32 ? 4 : 2, ks = STEP / de;  // bytes of D's values, K-steps' values
   char* D = ws + p.D;
-  const int64_t drows = up(std::max<int64_t>(rows, 1), 256);
-  const bool need_dx = dx && rows;
-  // what the gradients' products read
-  const Operand Xh = p.type == PST_F16 ? Operand{ws + p.xh, X.rows * X.ld, X.ld, X.rows, X.bytes} : X;
-  const Operand Wh = p.type == PST_F16 ? Operand{ws + p.wh, vocab * X.ld, X.ld, (int32_t)vocab, X.bytes} : W;
-  for (int64_t v0 = 0; v0 < vocab; v0 += p.piece) {
-    const int64_t nv = std::min(p.piece, vocab - v0), ldd = up(nv, 256);
-    const Operand dop{D, drows * ldd * de, ldd * de, (int32_t)drows, (int32_t)ldd * de};
-    Operand Wv = W;
-    Wv.p += v0 * W.ld;
-    Wv.rows = (int32_t)nv;
-    GemmArgs g{};
-    g.A = Wv;
-    g.B = X;
-    g.M = (int32_t)nv;
-    g.N = (int32_t)rows;
-    g.steps = (int32_t)(p.width_pad * e / STEP);
-    g.targets = t;
-    g.lse = lse;
-    g.gloss = gloss;
-    g.D = D;
-    g.dplane = dop.plane;
-    g.ldd = ldd;
-    g.v0 = (int32_t)v0;
-    if (rows) HEADCHK(launch_gemm(DLOGIT, p.elem, tile_for(nv, rows, g.steps, p.type == PST_F32, 4), g, st));
-    GradArgs b{};
-    b.dx.A = Wh;
-    b.dx.A.p += v0 * Wh.ld;
-    b.dx.A.rows = (int32_t)nv;
-    b.dx.B = b.dw.B = dop;
-    b.dx.M = b.dw.M = (int32_t)width;
-    b.dx.N = (int32_t)rows;
-    b.dx.range = (int32_t)ceil_div(nv, ks);
-    b.dw.range = (int32_t)ceil_div(rows, ks);
-    b.dx.products = b.dw.products = p.products;
-    b.dx.steps = b.dx.range * p.products;
-    b.dw.steps = b.dw.range * p.products;
-    b.dx.nz = p.zx;
-    b.dx.part_out = (float*)(ws + p.dxp);
-    b.dx.ldp = b.dw.ldp = p.width_pad;
-    b.dx.zstride = rows * p.width_pad;
-    b.dx.add = v0 > 0;
-    b.dw.A = Xh;
-    b.dw.N = (int32_t)nv;
-    b.dw.nz = p.zw;
-    b.dw.v0 = (int32_t)v0;
-    b.dw.out = dw;
-    b.dw.ldo = lddw;
-    b.dw.otype = type;
-    b.dw.wide = lddw % (16 / e) == 0 && ((uintptr_t)dw & 15) == 0;
-    if (p.zw > 1) {
-      b.dw.part_out = (float*)(ws + p.dwp);
-      b.dw.zstride = vocab * p.width_pad;
+  const bool spans = rows > p.span;
+  // no positions: 64 of zeros stand for them, so that dW is written as the zeros that it is
+  for (int64_t n0 = 0; n0 < std::max<int64_t>(rows, 1); n0 += p.span) {
+    const int64_t n = std::min(p.span, rows - n0), drows = up(std::max<int64_t>(n, 1), 256);
+    const bool last = n0 + p.span >= rows, need_dx = dx && n;
+    const Targets t{targets ? (const char*)targets + n0 * (tbits / 8) : nullptr, ignore, tbits, (int32_t)vocab};
+    Operand X, W;
+    rc = operands(p, x ? (const char*)x + n0 * ldx * e : nullptr, ldx, n, w, ldw, n0 == 0, t, true, ws, st, &X, &W);
+    if (rc != PST_OK) return rc;
+    // what the gradients' products read
+    const Operand Xh = type == PST_F16 ? Operand{ws + p.xh, X.rows * X.ld, X.ld, X.rows, X.bytes} : X;
+    const Operand Wh = type == PST_F16 ? Operand{ws + p.wh, vocab * X.ld, X.ld, (int32_t)vocab, X.bytes} : W;
+    for (int64_t v0 = 0; v0 < vocab; v0 += p.piece) {
+      const int64_t nv = std::min(p.piece, vocab - v0), ldd = up(nv, 256);
+      const Operand dop{D, drows * ldd * de, ldd * de, (int32_t)drows, (int32_t)(ldd * de)};
+      GemmArgs g{};
+      g.A = W;
+      g.A.p += v0 * W.ld;
+      g.A.rows = (int32_t)nv;
+      g.B = X;
+      g.M = (int32_t)nv;
+      g.N = (int32_t)n;
+      g.steps = (int32_t)(p.width_pad * e / STEP);
+      g.targets = t;
+      g.lse = lse + n0;
+      g.gloss = gloss + n0;
+      g.D = D;
+      g.dplane = dop.plane;
+      g.ldd = ldd;
+      g.v0 = (int32_t)v0;
+      if (n) HEADCHK(launch_gemm(DLOGIT, p.elem, tile_for(nv, n, g.steps, type == PST_F32, 4), g, st));
+      GradArgs b{};
+      b.dx.A = Wh;
+      b.dx.A.p += v0 * Wh.ld;
+      b.dx.A.rows = (int32_t)nv;
+      b.dw.A = Xh;
+      b.dx.B = b.dw.B = dop;
+      b.dx.M = b.dw.M = (int32_t)width;
+      b.dx.N = (int32_t)n;
+      b.dw.N = (int32_t)nv;
+      b.dx.range = (int32_t)ceil_div(nv, ks);
+      b.dw.range = (int32_t)ceil_div(n, ks);
+      b.dx.products = b.dw.products = p.products;
+      b.dx.steps = b.dx.range * p.products;
+      b.dw.steps = b.dw.range * p.products;
+      b.dx.nz = p.zx;
+      b.dw.nz = p.zw;
+      b.dx.ldp = b.dw.ldp = p.width_pad;
+      b.dx.part_out = (float*)(ws + p.dxp);
+      b.dx.zstride = n * p.width_pad;
+      b.dx.add = v0 > 0;
+      if (p.zw > 1 || spans) {
+        b.dw.part_out = (float*)(ws + p.dwp) + v0 * p.width_pad;
+        b.dw.zstride = vocab * p.width_pad;
+        b.dw.add = n0 > 0;
+      }
+      b.dw.v0 = (int32_t)v0;
+      b.dw.out = dw;
+      b.dw.ldo = lddw;
+      b.dw.otype = type;
+      b.dw.wide = lddw % (16 / e) == 0 && ((uintptr_t)dw & 15) == 0;
+      HEADCHK(launch_grads(p.tile, b, need_dx, dw != nullptr, st));
     }
-    HEADCHK(launch_grads(p.tile, b, need_dx, dw != nullptr, st));
-  }
-  FinishArgs f{};
-  f.width = (int32_t)width;
-  f.otype = type;
-  f.targets = t;
-  auto job = [&](int which, int64_t part, int64_t n, int nz, void* out, int64_t ldo) {
-    f.job[which] = {(const float*)(ws + part), p.width_pad, n * p.width_pad, n, nz, which == 0, out, ldo,
-                    ldo % 4 == 0 && ((uintptr_t)out & (type == PST_F32 ? 15 : 7)) == 0};
-    f.blocks[which] = row_grid(n, ceil_div(width, 4));
-  };
-  if (need_dx) job(0, p.dxp, rows, p.zx, dx, lddx);
-  if (dw && p.zw > 1) job(1, p.dwp, vocab, p.zw, dw, lddw);
-  if (f.blocks[0] + f.blocks[1]) {
-    hipLaunchKernelGGL(k_finish, dim3((unsigned)(f.blocks[0] + f.blocks[1])), dim3(256), 0, st, f);
-    HEADCHK(hipGetLastError());
+    FinishArgs f{};
+    f.width = (int32_t)width;
+    f.otype = type;
+    f.targets = t;
+    auto job = [&](int which, int64_t part, int64_t count, int nz, char* out, int64_t ldo) {
+      f.job[which] = {(const float*)(ws + part), p.width_pad, count * p.width_pad, count, nz, which == 0, out, ldo,
+                      ldo % 4 == 0 && ((uintptr_t)out & (type == PST_F32 ? 15 : 7)) == 0};
+      f.blocks[which] = row_grid(count, ceil_div(width, 4));
+    };
+    if (need_dx) job(0, p.dxp, n, p.zx, (char*)dx + n0 * lddx * e, lddx);
+    if (dw && last && (p.zw > 1 || spans)) job(1, p.dwp, vocab, p.zw, (char*)dw, lddw);
+    if (f.blocks[0] + f.blocks[1]) {
+      hipLaunchKernelGGL(k_finish, dim3((unsigned)(f.blocks[0] + f.blocks[1])), dim3(256), 0, st, f);
+      HEADCHK(hipGetLastError());
+    }
   }
   return PST_OK;
 }

@@ -193,3 +193,16 @@ def test_masks_of_infinity(rows, vocab, width, dtype):
     # (the bias column of hidden's gradient is a sum over 0 (-inf))
     dx, _ = check_grad(x, w, t, gl, lse, columns=slice(0, -1))
     assert not dx[t != -100, -1].isfinite().any()
+
+
+# more positions than a piece of the logits' gradient holds: the table's gradient is summed over the pieces
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("rows,vocab,width", [(20000, 9001, 40), (8193, 16000, 24), (299000, 50, 16)])
+def test_pieces_of_the_positions(rows, vocab, width, dtype):
+    x, w, t, gl = make(rows, vocab, width, dtype, seed=6)
+    lse = head.token_loss(x, w, t)[1]
+    dx, dw = check_grad(x, w, t, gl, lse)
+    a, none = head.token_loss_grad(x, w, t, lse, gl, need_weight=False)
+    assert none is None and torch.equal(a, dx)
+    none, b = head.token_loss_grad(x, w, t, lse, gl, need_hidden=False)
+    assert none is None and torch.equal(b, dw)

@@ -140,3 +140,15 @@ def test_workspaces_of_sizes_that_are_too_large():
             assert b"over 2^30" in L.pst_head_error()
             with pytest.raises(NotImplementedError, match="2\\^30"):
                 head._workspace_bytes(fn, *args)
+
+
+@pytest.mark.parametrize("type,size", [(BF16, 2), (F16, 2), (F32, 4)])
+def test_the_gradient_s_workspace_does_not_grow_with_the_positions(type, size):
+    L = _native.lib()
+    for vocab, width in ((64003, 1024), (4099, 1024), (432, 256)):
+        # pieces of the logits' gradient, and of the positions that have one: copies of hidden (float16: and halves) and
+        # up to eight sums of its gradient; up to two sums of all of the weight's (float16: and its halves)
+        span = max(8192, (288 << 20) // (4 * ((vocab + 255) // 256 * 256)))
+        most = (288 << 20) + span * width * (size + 4 + 4 * 8) + vocab * width * 4 * 3 + 4096
+        for rows in (131072, 524288, 1 << 24):
+            assert 0 < L.pst_token_loss_grad_workspace(type, P, width, P, width, rows, vocab, width) <= most
