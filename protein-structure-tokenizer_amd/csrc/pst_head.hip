@@ -1022,7 +1022,7 @@ int64_t thin_rows(int64_t m, int tile) {
   return THIN[tile] > 0 && m > rest && rest <= 64 ? rest : 0;
 }
 // m x n of the loss, the logits' gradient and the scores; a compute unit stores about 20 KB in a us (5 TB/s of all)
-int tile_for(int64_t m, int64_t n, int64_t steps, bool f32, int out_bytes) {
+int tile_for(int64_t m, int64_t n, int64_t steps, bool f32, int out_bytes, double* estimate = nullptr) {
   int best = TILE64;
   double us = 1e30;
   for (int t = f32 ? FLOAT128 : TILE256; t >= (f32 ? FLOAT64 : TILE64); --t) {
@@ -1033,6 +1033,7 @@ int tile_for(int64_t m, int64_t n, int64_t steps, bool f32, int out_bytes) {
     if (thin && full + ceil_div(n, 64) > ceil_div(full, slots) * slots) e += THIN[t] * one;  // not into what the last round leaves free
     if (e < us) us = e, best = t;
   }
+  if (estimate) *estimate = us;
   return best;
 }
 
@@ -1158,46 +1159,62 @@ Plan plan_loss(int type, const void* x, int64_t ldx, const void* w, int64_t ldw,
   p.bytes = b.n;
   return p;
 }
-// The tiles of the two gradients' launch and the parts zx, zw of their K loops: the least of the estimated launch and of
-// the parts' way back through memory (4.5 TB/s). 32-bit operands: tiles of 64 alone, which fill the card sooner and lose nothing
-// to those of 128 (both gradients, us: 300 x 432 x 512 29 and 36, 4096 x 4099 x 512 427 and 455, 2048 x 8192 x 2048 1493
-// and 1481). The last choice is kept, by the sizes alone.
-void split_grads(Plan& p, int64_t nv, bool pieces) {
+// The tiles of the two gradients' launch and the parts zx, zw of their K loops, for pieces of nv vocabulary rows: the least of
+// the estimated launch and of the parts' way back through memory (4.5 TB/s), which is returned. 32-bit operands: tiles of 64
+// alone, which fill the card sooner and lose nothing to those of 128 (both gradients, us: 300 x 432 x 512 29 and 36,
+// 4096 x 4099 x 512 427 and 455, 2048 x 8192 x 2048 1493 and 1481).
+double split_grads(Plan& p, int64_t nv, bool pieces) {
+  constexpr int Z[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
+  const bool f32 = p.type == PST_F32;
+  const int64_t ks = STEP / (f32 ? 4 : 2), sx = p.products * ceil_div(nv, ks), sw = p.products * ceil_div(p.rows, ks), least = 4;
+  double best = 1e30;
+  for (int t = f32 ? FLOAT64 : TILE256; t >= (f32 ? FLOAT64 : TILE64); --t) {
+    const int64_t thin_x = thin_rows(p.rows, t), thin_w = thin_rows(nv, t);
+    const double slots = (double)CUS * TILE_SLOTS[t];
+    const double one_x = tiles_of(p.width_pad, p.rows - thin_x, t), one_w = tiles_of(p.width, nv - thin_w, t);
+    const double thins_x = thin_x ? ceil_div(p.width_pad, 64) : 0, thins_w = thin_w ? ceil_div(p.width, 64) : 0;
+    for (int zx : Z)
+      for (int zw : Z) {
+        if ((zx > 1 && sx < least * zx) || (zw > 1 && (pieces || sw < least * zw))) continue;
+        const double n = one_x * zx + one_w * zw, thins = thins_x * zx + thins_w * zw;
+        const double tx = tile_us(t, n, ceil_div(sx, zx)), tw = tile_us(t, n, ceil_div(sw, zw)), longest = std::max(tx, tw);
+        double us = longest;
+        // both kinds share the slots; the last to start ends half its time behind the rest
+        if (n > slots) us = std::max((one_x * zx * tx + one_w * zw * tw) / slots + 0.5 * longest, longest + std::min(tx, tw));
+        if (n + thins > ceil_div((int64_t)n, (int64_t)slots) * slots) us += THIN[t] * longest;
+        us += 4.0 * p.width_pad * (p.rows * (double)zx + (zw > 1 ? nv * (double)zw : 0.0)) / 4.5e6 + 0.3 * (zx + zw);
+        if (us < best) best = us, p.tile = t, p.zx = zx, p.zw = zw;
+      }
+  }
+  return best;
+}
+// The vocabulary rows of a piece, `most` at most, and how its gradients are made: of the fewest pieces and a few more, what is
+// estimated to take least, since a piece whose tiles fill the card unevenly, or whose two gradients have K loops of very different
+// lengths, costs more than another launch. By a rule that filled whole rounds alone, and so (bf16, ms): 8448 x 64003 x 1024
+// 5.8 and 5.0, 2048 x 64003 x 1024 1.46 and 1.22, 8192 x 64003 x 1024 4.55 and 4.55. The last choice
+// is kept, by the sizes alone.
+void choose_pieces(Plan& p, int64_t most) {
   struct Last {
-    int64_t rows = -1, nv, width;
+    int64_t rows = -1, vocab, width, piece;
     int products, tile, zx, zw;
-    bool pieces;
   };
   thread_local Last last;
-  if (last.rows != p.rows || last.nv != nv || last.width != p.width || last.products != p.products || last.pieces != pieces) {
-    constexpr int Z[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
-    const bool f32 = p.type == PST_F32;
-    const int64_t ks = STEP / (f32 ? 4 : 2), sx = p.products * ceil_div(nv, ks), sw = p.products * ceil_div(p.rows, ks), least = 4;
+  if (last.rows != p.rows || last.vocab != p.vocab || last.width != p.width || last.products != p.products) {
+    const int64_t fewest = ceil_div(p.vocab, most), steps = p.width_pad * size_of(p.type) / STEP;
     double best = 1e30;
-    for (int t = f32 ? FLOAT64 : TILE256; t >= (f32 ? FLOAT64 : TILE64); --t) {
-      const int64_t thin_x = thin_rows(p.rows, t), thin_w = thin_rows(nv, t);
-      const double slots = (double)CUS * TILE_SLOTS[t];
-      const double one_x = tiles_of(p.width_pad, p.rows - thin_x, t), one_w = tiles_of(p.width, nv - thin_w, t);
-      const double thins_x = thin_x ? ceil_div(p.width_pad, 64) : 0, thins_w = thin_w ? ceil_div(p.width, 64) : 0;
-      for (int zx : Z)
-        for (int zw : Z) {
-          if ((zx > 1 && sx < least * zx) || (zw > 1 && (pieces || sw < least * zw))) continue;
-          const double n = one_x * zx + one_w * zw, thins = thins_x * zx + thins_w * zw;
-          const double tx = tile_us(t, n, ceil_div(sx, zx)), tw = tile_us(t, n, ceil_div(sw, zw)), longest = std::max(tx, tw);
-          double us = longest;
-          // both kinds share the slots; the last to start ends half its time behind the rest
-          if (n > slots) us = std::max((one_x * zx * tx + one_w * zw * tw) / slots + 0.5 * longest, longest + std::min(tx, tw));
-          if (n + thins > ceil_div((int64_t)n, (int64_t)slots) * slots) us += THIN[t] * longest;
-          us += 4.0 * p.width_pad * (p.rows * (double)zx + (zw > 1 ? nv * (double)zw : 0.0)) / 4.5e6 + 0.3 * (zx + zw);
-          if (us < best) best = us, last.tile = t, last.zx = zx, last.zw = zw;
-        }
+    for (int64_t k = fewest; k <= (fewest > 1 ? fewest + 8 : 1); ++k) {
+      const int64_t piece = up(ceil_div(p.vocab, k), 256);
+      double us;
+      (void)tile_for(std::min(piece, p.vocab), p.rows, steps, p.type == PST_F32, 4, &us);
+      us = (us + split_grads(p, std::min(piece, p.vocab), k > 1) + 10.0) * ceil_div(p.vocab, piece);
+      if (us < best) best = us, last.piece = piece, last.tile = p.tile, last.zx = p.zx, last.zw = p.zw;
     }
     last.rows = p.rows;
-    last.nv = nv;
+    last.vocab = p.vocab;
     last.width = p.width;
     last.products = p.products;
-    last.pieces = pieces;
   }
+  p.piece = last.piece;
   p.tile = last.tile;
   p.zx = last.zx;
   p.zw = last.zw;
@@ -1217,15 +1234,8 @@ Plan plan_grad(int type, const void* x, int64_t ldx, const void* w, int64_t ldw,
     p.wh = b.take(vocab * p.width_pad * 4);
   }
   const int64_t drows = up(span, 256);
-  int64_t most = PIECE_BYTES / (drows * 4) / 256 * 256;
-  // several pieces: of a size that gives both gradients' largest tiles in whole rounds, where that is not much smaller
-  const int64_t across = ceil_div(p.width_pad, 256), round = CUS / across * 256;
-  const int64_t first = (CUS - across * (drows / 256) % CUS) / across * 256;
-  if (vocab > most && round > 0 && first > 0 && most >= first && first + (most - first) / round * round >= most / 2)
-    most = first + (most - first) / round * round;
-  p.piece = vocab > most ? most : up(vocab, 256);
+  choose_pieces(p, PIECE_BYTES / (drows * 4) / 256 * 256);
   p.D = b.take(drows * p.piece * 4);
-  split_grads(p, std::min(p.piece, vocab), vocab > p.piece);
   p.dxp = b.take(p.zx * span * p.width_pad * 4);
   if (p.zw > 1 || rows > span) p.dwp = b.take(p.zw * vocab * p.width_pad * 4);
   p.bytes = b.n;
