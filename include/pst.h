@@ -229,7 +229,8 @@ int pst_decoder_get_timing(pst_decoder* dec, float* ms);
  * Token head: operators over a learned table weight [V, d] with one row per token id (the codes of a codebook and,
  * usually, a few marks), for a sequence model over the ids that pst_tokenize makes; pst_codebook_aux gives the same
  * kind of scores over the implicit codebook. Matrices are row-major with unit column stride and row strides ld_* in
- * elements (any stride >= the row's length, any alignment of the type; 16-byte aligned rows of a multiple of 8 (16:
+ * elements (any stride >= the row's length, up to 2^21 in the loss and its gradient and 2^23 of the int8 table, else
+ * PST_E_TOO_LARGE; any alignment of the type; 16-byte aligned rows of a multiple of 8 (16:
  * int8) elements are read in place, others are copied into the workspace first). No context: a call names its device and
  * launches on `stream` (a hipStream_t of that device, NULL = its default stream) without synchronising, so it can be
  * captured into a graph; the calling thread's current device stays what it was. Calls on different streams or threads

@@ -8,7 +8,8 @@ scores over the implicit codebook).
     qweight, scale = quantize_rows(weight)                       # once
     scores = token_scores_int8(hidden, qweight, scale)           # 8-bit products, a scale for each row and each id
 
-Arguments are torch tensors on one GPU: matrices with unit column stride and any row stride. Calls launch on torch's
+Arguments are torch tensors on one GPU: matrices with unit column stride and any row stride (rows more than
+2^21 elements apart, 2^23 of an int8 table, are copied together first). Calls launch on torch's
 current stream of that GPU and do not synchronise; workspaces come from torch's allocator, so calls on several streams
 and captured graphs each have their own. Types: float32, bfloat16, float16 (hidden and weight of the same type).
 `ValueError` names an argument that does not fit, `NotImplementedError` a size past the limits (2^30 rows or ids,
@@ -77,6 +78,18 @@ def _matrix(t, name, device=None):
     return t.data_ptr(), s0
 
 
+_FAR, _FAR_INT8 = 1 << 21, 1 << 23  # row strides, in elements, that the kernels' offsets within a tile take
+
+
+def _near(t, name, device=None, far=_FAR):
+    """(matrix, pointer, row stride), a copy where the rows are further apart than `far`."""
+    p, ld = _matrix(t, name, device)
+    if ld > far:
+        t = t.contiguous()
+        p, ld = _matrix(t, name, device)
+    return t, p, ld
+
+
 def _vector(t, name, n, device, dtype=None):
     if t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
         raise ValueError(f"{name} has shape {tuple(t.shape)} and strides {t.stride()}: a contiguous vector of {n} is needed")
@@ -110,13 +123,13 @@ def _head(torch, hidden, weight):
     code = _code(hidden, "hidden")
     if weight.dtype != hidden.dtype:
         raise ValueError(f"weight is {weight.dtype} and hidden {hidden.dtype}: one type is needed")
-    x, ldx = _matrix(hidden, "hidden")
-    w, ldw = _matrix(weight, "weight", device)
+    hidden, x, ldx = _near(hidden, "hidden")
+    weight, w, ldw = _near(weight, "weight", device)
     if weight.shape[1] != hidden.shape[1]:
         raise ValueError(f"weight has {weight.shape[1]} columns and hidden {hidden.shape[1]}")
     if weight.shape[0] < 1 or weight.shape[1] < 1:
         raise ValueError(f"weight has shape {tuple(weight.shape)}: a row and a column are needed at least")
-    return device, code, x, ldx, w, ldw
+    return hidden, weight, device, code, x, ldx, w, ldw
 
 
 def _targets(targets, rows, device):
@@ -174,7 +187,7 @@ def token_loss(hidden, weight, targets, *, ignore_index=-100):
 
 
 def _loss(torch, hidden, weight, targets, ignore_index):
-    device, code, x, ldx, w, ldw = _head(torch, hidden, weight)
+    hidden, weight, device, code, x, ldx, w, ldw = _head(torch, hidden, weight)
     rows, width = hidden.shape
     vocab = weight.shape[0]
     t, bits = _targets(targets, rows, device)
@@ -195,7 +208,7 @@ def token_loss_grad(hidden, weight, targets, lse, grad_loss, *, ignore_index=-10
     gradient and add nothing to the weight's, whatever their hidden row holds; a target out of range gives NaN. The logits' gradient is held to 2^-16 of each entry for 16-bit types.
     float16: scale the loss, since gradients below 6e-8 vanish in the type."""
     torch = _torch()
-    device, code, x, ldx, w, ldw = _head(torch, hidden, weight)
+    hidden, weight, device, code, x, ldx, w, ldw = _head(torch, hidden, weight)
     rows, width = hidden.shape
     vocab = weight.shape[0]
     t, bits = _targets(targets, rows, device)
@@ -242,7 +255,7 @@ def token_scores_int8(hidden, qweight, scale, *, out_dtype=None):
     rows, width = hidden.shape
     if qweight.dtype != torch.int8:
         raise ValueError(f"qweight is {qweight.dtype}: int8 is needed")
-    w, ldw = _matrix(qweight, "qweight", device)
+    qweight, w, ldw = _near(qweight, "qweight", device, _FAR_INT8)
     vocab = qweight.shape[0]
     if qweight.shape[1] != width:
         raise ValueError(f"qweight has {qweight.shape[1]} columns and hidden {width}")

@@ -128,3 +128,32 @@ def test_captured_and_replayed():
         want = (loss, *head.token_loss_grad(a, b, t, lse, torch.full_like(loss, 1 / len(t))))
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(out, want))
+
+
+def test_rows_further_apart_than_the_kernels_take():
+    """The last positions of whole sequences, and tables that are slices of something wide: strides past 2^21 (int8 2^23)."""
+    states = torch.zeros(5, 4096, 1024, dtype=torch.bfloat16, device=DEV)
+    x, w, t = make(5, 40, 1024, torch.bfloat16)
+    states[:, -1] = x
+    far = states[:, -1]
+    assert far.stride(0) == 1 << 22
+    wide = torch.zeros(40, (1 << 21) + 8, dtype=torch.bfloat16, device=DEV)
+    wide[:, :1024] = w
+    loss, lse = head.token_loss(x, w, t)
+    gl = torch.ones_like(loss)
+    dx, dw = head.token_loss_grad(x, w, t, lse, gl)
+    for a, b in ((far, w), (x, wide[:, :1024]), (far, wide[:, :1024])):
+        got, got_lse = head.token_loss(a, b, t)
+        assert torch.equal(got, loss) and torch.equal(got_lse, lse)
+        assert all(torch.equal(p, q) for p, q in zip(head.token_loss_grad(a, b, t, lse, gl), (dx, dw)))
+    a = far.detach().requires_grad_()
+    head.token_loss(a, w, t)[0].sum().backward()
+    assert torch.equal(a.grad, dx)
+    q, s = head.quantize_rows(w)
+    fq, fs = head.quantize_rows(wide[:, :1024])
+    assert torch.equal(fq, q) and torch.equal(fs, s)
+    want = head.token_scores_int8(x, q, s)
+    held = torch.zeros(40, (1 << 23) + 16, dtype=torch.int8, device=DEV)
+    held[:, :1024] = q
+    for table in (q, held[:, :1024]):
+        assert torch.equal(head.token_scores_int8(far, table, s), want)
