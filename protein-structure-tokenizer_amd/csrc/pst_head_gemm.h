@@ -92,10 +92,14 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) {
 }
 
 // 16 bytes a lane from base + off to LDS at `lds` + 16 lane; nothing returns to registers. The M0 write needs a
-// wait state before the load reads it.
+// wait state before the load reads it. (M0 is named as clobbered, so that no value of the compiler's is taken to outlive it
+// there; that it is a reserved register is what the warning would say.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void load_lds(const char* base, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "m0", "memory");
 }
+#pragma clang diagnostic pop
 
 // All but the last N of this wave's loads have landed (they return in the order of their issue) and everything it read
 // from LDS has been read, then all waves meet.
