@@ -105,7 +105,8 @@ struct Spread {
   }
 };
 
-// A matrix copied into rows of whole K-steps with zeros behind. Bound by its bytes where they are many.
+// A matrix copied into rows of whole K-steps with zeros behind. Bound by its bytes where they are many: 8192 x 1024 bf16 8.3 us,
+// 1023 + 4099 odd rows of 333 f32, read four bytes at a time, 8.4; 8192 + 64003 rows of 1024 f16 into halves 73 (6.3 TB/s).
 struct PackJob {
   const char* src;
   int64_t ld;              // bytes
@@ -314,7 +315,8 @@ __device__ __forceinline__ void tiles(const GemmArgs& g, int tile, int stride, i
 // exp(l - maximum) in registers, then over the column's four lanes and the two wave rows, and 8 bytes a tile and position
 // go to memory. One exponential a logit (16 clocks of a SIMD for 64 of them) is 1/8 of the matrix work at d = 1024;
 // persistent workgroups load the next tile meanwhile.
-// 8192 x 64003 x 1024 bf16: 829 us, 1.30 PFLOP/s (the library's product of that shape alone, logits to memory: 961 us).
+// 8192 x 64003 x 1024 bf16: 858 us, 1.25 PFLOP/s (the library's product of that shape alone, logits to memory: 961 us);
+// 4096 x 4096 x 1024 f32 245 us a call, 0.140 PFLOP/s.
 struct LossEpilogue {
   struct Inputs {
     int target;
@@ -411,7 +413,7 @@ struct JoinArgs {
   float *loss, *lse;
   int32_t n, tiles;
 };
-// 1024 threads share the vocabulary tiles of COLS positions; 8192 positions of 251 tiles (16 MB): 7.7 us
+// 1024 threads share the vocabulary tiles of COLS positions; 8192 positions of 251 tiles (16 MB): 6.2 us
 template <int COLS>
 __global__ __launch_bounds__(1024) void k_join(JoinArgs a) {
   constexpr int ROWS = 1024 / COLS;
@@ -453,7 +455,7 @@ void launch_join(const JoinArgs& j, hipStream_t st) {
 // the largest |g|, would drop probabilities and weights far below it. (32-bit operands: D in 32 bits.) The second
 // half is a second run of the products (see Loop): 8192 x 64003 x 1024 bf16 4.46 ms, with hi alone 2.71.
 // exp(l - lse) as 2^((l - lse) log2 e): the difference first, so that large logits lose nothing in the product. Stores of
-// 16 bytes a lane.
+// 16 bytes a lane. 8192 x 8192 x 1024 bf16 144 us (0.95 PFLOP/s with 268 MB of halves); f32 1000 x 4096 x 512 39.
 template <int E>
 struct DlogitEpilogue {
   struct Inputs {
@@ -579,7 +581,7 @@ __device__ __forceinline__ void store_part(const f32x4 (&acc)[T::MI][T::NI], con
   }
 }
 
-// a gradient from its parts' sums; 2 x 3 parts of 4096 x 512 (50 MB, in the cache): 11 us
+// a gradient from its parts' sums; 4096 and 4099 rows of 512 from theirs (50 MB, in the cache): 11 us
 struct FinishJob {
   const float* part;
   int64_t ldp, zstride;
@@ -601,21 +603,22 @@ __global__ __launch_bounds__(256) void k_finish(FinishArgs a) {
   const int block = (int)blockIdx.x - (which ? a.blocks[0] : 0);
   const FinishJob& f = a.job[which];
   const Spread at_row(block, a.blocks[which], (a.width + 3) / 4);
-  for (int64_t n = at_row.row; n < f.rows; n += at_row.rows)
-  for (int c = at_row.piece * 4; c < a.width; c += at_row.pieces * 4) {
-    f32x4 s = {0, 0, 0, 0};
-#pragma unroll 4
-    for (int z = 0; z < f.nz; ++z) {
-      const f32x4 v = *(const f32x4*)(f.part + z * f.zstride + n * f.ldp + c);
-      s.x += v.x;
-      s.y += v.y;
-      s.z += v.z;
-      s.w += v.w;
-    }
+  for (int64_t n = at_row.row; n < f.rows; n += at_row.rows) {
     bool counts = true;
     if (f.rows_count) (void)target_of(a.targets, n, counts);
-    const float v[4] = {counts ? s.x : 0.0f, counts ? s.y : 0.0f, counts ? s.z : 0.0f, counts ? s.w : 0.0f};
-    store4(f.out, a.otype, n * f.ldo + c, v, a.width - c, f.wide);
+    for (int c = at_row.piece * 4; c < a.width; c += at_row.pieces * 4) {
+      f32x4 s = {0, 0, 0, 0};
+#pragma unroll 4
+      for (int z = 0; z < f.nz; ++z) {
+        const f32x4 v = *(const f32x4*)(f.part + z * f.zstride + n * f.ldp + c);
+        s.x += v.x;
+        s.y += v.y;
+        s.z += v.z;
+        s.w += v.w;
+      }
+      const float v[4] = {counts ? s.x : 0.0f, counts ? s.y : 0.0f, counts ? s.z : 0.0f, counts ? s.w : 0.0f};
+      store4(f.out, a.otype, n * f.ldo + c, v, a.width - c, f.wide);
+    }
   }
 }
 
@@ -666,8 +669,9 @@ __device__ __forceinline__ void store_rows(const f32x4 (&acc)[T::MI][T::NI], con
   else store_rows_of<PST_F32, T>(acc, g, p, row0);
 }
 
-// Both gradients of a piece of the vocabulary in one launch, since D feeds both and neither fills the card evenly (8192 x
-// 16384 x 1024 bf16: 426 us, 1.29 PFLOP/s; 4096 x 4099 x 512: 43 us together, 31 and 45 in launches of their own):
+// Both gradients of a piece of the vocabulary in one launch, since D feeds both and neither fills the card evenly (4096 x
+// 4099 x 512 with one plane of D: 43 us together, 31 and 45 in launches of their own; with both planes 75). 8192 x 8192 x 1024
+// bf16: 421 us, 1.31 PFLOP/s of the four products; f16 620 of its six; 1000 x 4096 x 512 f32 71, 0.119 of its two:
 // dx's parts (m = column, n = position, k = vocabulary row of the piece, its K loop in nz parts) and rows v0 ... of dW
 // (m = column, n = vocabulary row, k = position; in one part straight to the output, or in parts as dx).
 template <int E, class T, bool DX>
@@ -699,9 +703,9 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES) void k_grads(GradArgs g) {
   }
 }
 
-// 8-bit scores: m = vocabulary row, n = position. Few positions are bound by the table's bytes: 16 x 64003 x 1024 12.8 us,
-// 5.3 TB/s with the scores; many by power, as the other products, and by their stores: 8192 x 64003 x 1024 to bf16 618 us,
-// 1.74 POP/s and 1.7 TB/s.
+// 8-bit scores: m = vocabulary row, n = position. Few positions are bound by the table's bytes: 16 x 64003 x 1024 12.9 us,
+// 5.3 TB/s with the scores; many by power, as the other products, and by their stores: 8192 x 64003 x 1024 to bf16 622 us,
+// 1.73 POP/s and 1.7 TB/s.
 struct ScoresEpilogue {
   struct Inputs {
     float sm, sn;
@@ -1007,7 +1011,7 @@ constexpr int TILE_M[5] = {64, 128, 256, 64, 128};
 // each K-step of 64, STEP + MORE for each workgroup that shares the compute unit, up to `slots` of them. Over 71 sizes of the
 // loss and the scores with each tile forced, what the estimate takes is 0.4 % slower than the fastest (8 % at most). The largest
 // tiles reach 1.3 PFLOP/s, those of 128 about 0.95, those of 64 about 0.65; the smaller ones fill the card sooner. The two
-// of 32-bit values, whose K-steps are of 32, are bound by their instructions alone (0.145 PFLOP/s of tiles of 128, 0.135 of 64).
+// of 32-bit values, whose K-steps are of 32, are bound by their instructions alone (0.14 PFLOP/s of tiles of 128, 0.13 of 64).
 constexpr int CUS = 256;  // the card's compute units, whatever device is asked: a workspace's size needs none
 constexpr double TILE_BASE[5] = {2.0, 3.0, 4.0, 2.0, 3.0}, TILE_STEP[5] = {0.45, 0.55, 1.5, 0.1, 0.0}, TILE_MORE[5] = {0.1, 0.27, 0.0, 0.45, 1.75};
 constexpr int TILE_SLOTS[5] = {4, 2, 1, 4, 2};

@@ -7,21 +7,23 @@
 //
 // What bounds the large products is power: with operands of random bits the card sustains 2.06 PFLOP/s of bf16
 // 16x16x32 and 1.77 of 32x32x16 (whose sums move twice the bits for each product; 8-bit: 4.04 and 3.40), all from
-// registers. So the small block is used, and bytes are moved as rarely as the registers allow: 128 x 64 a wave. At 1.29
-// PFLOP/s the matrix cores are busy 2/3 of the time at 1.87 GHz; without the loads to LDS (leaving all else) the same
-// instructions take 155 us instead of 216, without the LDS reads 195: what remains is moving operands. 80 % of the loads
-// hit L2, whose share of the rest is what the tile order leaves: each matrix once from behind it.
+// registers. So the small block is used, and bytes are moved as rarely as the registers allow: 128 x 64 a wave. What the
+// loop waits for was taken from a launch of dW alone, in one plane (8192 x 16128 x 1024 bf16, 216 us, 1.25 PFLOP/s): matrix
+// cores busy 2/3 of the time at 1.87 GHz; without the loads to LDS (leaving all else) 155 us, without the LDS reads 195:
+// what remains is moving operands. 80 % of the loads hit L2, whose share of the rest is what the tile order leaves: each
+// matrix once from behind it. 32-bit products are bound by their instructions: 0.14 PFLOP/s of 0.157.
 //
 // A K-step is 128 bytes of k (64 16-bit values, 32 32-bit ones, 128 8-bit ones) of every tile row. Operands are staged by
 // global_load_lds_dwordx4 (global memory to LDS without registers: lane i of the instruction fills 16 bytes
 // at base + 16 i, so what is permuted is the global address each lane reads) in two forms:
 //   ROWS  memory holds k contiguous in each row. LDS: [row][8 chunks of 16 bytes], chunk c of row r at place
 //         c ^ (r >> 1 & 7): 16 rows read at one c fill the 64 banks once.
-//   COLS  memory holds the tile's rows as columns: [k][m]. LDS: [k][m], 32-byte pieces of row k permuted by swizzle(k)
+//   COLS  memory holds the tile's rows as columns: [k][m]. LDS: [k][m], pieces of 16 values of row k permuted by swizzle(k)
 //         so that the 16 k-rows of a read spread over the banks; ds_read_b64_tr_b16 turns four k-rows of 16
-//         columns into four consecutive k of one column per lane: no transposed copy of a matrix is ever made.
-// k that passes the end: the last K-step reads the last valid chunk or row again; the caller sees to it that
-// the other operand holds zeros there.
+//         columns into four consecutive k of one column per lane (32-bit values are read one by one): no transposed copy
+//         of a matrix is ever made.
+// k that passes the end: the last K-step reads the last valid chunk or row again, against zeros that the caller sees to in
+// the other operand; of ROWS of floats in A what was read again is cleared.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -234,7 +236,7 @@ struct Tile {
 // A ring of S LDS stages: the loads of K-step t + S start when all waves have read the last of step t, and fly while the
 // steps between are multiplied. A K-step is four parts, (k half, half of the wave's rows): each part's fragments are read
 // from LDS while the part before is multiplied, also across the one barrier of a K-step.
-// Measured at 8192 x 16128 x 1024 bf16 (dW, 210 - 216 us as it is): K-steps of 64 bytes in rings of 3, 4 and 5 stages
+// Measured on that launch of dW (210 - 216 us as it is): K-steps of 64 bytes in rings of 3, 4 and 5 stages
 // 226 - 228 (twice the barriers; deeper prefetch gains nothing), two 256 x 128 workgroups a unit 252 (half as much again
 // through LDS), four waves of 128 x 128 224, blocks of 32 x 32 227, loads in one burst 222.
 // HALVES: operands that are sums of two planes, hi and lo, come in `products` runs through the same `range` of K-steps: of B alone
