@@ -248,7 +248,8 @@ const char* pst_head_error(void);
  *   targets [rows]  int32 or int64 (target_bits; uint32 token ids below 2^31 are int32 ids). Positions whose target is
  *                   `ignore` have loss 0; a target outside [0, vocab) that is not `ignore` gives loss NaN.
  *   loss, lse [rows] f32 (lse of ignored positions too). A logit of -infinity (a mask in the table) has probability 0;
- *                   one of +infinity or NaN makes its position's lse and loss NaN.
+ *                   one of +infinity or NaN makes its position's lse and loss NaN Where all are -infinity lse
+ *                   is -infinity and the loss NaN.
  * rows = 0 writes nothing. *_workspace: bytes of the 256-byte aligned device workspace that a call with these
  * arguments needs (negative: PST_E_*).
  */

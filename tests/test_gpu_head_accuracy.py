@@ -206,3 +206,23 @@ def test_pieces_of_the_positions(rows, vocab, width, dtype):
     assert none is None and torch.equal(a, dx)
     none, b = head.token_loss_grad(x, w, t, lse, gl, need_hidden=False)
     assert none is None and torch.equal(b, dw)
+
+
+# a position whose mask leaves no id: nothing to divide by, and it says so; the others do not notice
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("rows,vocab,width", [(3, 70, 64), (300, 700, 72), (1200, 2100, 100)])
+def test_a_mask_that_leaves_nothing(rows, vocab, width, dtype):
+    x, w, t, _ = make(rows, vocab, width, dtype, seed=7)
+    x, w = with_bias(x, w)
+    x[:, -1] = 0
+    whole_loss, whole_lse = head.token_loss(x, w, t)
+    w[:, -1] = -torch.inf
+    x[:, -1] = 1
+    loss, lse = head.token_loss(x, w, t)
+    assert (lse == -torch.inf).all() and loss[t != -100].isnan().all() and (loss[t == -100] == 0).all()
+    w[:, -1] = torch.where(torch.arange(vocab, device=DEV) % 2 == 0, -torch.inf, 0.0).to(dtype)
+    loss, lse = head.token_loss(x, w, t)
+    l = x[:, :-1].double() @ w[1::2, :-1].double().T
+    off = (x[:, :-1].double().abs() @ w[1::2, :-1].double().abs().T).amax(1) * U32 * (width + 2)
+    assert ((lse.double() - torch.logsumexp(l, 1)).abs() <= off + (200 + vocab / 1024) * U32 + 8 * U32 * (lse.abs() + 1)).all()
+    assert (loss[(t != -100) & (t % 2 == 0)] == torch.inf).all() and whole_loss.isfinite().all() and whole_lse.isfinite().all()
